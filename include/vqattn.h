@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define VQATTN_VERSION 202
+#define VQATTN_VERSION 203
 #define VQATTN_BLOCK 128   /* key/query block size; ops/attn_vq.py:23 BLOCK_SIZE ("MUST MATCH KERNEL") */
 #define VQATTN_MAX_DIMS 5
 
@@ -31,7 +31,8 @@ typedef enum VqDtype {
     VQ_U16 = 3,
     VQ_I32 = 4,
     VQ_I64 = 5,
-    VQ_F16 = 6   /* IEEE half: the dtype of the reference's own self-test (ops/attn_vq.py:534-556) */
+    VQ_F16 = 6,  /* IEEE half: the dtype of the reference's own self-test (ops/attn_vq.py:534-556) */
+    VQ_I8 = 7    /* rows of a paged cache in 8 bits, each with its own scale */
 } VqDtype;
 
 typedef enum VqStatus {
@@ -72,6 +73,8 @@ typedef enum VqPrefillImpl { VQ_IMPL_AUTO = 0, VQ_IMPL_SIMT = 1, VQ_IMPL_TENSOR 
 #define VQ_WORD_TIMEOUT 1       /* a bounded device-side wait expired            -> VQ_ETIMEOUT   */
 #define VQ_WORD_BAD_POSITION 2  /* vqattn_rope: position outside the cos/sin tables -> VQ_EINVAL_ARG */
 #define VQ_WORD_BAD_CODE 3      /* vqattn_cache_advance: code outside [0, K)       -> VQ_EINVAL_ARG */
+#define VQ_WORD_BAD_PAGE 4      /* vqattn_paged_*: page or snapshot outside its pool -> VQ_EINVAL_ARG */
+#define VQ_WORD_BAD_LENGTH 5    /* vqattn_paged_*: token counts and lengths that do not fit -> VQ_EINVAL_ARG */
 
 int vqattn_version(void);
 const char *vqattn_status_string(int status);
@@ -330,6 +333,86 @@ int vqattn_cache_advance(const VqTensorDesc *codes, const VqTensorDesc *v_new, i
 int vqattn_store_window(const VqTensorDesc *k1, const VqTensorDesc *k3, const VqTensorDesc *v, VqTensorDesc *k1_win,
                         VqTensorDesc *k3_win, VqTensorDesc *v_win, const VqTensorDesc *vsum_f32, VqTensorDesc *vsum_act_or_null,
                         void *stream);
+
+/*
+ * A cache in pages: the window rows of many sequences of different lengths in one pool (no counterpart in the reference, whose cache
+ * holds one length per batch, ops/attn_vq.py:31-173).  Token j of sequence s lies in page table[s][j / P] at row j % P; only the pages
+ * of live rows need an entry (rows before the boundary of a sequence's next query are in its per-code sums and are not read).
+ *   k1, k3, v  [NP,Hkv,P,D]  rotated keys, raw keys, values: f32 | bf16 | f16, or i8 with scales; P in {16,32,64,128}, D in {64,128}.
+ *              k3.ptr NULL: plain rotary positions, the rotated keys take the place of the raw ones.
+ *   *_scale    [NP,Hkv,P] f32 with i8 rows, ptr NULL otherwise.  An i8 row x of fp32 values is held as
+ *              scale = max|x| * (1/127), code = round_to_nearest_even(x * (1 / scale)), every operation rounded to fp32;
+ *              a scale below the normal numbers becomes 0 with codes 0; a row with a value that is not finite gets the scale NaN.
+ *   table      [S,MB] i32
+ *   cu_q       [S+1] i32     new tokens of sequence s: rows cu_q[s] .. cu_q[s+1]-1 of the packed tensors; rows from cu_q[S] on are
+ *                            left as they are.  A sequence may have none.
+ *   lens       [S] i32       tokens of sequence s, the new ones included (they are its last)
+ * Row and outer strides of the pools are free (multiples of 16 bytes; strides of scales: any).  table, cu_q and lens are read on the
+ * device: a captured call replays with the values they then hold.  Lengths that do not fit (cu_q decreasing or beyond the packed rows, more
+ * new tokens than tokens) leave that sequence out and raise VQ_WORD_BAD_LENGTH.  A page that is needed and lies outside the pool raises
+ * VQ_WORD_BAD_PAGE: nothing is read or written for it, and output rows that would need it are unspecified (finite or not).
+ */
+typedef struct VqPagedKv {
+    VqTensorDesc k1, k3, v;
+    VqTensorDesc k1_scale, k3_scale, v_scale;
+    VqTensorDesc table, cu_q, lens;
+} VqPagedKv;
+
+/*
+ * Appends the new tokens to their pages in one launch: k [T,Hkv,D] rotated to its position -> k1, as it is -> k3 (unless k3.ptr is
+ * NULL), v [T,Hkv,D] -> v, rounded to the pools' type or quantised to i8 (from the fp32 rotation, not from a rounded one).
+ * q [T,Hq,D] (ptr NULL: none) -> q1 [T,Hq,D] rotated to the tokens' positions, and q2 [T,Hq,D] (ptr NULL: none) rotated to const_pos.
+ * cos_tab / sin_tab [n_pos, D/2] f32 as for vqattn_rope; NULL: keys (and queries) are stored as they are.
+ * The pools' type is k's, or i8.  A position outside the tables raises VQ_WORD_BAD_POSITION and uses the nearest row.
+ */
+typedef struct VqPagedAppendArgs {
+    VqPagedKv kv;
+    VqTensorDesc k, v, q, q1, q2;
+    const float *cos_tab, *sin_tab;
+    int64_t n_pos, const_pos;
+    int32_t *status_word;
+} VqPagedAppendArgs;
+
+int vqattn_paged_append(const VqPagedAppendArgs *args, void *stream);
+
+/*
+ * Reads rows back, dense: out[i][s][h][r] = row start[s] + r of sequence s in pool i, r in [0, n); rows before 0 or at or behind lens[s]
+ * are zeros.  Up to three pools (pool[i].ptr NULL ends the list) of one type in one launch.
+ *   pool [NP,Hkv,P,D] f32 | bf16 | f16 | i8 (then scale [NP,Hkv,P] f32), table [S,MB] i32, start, lens [S] i32,
+ *   out [S,Hkv,n,D] dense f32 | bf16 | f16: the pool's type, or for i8 any of them: code * scale, rounded once more.
+ */
+typedef struct VqPagedReadArgs {
+    VqTensorDesc pool[3], scale[3], out[3];
+    VqTensorDesc table, start, lens;
+    int32_t *status_word;
+} VqPagedReadArgs;
+
+int vqattn_paged_read(const VqPagedReadArgs *args, void *stream);
+
+/*
+ * Attention of the new tokens over a paged cache that already holds them: row t of sequence s at position
+ * i = lens[s] - (cu_q[s+1] - cu_q[s]) + (t - cu_q[s]) gets what row i of vqattn_prefill over the whole sequence is defined to be, with
+ * boundary = max(0, ((i - window) / 128) * 128):
+ *   keys [max(0,i-window), i] scored q1.k1, keys [boundary, max(0,i-window)) scored q2.k3 (k3.ptr NULL: q2.k1), older keys through counts
+ *   and value sums per code of the snapshot of that boundary: snapshot snap_table[s][(boundary / 128) % MS] of cnt and vsum.
+ *   A decode therefore needs one column (the running aggregates), a chunk of c tokens (c - 1) / 128 + 2 of them at most.
+ *   q1, q2, out [T,Hq,D] f32 | bf16 | f16 (q2 may alias q1);  pools of that type or i8;
+ *   codebook [Hkv,MK,D], vsum [NS,Hkv,MK,D] of the activations' type, cnt [NS,Hkv,MK] f32, all dense, MK % 128 == 0;
+ *   snap_table [S,MS] i32 (boundary 0 has no snapshot).  codebook.ptr NULL: the local part only.
+ *   max_q: an upper bound of the new tokens of any sequence; a sequence with more is left out (VQ_WORD_BAD_LENGTH).
+ * Codes with cnt == 0 are excluded and their vsum rows must be finite.  Values of a sequence are expected to be finite; what lies behind its
+ * end in its last page may be anything.
+ */
+typedef struct VqPagedAttentionArgs {
+    VqPagedKv kv;
+    VqTensorDesc q1, q2, out;
+    VqTensorDesc codebook, cnt, vsum, snap_table;
+    int64_t window, max_q;
+    float scale;           /* <= 0: 1/sqrt(D) */
+    int32_t *status_word;
+} VqPagedAttentionArgs;
+
+int vqattn_paged_attention(const VqPagedAttentionArgs *args, void *stream);
 
 #ifdef __cplusplus
 }

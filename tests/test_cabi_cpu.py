@@ -90,3 +90,83 @@ def test_api_refuses_cpu_tensors():
     from vqtree_b200 import api
     with pytest.raises(ValueError):
         api.assign_codes(torch.zeros(1, 1, 128, 64), torch.zeros(1, 1, 128, 64))
+
+
+def test_paged_entry_points_refuse_bad_arguments_without_a_device():
+    native = _native()
+    lib, desc = native.lib, native.desc
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
+
+    def append(**kw):
+        t = dict(k1=torch.zeros(4, 2, 16, 64), k3=torch.zeros(4, 2, 16, 64), v_pool=torch.zeros(4, 2, 16, 64), table=i32(3, 5), cu_q=i32(4), lens=i32(3),
+                 k=torch.zeros(7, 2, 64), v=torch.zeros(7, 2, 64), q=None, q1=None, q2=None, k1_scale=None, v_scale=None, k3_scale=None)
+        tab = torch.zeros(32, 32)
+        extra = dict(cos=tab.data_ptr(), sin=tab.data_ptr(), n_pos=32, const_pos=0)
+        t.update({k: v for k, v in kw.items() if k in t})
+        extra.update({k: v for k, v in kw.items() if k in extra})
+        a = native.VqPagedAppendArgs()
+        for name in ("k1", "k3", "table", "cu_q", "lens", "k1_scale", "v_scale", "k3_scale"):
+            desc(t[name], getattr(a.kv, name))
+        desc(t["v_pool"], a.kv.v)
+        for name in ("k", "v", "q", "q1", "q2"):
+            desc(t[name], getattr(a, name))
+        a.cos_tab, a.sin_tab, a.n_pos, a.const_pos = extra["cos"], extra["sin"], extra["n_pos"], extra["const_pos"]
+        return lib.vqattn_paged_append(ctypes.byref(a), None)
+
+    z = torch.zeros
+    assert append() == -4                                           # host tensors
+    assert append(k=None) == -7 and append(k1=None) == -7 and append(v_pool=None) == -7
+    assert append(k=z(7, 2, 64, dtype=torch.int32)) == -2 and append(k=z(7, 2, 64, dtype=torch.bfloat16)) == -2
+    assert append(v=z(7, 3, 64)) == -1 and append(v=z(6, 2, 64)) == -1 and append(k=z(7, 2)) == -1
+    assert append(v_pool=z(4, 2, 32, 64)) == -1 and append(k3=z(5, 2, 16, 64)) == -1
+    assert append(k1=z(4, 2, 24, 64), k3=z(4, 2, 24, 64), v_pool=z(4, 2, 24, 64)) == -8      # page size
+    assert append(k1=z(4, 2, 16, 32), k3=z(4, 2, 16, 32), v_pool=z(4, 2, 16, 32), k=z(7, 2, 32), v=z(7, 2, 32)) == -8
+    assert append(k1=z(4, 2, 64, 16).transpose(2, 3)) == -3
+    assert append(cu_q=i32(3)) == -1 and append(cu_q=z(4)) == -2 and append(lens=i32(4)) == -1 and append(table=z(3, 5)) == -2
+    assert append(sin=None) == -7 and append(n_pos=0) == -7
+    q = dict(q=z(7, 4, 64), q1=z(7, 4, 64))
+    assert append(**q) == -4 and append(q=q["q"]) == -7 and append(q=q["q"], q1=z(7, 2, 64)) == -1
+    assert append(**q, q2=z(7, 4, 64), const_pos=32) == -7 and append(**q, q2=z(7, 4, 64), const_pos=31) == -4
+    assert append(k=z(7, 2, 65)[:, :, 1:]) == -3                    # rows that do not start on 16 bytes
+    i8 = lambda: z(4, 2, 16, 64, dtype=torch.int8)
+    sc = lambda: z(4, 2, 16)
+    assert append(k1=i8(), k3=i8(), v_pool=i8()) == -7              # scales missing
+    assert append(k1=i8(), k3=i8(), v_pool=i8(), k1_scale=sc(), k3_scale=sc(), v_scale=z(4, 2, 8)) == -1
+    assert append(k1=i8(), k3=i8(), v_pool=i8(), k1_scale=sc(), k3_scale=sc(), v_scale=sc()) == -4
+    assert append(v_scale=sc()) == -7                               # scales of rows that have none
+
+    def read(pool, out, scale=None, table=i32(3, 5), start=i32(3), lens=i32(3)):
+        a = native.VqPagedReadArgs()
+        desc(pool, a.pool[0]); desc(out, a.out[0]); desc(scale, a.scale[0])
+        desc(table, a.table); desc(start, a.start); desc(lens, a.lens)
+        return lib.vqattn_paged_read(ctypes.byref(a), None)
+
+    assert read(z(4, 2, 16, 64), z(3, 2, 9, 64)) == -4
+    assert read(None, z(3, 2, 9, 64)) == -7 and read(z(4, 2, 16, 64), None) != 0
+    assert read(z(4, 2, 16, 64), z(3, 2, 9, 64, dtype=torch.float16)) == -2 and read(z(4, 2, 16, 64, dtype=torch.int32), z(3, 2, 9, 64)) == -2
+    assert read(z(4, 2, 16, 64), z(2, 2, 9, 64)) == -1 and read(z(4, 2, 16, 64), z(3, 2, 64, 9).transpose(2, 3)) == -3
+    assert read(i8(), z(3, 2, 9, 64)) == -7 and read(i8(), z(3, 2, 9, 64), sc()) == -4
+
+    def attend(**kw):
+        t = dict(k1=z(4, 2, 16, 64), k3=z(4, 2, 16, 64), v=z(4, 2, 16, 64), table=i32(3, 5), cu_q=i32(4), lens=i32(3), q1=z(7, 4, 64), q2=z(7, 4, 64),
+                 out=z(7, 4, 64), codebook=z(2, 128, 64), cnt=z(5, 2, 128), vsum=z(5, 2, 128, 64), snap_table=i32(3, 2))
+        s = dict(window=128, max_q=7)
+        t.update({k: v for k, v in kw.items() if k in t})
+        s.update({k: v for k, v in kw.items() if k in s})
+        a = native.VqPagedAttentionArgs()
+        for name in ("k1", "k3", "v", "table", "cu_q", "lens"):
+            desc(t[name], getattr(a.kv, name))
+        for name in ("q1", "q2", "out", "codebook", "cnt", "vsum", "snap_table"):
+            desc(t[name], getattr(a, name))
+        a.window, a.max_q = s["window"], s["max_q"]
+        return lib.vqattn_paged_attention(ctypes.byref(a), None)
+
+    assert lib.vqattn_paged_attention(None, None) == -7 and lib.vqattn_paged_append(None, None) == -7 and lib.vqattn_paged_read(None, None) == -7
+    assert attend() == -4 and attend(codebook=None) == -4
+    assert attend(window=100) == -7 and attend(window=0) == -7 and attend(max_q=0) == -7
+    assert attend(q1=z(7, 3, 64), q2=z(7, 3, 64), out=z(7, 3, 64)) == -1      # 3 query heads over 2
+    assert attend(q2=z(7, 4, 64, dtype=torch.float16)) == -2 and attend(out=None) == -7 and attend(out=z(8, 4, 64)) == -1
+    assert attend(codebook=z(2, 100, 64), cnt=z(5, 2, 100), vsum=z(5, 2, 100, 64)) == -8
+    assert attend(cnt=z(4, 2, 128)) == -1 and attend(cnt=None) == -7 and attend(snap_table=i32(2, 2)) == -1 and attend(snap_table=z(3, 2)) == -2
+    assert attend(vsum=z(5, 2, 64, 128).transpose(2, 3)) == -3
+    assert attend(q1=z(7, 258, 64), q2=z(7, 258, 64), out=z(7, 258, 64)) == -8   # more than 128 query heads per kv head

@@ -9,12 +9,13 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import native
-from .native import BLOCK, VqDecodeArgs, VqPrefillArgs, check, desc, lib, stream_ptr
+from .native import (BLOCK, VqDecodeArgs, VqPagedAppendArgs, VqPagedAttentionArgs, VqPagedReadArgs, VqPrefillArgs, check, desc, lib,
+                     stream_ptr)
 
 _IMPL = {"auto": native.IMPL_AUTO, "simt": native.IMPL_SIMT, "tensor": native.IMPL_TENSOR}
 
@@ -154,6 +155,7 @@ def build_aggregates(codes: torch.Tensor, v: torch.Tensor, K: int, nb: Optional[
 
 
 _ROPE_TABLES = {}
+_ROPE_REPLACED = []     # tables that a longer one replaced: a captured graph may still read them (together they are shorter than the longest)
 
 
 def rope_tables(n_pos: int, dim: int, device, base: float = 10000.0):
@@ -165,6 +167,8 @@ def rope_tables(n_pos: int, dim: int, device, base: float = 10000.0):
         n = max(n_pos, 2 * have[0].shape[0] if have is not None else 0)
         inv = 1.0 / (base ** (torch.arange(0, dim, 2, dtype=torch.float64, device=dev) / dim))
         ang = torch.outer(torch.arange(n, dtype=torch.float64, device=dev), inv)
+        if have is not None:
+            _ROPE_REPLACED.append(have)
         have = _ROPE_TABLES[key] = (ang.cos().float().contiguous(), ang.sin().float().contiguous())
     return have
 
@@ -443,6 +447,130 @@ def store_window(k1, k3, v, k1_win, k3_win, v_win, vsum_f32=None, vsum_act=None)
     with torch.cuda.device(dev):
         check(lib.vqattn_store_window(desc(k1), desc(k3), desc(v), desc(k1_win), desc(k3_win), desc(v_win), desc(vsum_f32), desc(vsum_act),
                                       stream_ptr(dev)), "vqattn_store_window")
+
+
+# ---------------------------------------------------------------------------------------------
+# A cache in pages: sequences of different lengths, new tokens in chunks of any length, rows of 16 (32) or 8 bits.
+
+class PagedKV(NamedTuple):
+    """The pools of a paged cache: rotated keys, values and (ReRoPE) raw keys [NP,Hkv,P,D], pages of P = 16, 32, 64 or 128 tokens, in
+    the activations' type or int8 with a scale per row [NP,Hkv,P] f32.  k3 None: plain rotary positions.  Any strides that are
+    multiples of 16 bytes with a contiguous last dim ([NP,P,Hkv,D] storage viewed as [NP,Hkv,P,D], a slice of a pool of all layers)."""
+    k1: torch.Tensor
+    v: torch.Tensor
+    k3: Optional[torch.Tensor] = None
+    k1_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+    k3_scale: Optional[torch.Tensor] = None
+
+    @classmethod
+    def allocate(cls, num_pages: int, Hkv: int, page_size: int, D: int, dtype: torch.dtype, device, raw_keys: bool = True) -> "PagedKV":
+        """Pools of ``num_pages`` pages; dtype torch.int8 allocates the scales too."""
+        pool = lambda: torch.zeros(num_pages, Hkv, page_size, D, dtype=dtype, device=device)
+        scale = lambda: torch.zeros(num_pages, Hkv, page_size, dtype=torch.float32, device=device) if dtype == torch.int8 else None
+        return cls(pool(), pool(), pool() if raw_keys else None, scale(), scale(), scale() if raw_keys else None)
+
+
+def _paged_kv(kv, pages: PagedKV, block_table, cu_q, seq_lens) -> None:
+    for name, t in zip(("k1", "v", "k3", "k1_scale", "v_scale", "k3_scale"), pages):
+        desc(t, getattr(kv, name))
+    desc(block_table, kv.table)
+    desc(cu_q, kv.cu_q)
+    desc(seq_lens, kv.lens)
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, pages: PagedKV, block_table: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor,
+                 q: Optional[torch.Tensor] = None, const_pos: Optional[int] = None, rotate: bool = True, base: float = 10000.0,
+                 n_pos: Optional[int] = None):
+    """New tokens into their pages, in one launch: k [T,Hkv,D] rotated to its position -> k1, as it is -> k3, v [T,Hkv,D] -> v, rounded to
+    the pools' type or quantised to int8 rows with a scale.  q [T,Hq,D] (optional) is rotated on the way: returns (q1, q2), q2 rotated to
+    ``const_pos`` (None without one).
+
+    block_table int32 [S,MB]: page of tokens [P*c, P*(c+1)) of a sequence; cu_q int32 [S+1]: sequence s brings rows cu_q[s] ..
+    cu_q[s+1]-1; seq_lens int32 [S]: its length with them.  rotate=False stores keys (and returns queries) as they are.
+    n_pos: an upper bound of the positions + 1 (None: what the table can address)."""
+    dev = _require_cuda(k, v, *pages, block_table, cu_q, seq_lens, q)
+    T, _, D = k.shape
+    new = lambda: torch.empty(q.shape, dtype=q.dtype, device=dev)
+    q1 = new() if q is not None else None
+    q2 = new() if q is not None and const_pos is not None else None
+    if T == 0:
+        return q1, q2
+    a = VqPagedAppendArgs()
+    _paged_kv(a.kv, pages, block_table, cu_q, seq_lens)
+    for name, t in (("k", k), ("v", v), ("q", q), ("q1", q1), ("q2", q2)):
+        desc(t, getattr(a, name))
+    if rotate:
+        n = n_pos if n_pos is not None else block_table.shape[1] * pages.k1.shape[2]
+        cos, sin = rope_tables(max(n, (const_pos or 0) + 1), D, dev, base)
+        a.cos_tab, a.sin_tab, a.n_pos = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    a.const_pos = int(const_pos or 0)
+    a.status_word = device_status_word(dev).data_ptr()
+    with torch.cuda.device(dev):
+        check(lib.vqattn_paged_append(ctypes.byref(a), stream_ptr(dev)), "vqattn_paged_append")
+    return q1, q2
+
+
+def paged_read(pools, block_table: torch.Tensor, starts: torch.Tensor, seq_lens: torch.Tensor, n: int,
+               out_dtype: Optional[torch.dtype] = None):
+    """Rows [starts[s], starts[s] + n) of every sequence out of its pages, dense: a list of [S,Hkv,n,D], one per pool; rows before 0 or at
+    or behind seq_lens[s] are zeros.
+
+    pools: up to three pairs (pool, scale or None) of one type; starts, seq_lens int32 [S].  out_dtype: type of the values of an int8
+    pool (default float32)."""
+    pools = [p if isinstance(p, tuple) else (p, None) for p in pools]
+    if not 1 <= len(pools) <= 3:
+        raise ValueError("one to three pools")
+    dev = _require_cuda(*(t for p in pools for t in p), block_table, starts, seq_lens)
+    first = pools[0][0]
+    dt = out_dtype or (torch.float32 if first.dtype == torch.int8 else first.dtype)
+    S = block_table.shape[0]
+    outs = [torch.empty((S, first.shape[1], n, first.shape[3]), dtype=dt, device=dev) for _ in pools]
+    if S == 0 or n == 0:
+        return outs
+    a = VqPagedReadArgs()
+    for i, ((pool, scale), out) in enumerate(zip(pools, outs)):
+        desc(pool, a.pool[i])
+        desc(scale, a.scale[i])
+        desc(out, a.out[i])
+    desc(block_table, a.table)
+    desc(starts, a.start)
+    desc(seq_lens, a.lens)
+    a.status_word = device_status_word(dev).data_ptr()
+    with torch.cuda.device(dev):
+        check(lib.vqattn_paged_read(ctypes.byref(a), stream_ptr(dev)), "vqattn_paged_read")
+    return outs
+
+
+def paged_attention(q1: torch.Tensor, q2: torch.Tensor, pages: PagedKV, block_table: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor,
+                    window: int, max_q: int, codebook: Optional[torch.Tensor] = None, cnt: Optional[torch.Tensor] = None,
+                    vsum: Optional[torch.Tensor] = None, snap_table: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the new tokens of S sequences over their pages (which hold them already): every row is what the same row of
+    ``vq_attention_prefill`` over the whole sequence is defined to be.
+
+    q1, q2 [T,Hq,D] (q2 may be q1) packed by cu_q; block_table, cu_q, seq_lens as in ``paged_append``; max_q: an upper bound of the new
+    tokens of one sequence.  codebook [Hkv,MK,D], cnt [NS,Hkv,MK] f32, vsum [NS,Hkv,MK,D], snap_table int32 [S,MS]: keys before the
+    boundary b of a query count through snapshot ``snap_table[s, b // 128 % MS]`` (None: the local part only).  Returns [T,Hq,D]; rows
+    from cu_q[S] on are left as they are."""
+    far = (codebook, cnt, vsum, snap_table)
+    if codebook is not None and any(t is None for t in far):
+        raise ValueError("codebook, cnt, vsum and snap_table go together")
+    dev = _require_cuda(q1, q2, *pages, block_table, cu_q, seq_lens, *far, out)
+    if out is None:
+        out = torch.empty(q1.shape, dtype=q1.dtype, device=dev)
+    if q1.shape[0] == 0:
+        return out
+    a = VqPagedAttentionArgs()
+    _paged_kv(a.kv, pages, block_table, cu_q, seq_lens)
+    for name, t in zip(("q1", "q2", "out", "codebook", "cnt", "vsum", "snap_table"), (q1, q2, out) + (far if codebook is not None else (None,) * 4)):
+        desc(t, getattr(a, name))
+    a.window, a.max_q = int(window), int(max_q)
+    a.scale = float(scale) if scale else 0.0
+    a.status_word = device_status_word(dev).data_ptr()
+    with torch.cuda.device(dev):
+        check(lib.vqattn_paged_attention(ctypes.byref(a), stream_ptr(dev)), "vqattn_paged_attention")
+    return out
 
 
 # ---------------------------------------------------------------------------------------------

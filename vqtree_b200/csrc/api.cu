@@ -36,7 +36,9 @@ extern "C" int vqattn_status_from_word(int32_t word)
     case 0: return VQ_OK;
     case VQ_WORD_TIMEOUT: return VQ_ETIMEOUT;
     case VQ_WORD_BAD_POSITION:
-    case VQ_WORD_BAD_CODE: return VQ_EINVAL_ARG;
+    case VQ_WORD_BAD_CODE:
+    case VQ_WORD_BAD_PAGE:
+    case VQ_WORD_BAD_LENGTH: return VQ_EINVAL_ARG;
     default: return VQ_ELAUNCH;
     }
 }

@@ -15,8 +15,8 @@ _LIB_PATH = Path(__file__).resolve().parent / "lib" / "libvqattn.so"
 MAX_DIMS = 5
 BLOCK = 128
 
-VQ_F32, VQ_BF16, VQ_U8, VQ_U16, VQ_I32, VQ_I64, VQ_F16 = range(7)
-WORD_TIMEOUT, WORD_BAD_POSITION, WORD_BAD_CODE = 1, 2, 3
+VQ_F32, VQ_BF16, VQ_U8, VQ_U16, VQ_I32, VQ_I64, VQ_F16, VQ_I8 = range(8)
+WORD_TIMEOUT, WORD_BAD_POSITION, WORD_BAD_CODE, WORD_BAD_PAGE, WORD_BAD_LENGTH = 1, 2, 3, 4, 5
 IMPL_AUTO, IMPL_SIMT, IMPL_TENSOR = 0, 1, 2
 
 _DTYPES = {
@@ -27,6 +27,7 @@ _DTYPES = {
     torch.uint16: VQ_U16,
     torch.int32: VQ_I32,
     torch.int64: VQ_I64,
+    torch.int8: VQ_I8,
 }
 
 EXPORTS = (
@@ -37,6 +38,7 @@ EXPORTS = (
     "vqattn_assign_workspace_bytes", "vqattn_assign_codes_ws", "vqattn_rope",
     "vqattn_status_from_word", "vqattn_set_wait_limit_cycles", "vqattn_wait_selftest", "vqattn_rope_qk",
     "vqattn_decode_append", "vqattn_decode_step", "vqattn_store_window",
+    "vqattn_paged_append", "vqattn_paged_read", "vqattn_paged_attention",
 )
 
 
@@ -77,6 +79,26 @@ class VqDecodeStepArgs(ctypes.Structure):
                 ("pos", ctypes.c_int64), ("cos_tab", ctypes.c_void_p), ("sin_tab", ctypes.c_void_p), ("n_pos", ctypes.c_int64),
                 ("const_pos", ctypes.c_int64), ("q1", VqTensorDesc), ("q2", VqTensorDesc), ("row", ctypes.c_int64),
                 ("decode", VqDecodeArgs)]
+
+
+class VqPagedKv(ctypes.Structure):
+    _fields_ = [(n, VqTensorDesc) for n in ("k1", "k3", "v", "k1_scale", "k3_scale", "v_scale", "table", "cu_q", "lens")]
+
+
+class VqPagedAppendArgs(ctypes.Structure):
+    _fields_ = [("kv", VqPagedKv)] + [(n, VqTensorDesc) for n in ("k", "v", "q", "q1", "q2")] + [
+        ("cos_tab", ctypes.c_void_p), ("sin_tab", ctypes.c_void_p), ("n_pos", ctypes.c_int64), ("const_pos", ctypes.c_int64),
+        ("status_word", ctypes.c_void_p)]
+
+
+class VqPagedReadArgs(ctypes.Structure):
+    _fields_ = [(n, VqTensorDesc * 3) for n in ("pool", "scale", "out")] + [(n, VqTensorDesc) for n in ("table", "start", "lens")] + [
+        ("status_word", ctypes.c_void_p)]
+
+
+class VqPagedAttentionArgs(ctypes.Structure):
+    _fields_ = [("kv", VqPagedKv)] + [(n, VqTensorDesc) for n in ("q1", "q2", "out", "codebook", "cnt", "vsum", "snap_table")] + [
+        ("window", ctypes.c_int64), ("max_q", ctypes.c_int64), ("scale", ctypes.c_float), ("status_word", ctypes.c_void_p)]
 
 
 def _load() -> ctypes.CDLL:
@@ -123,6 +145,9 @@ def _load() -> ctypes.CDLL:
                                          P(VqTensorDesc), P(VqTensorDesc), P(VqTensorDesc), P(VqTensorDesc), ctypes.c_int64,
                                          ctypes.c_void_p, ctypes.c_void_p]
     lib.vqattn_decode_step.argtypes = [P(VqDecodeStepArgs), ctypes.c_void_p]
+    lib.vqattn_paged_append.argtypes = [P(VqPagedAppendArgs), ctypes.c_void_p]
+    lib.vqattn_paged_read.argtypes = [P(VqPagedReadArgs), ctypes.c_void_p]
+    lib.vqattn_paged_attention.argtypes = [P(VqPagedAttentionArgs), ctypes.c_void_p]
     lib.vqattn_status_from_word.argtypes = [ctypes.c_int32]
     lib.vqattn_set_wait_limit_cycles.argtypes = [ctypes.c_int64]
     lib.vqattn_set_wait_limit_cycles.restype = ctypes.c_int64
