@@ -35,4 +35,7 @@ struct PagedAttnParams {
     }
 };
 
+constexpr int kFewRows = 32;     // query rows (tokens times query heads of a kv head) of the few-token kernel
+int launch_paged_few(const PagedAttnParams &p, int dtype, bool q8, cudaStream_t stream);
+
 }  // namespace vq

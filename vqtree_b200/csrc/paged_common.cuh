@@ -44,7 +44,7 @@ struct PagedSeqs {
         q = __ldg(cu_q + s + 1) - t0;
         n = __ldg(lens + s);
         if (q == 0) return true;
-        if (t0 >= 0 && q > 0 && t0 + static_cast<int64_t>(q) <= T && q <= n && q <= max_q) return true;
+        if (t0 >= 0 && q > 0 && t0 + static_cast<int64_t>(q) <= T && q <= n && q <= max_q && n <= static_cast<int64_t>(MB) << log_p) return true;
         raise(VQ_WORD_BAD_LENGTH);
         return false;
     }
@@ -145,7 +145,7 @@ inline int check_paged_kv(const VqPagedKv &kv, int64_t T, int32_t *status, Paged
     if ((st = check_basic(&kv.table, 2)) != VQ_OK) return st;
     if (kv.table.dtype != VQ_I32) return VQ_EINVAL_DTYPE;
     const int64_t S = kv.table.shape[0];
-    if (S > (1 << 20) || kv.table.shape[1] > (1 << 24) || T > 0x7fffffff) return VQ_EUNSUPPORTED;
+    if (S > (1 << 20) || kv.table.shape[1] > (1 << 30) / shape[2] || T > 0x7fffffff) return VQ_EUNSUPPORTED;   // positions stay below 2^30
     if ((st = check_i32(kv.cu_q, S + 1)) != VQ_OK) return st;
     if ((st = check_i32(kv.lens, S)) != VQ_OK) return st;
     p.seqs = PagedSeqs{static_cast<const int32_t *>(kv.table.ptr), kv.table.stride[0], static_cast<int>(kv.table.shape[1]),
