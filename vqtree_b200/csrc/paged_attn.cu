@@ -234,6 +234,6 @@ extern "C" int vqattn_paged_attention(const VqPagedAttentionArgs *a, void *strea
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv.dtype == VQ_I8;
     if (is_16bit(dt) && static_cast<int64_t>(p.max_q) * G <= kFewRows) return launch_paged_few(p, dt, q8, s);
-    if (dt == VQ_F32) return launch_simt_kv<float>(p, q8, s);
-    return dt == VQ_F16 ? launch_simt_kv<__half>(p, q8, s) : launch_simt_kv<__nv_bfloat16>(p, q8, s);
+    if (is_16bit(dt)) return launch_paged_chunk(p, dt, q8, s);
+    return launch_simt_kv<float>(p, q8, s);
 }

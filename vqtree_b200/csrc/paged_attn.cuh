@@ -37,5 +37,6 @@ struct PagedAttnParams {
 
 constexpr int kFewRows = 32;     // query rows (tokens times query heads of a kv head) of the few-token kernel
 int launch_paged_few(const PagedAttnParams &p, int dtype, bool q8, cudaStream_t stream);
+int launch_paged_chunk(const PagedAttnParams &p, int dtype, bool q8, cudaStream_t stream);
 
 }  // namespace vq

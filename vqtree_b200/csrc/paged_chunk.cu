@@ -1,0 +1,765 @@
+// Attention over a paged cache for chunks of new tokens, on the sm_100a tensor cores.
+//
+// One CTA owns up to 128 query rows of one kv head - its G query heads times 128 / G tokens of one sequence, all in one 128-block of positions,
+// so that they share a boundary and every tile of keys and values is fetched once for all heads of the group - and walks their
+// work items with one online softmax: codebook tiles against the boundary's snapshot, the boundary block (raw keys, then rotated ones), the
+// blocks between, the causal block.  The softmax protocol is that of the prefill kernel with 128-key steps (prefill_tc4.cu): score buffers in
+// tensor memory that P overwrites, one thread per row and buffer, a reference maximum handed from step to step, lazily raised.
+// Which rows a tile has is read on the device (one warp counts the tiles of 32 sequences at a time), so a captured call may be
+// replayed with other lengths.
+//   16-bit rows   a thread loads pages by TMA, 128 / P boxes a tile; three softmax warpgroups, a ring of three 32 KB slots.
+//   8-bit rows    a warpgroup fetches the codes, turns them into 16-bit floats (exact) and writes them in the swizzled layout the tensor
+//                 cores read; the scales of a step's keys multiply scores, those of its values weights, per column.  Two softmax
+//                 warpgroups, a ring of four.
+// Rows behind a sequence's end hold anything: their scores are masked and their value rows are zeroed before the product.
+#include "codes8.cuh"
+#include "paged_attn.cuh"
+#include "tc_softmax.cuh"
+
+namespace vq {
+
+constexpr int kChunkPages = 256;        // page table entries of a tile kept in shared memory; the rest is read where it is needed
+
+template <int D, bool Q8>
+struct ChunkCfg {
+    static constexpr int kBufs = Q8 ? 2 : 3;                  // S/P buffers = softmax warpgroups
+    static constexpr int kSoft = 4 * kBufs;                   // softmax warps
+    static constexpr int kLoad = Q8 ? 4 : 1;                  // loading warps
+    static constexpr int kWarpMma = kSoft, kWarpLoad = kSoft + 1;
+    static constexpr int kThreads = (kSoft + 1 + kLoad) * 32;
+    static constexpr int NH = D / 64;
+    static constexpr int kTile = NH * kHalfBytes;             // 128 x D
+    static constexpr int kSlots = Q8 ? 4 : 3;
+    static constexpr int kQ = 0, kRing = 2 * kTile;
+    static constexpr int kTotal = kRing + kSlots * kTile + 1024;   // + slack for 1024-byte alignment
+    static constexpr uint32_t kColS = 0, kColO = kBlock * kBufs, kCols = 512;
+    static constexpr int kOq = D / 2;
+    static constexpr int kScal = Q8 ? 4 : 1;                  // steps whose scales are in flight
+};
+
+struct ChunkParams {
+    PagedAttnParams a;
+    int TQ;                      // tokens per tile
+};
+
+struct ChunkTile {
+    int s, t0, ntok, pos0, n, snap;
+};
+
+// The tile's items, in order: codebook tiles, boundary block (ReRoPE: two masked passes), blocks between, causal block.
+struct ChunkWork {
+    int kb0, n_far, n_bd, first_full, n_full, n_items, rerope;
+    __device__ __forceinline__ ChunkWork(const PagedAttnParams &p, const ChunkTile &t)
+    {
+        const int m = t.pos0 / kBlock;
+        rerope = p.rerope;
+        kb0 = m - p.W / kBlock;
+        n_far = t.snap >= 0 ? p.MK / kBlock : 0;
+        n_bd = kb0 >= 0 ? (rerope ? 2 : 1) : 0;
+        first_full = kb0 >= 0 ? kb0 + 1 : 0;
+        n_full = m - first_full;
+        n_items = n_far + n_bd + n_full + 1;
+    }
+    __device__ __forceinline__ int kind(int it) const
+    {
+        if (it < n_far) return kFar;
+        it -= n_far;
+        if (it < n_bd) return rerope ? (it == 0 ? kBdA : kBdB) : kFull;
+        return it - n_bd < n_full ? kFull : kDiag;
+    }
+    __device__ __forceinline__ int block(int it) const
+    {
+        if (it < n_far) return it;
+        it -= n_far;
+        return it < n_bd ? kb0 : first_full + it - n_bd;
+    }
+};
+
+// Tile number -> sequence and tokens, by one warp.  False: there are fewer tiles.
+__device__ __forceinline__ bool chunk_find(const PagedAttnParams &p, int TQ, int tile, ChunkTile &out)
+{
+    const int lane = threadIdx.x & 31, per = (kBlock + TQ - 1) / TQ;
+    int before = 0;
+    for (int base = 0; base < p.seqs.S; base += 32) {
+        int t0 = 0, q = 0, n = 0, cnt = 0;
+        if (base + lane < p.seqs.S && p.seqs.seq(base + lane, t0, q, n, p.max_q) && q > 0) {
+            const int i0 = n - q, nb = (n - 1) / kBlock - i0 / kBlock + 1;
+            cnt = nb == 1 ? (q + TQ - 1) / TQ
+                          : (kBlock - i0 % kBlock + TQ - 1) / TQ + (nb - 2) * per + ((n - 1) % kBlock + TQ) / TQ;
+        }
+        int sum = cnt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(~0u, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned mine = __ballot_sync(~0u, before + sum > tile);
+        if (mine) {
+            const int l = __ffs(mine) - 1;
+            int x = tile - before - (__shfl_sync(~0u, sum, l) - __shfl_sync(~0u, cnt, l));   // tile of the sequence
+            t0 = __shfl_sync(~0u, t0, l);
+            q = __shfl_sync(~0u, q, l);
+            n = __shfl_sync(~0u, n, l);
+            int i0 = n - q;
+            const int head = (min(kBlock - i0 % kBlock, q) + TQ - 1) / TQ;                   // tiles of its first block
+            int blk = i0 / kBlock;
+            if (x >= head) {
+                x -= head;
+                blk += 1 + x / per;
+                x %= per;
+            }
+            const int lo = max(i0, blk * kBlock) + x * TQ, hi = min(min(n, (blk + 1) * kBlock), lo + TQ);
+            out.s = base + l;
+            out.t0 = t0 + lo - i0;
+            out.ntok = hi - lo;
+            out.pos0 = lo;
+            out.n = n;
+            out.snap = p.snapshot(out.s, p.boundary(lo));
+            return true;
+        }
+        before += __shfl_sync(~0u, sum, 31);
+    }
+    return false;
+}
+
+__device__ __forceinline__ void fmul2(float &d0, float &d1, float a0, float a1, float b0, float b1)
+{
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
+// 8-bit rows: scores of 64 columns in log2 units (ks: scale of each key times the softmax scale), excluded ones -inf
+__device__ __forceinline__ void q8_scores(uint32_t s_addr, int kind, int lo, int hi, const float *ks, uint32_t (&r)[64])
+{
+    tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+    tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+    tc_wait_ld();
+#pragma unroll
+    for (int c = 0; c < 64; c += 4) {
+        const float4 k = *reinterpret_cast<const float4 *>(ks + c);
+        float x0, x1, x2, x3;
+        fmul2(x0, x1, __uint_as_float(r[c]), __uint_as_float(r[c + 1]), k.x, k.y);
+        fmul2(x2, x3, __uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]), k.z, k.w);
+        r[c] = __float_as_uint(x0); r[c + 1] = __float_as_uint(x1); r[c + 2] = __float_as_uint(x2); r[c + 3] = __float_as_uint(x3);
+    }
+    if (kind != kFull) t4_mask_range(r, lo, hi);
+}
+// weights times value scales (vs), packed; returns sum plus the weights
+template <bool F16>
+__device__ __forceinline__ float q8_exp(const uint32_t (&r)[64], uint32_t p_addr, bool masked, const float *vs, float neg_m, float sum)
+{
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t pk[16];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = 32 * half + 4 * j;
+            const float4 v4 = *reinterpret_cast<const float4 *>(vs + c);
+            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float r0 = __uint_as_float(r[c + 2 * i]), r1 = __uint_as_float(r[c + 2 * i + 1]);
+                float t0, t1, w0, w1;
+                fadd2(t0, t1, r0, r1, neg_m, neg_m);
+                const float p0 = ex2(t0), p1 = ex2(t1);
+                fadd2(ls[2 * i], ls[2 * i + 1], ls[2 * i], ls[2 * i + 1], p0, p1);
+                fmul2(w0, w1, p0, p1, v[2 * i], v[2 * i + 1]);
+                if (masked) {                                 // a value that is not finite must not reach rows that do not see it
+                    if (r0 == -INFINITY) w0 = 0.f;
+                    if (r1 == -INFINITY) w1 = 0.f;
+                }
+                pk[2 * j + i] = pack16<F16>(w0, w1);
+            }
+        }
+        tmem_st16(p_addr + 16 * half, pk);
+        sum += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    }
+    return sum;
+}
+
+template <int D, bool F16, bool Q8>
+__global__ void __launch_bounds__(ChunkCfg<D, Q8>::kThreads, 1)
+paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_constant__ CUtensorMap tm_q2, const __grid_constant__ CUtensorMap tm_k1,
+                   const __grid_constant__ CUtensorMap tm_k3, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_cb,
+                   const __grid_constant__ CUtensorMap tm_vs, const ChunkParams cp)
+{
+    using C = ChunkCfg<D, Q8>;
+    using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
+    constexpr int NH = C::NH, NS = C::kSlots, NB = C::kBufs;
+    const PagedAttnParams &p = cp.a;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ __align__(8) uint64_t bar_q, kv_full[NS], kv_empty[NS], s_full[NB], p_full[NB], pv_done[NB], refbar[NB][4], endbar, sc_full[C::kScal];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_err, s_some;
+    __shared__ ChunkTile s_tile;
+    __shared__ int s_page[kChunkPages];
+    __shared__ __align__(16) float s_cw[C::kSoft][kBlock];   // [softmax warp][column]: counts of the codebook tile it works on
+    __shared__ float s_ref[kBlock];
+    __shared__ float s_lend[NB][kBlock], s_mend[NB][kBlock];
+    __shared__ __align__(16) float s_ks[C::kScal][Q8 ? kBlock : 4], s_vs[C::kScal][Q8 ? kBlock : 4], s_p2[C::kScal][Q8 && F16 ? kBlock : 4];
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int hk = blockIdx.y;
+    if (warp == 0) {
+        ChunkTile t;
+        const bool some = chunk_find(p, cp.TQ, blockIdx.x, t);
+        if (lane == 0) {
+            s_some = some;
+            s_tile = t;
+        }
+    }
+    if (tid == C::kWarpMma * 32) {
+        mbar_init(&bar_q, 1);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&kv_full[i], C::kLoad);
+            mbar_init(&kv_empty[i], 1);
+        }
+        for (int i = 0; i < NB; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&pv_done[i], 1);
+            for (int g = 0; g < 4; ++g) mbar_init(&refbar[i][g], 1);
+        }
+        for (int i = 0; i < C::kScal; ++i) mbar_init(&sc_full[i], C::kLoad);
+        mbar_init(&endbar, C::kSoft);
+        fence_mbar_init();
+        s_err = 0;
+    }
+    if (tid < kBlock) s_ref[tid] = -INFINITY;
+    __syncthreads();
+    if (!s_some) return;
+    if (warp == C::kWarpLoad) {
+        __syncwarp();
+        tmem_alloc(&s_tmem, C::kCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const ChunkTile tile = s_tile;
+    const ChunkWork work(p, tile);
+    const int n = work.n_items;
+    const int n_q2 = p.rerope ? work.n_far + (work.n_bd == 2 ? 1 : 0) : work.n_far;   // items scored with q2 come first
+    const int log_p = p.seqs.log_p, col0 = max(work.kb0, 0) * kBlock >> log_p, page_size = 1 << log_p;
+    auto page_of = [&](int key) {
+        const int x = (key >> log_p) - col0;
+        return x < kChunkPages ? s_page[x] : p.seqs.page(tile.s, x + col0);
+    };
+
+    if (warp >= C::kWarpLoad) {
+        // ================================================================== loads
+        const int lw = warp - C::kWarpLoad;
+        const bool leader = lw == 0 && elect_one();
+        if (leader) {
+            prefetch_tmap(&tm_q1); prefetch_tmap(&tm_q2); prefetch_tmap(&tm_cb); prefetch_tmap(&tm_vs);
+            mbar_expect_tx(&bar_q, (n_q2 > 0 ? 2 : 1) * NH * 128 * cp.TQ * p.G);
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                tma_load_3d(smem + C::kQ + h * kHalfBytes, &tm_q1, &bar_q, 64 * h, hk * p.G, tile.t0);
+                if (n_q2 > 0) tma_load_3d(smem + C::kQ + C::kTile + h * kHalfBytes, &tm_q2, &bar_q, 64 * h, hk * p.G, tile.t0);
+            }
+        }
+        {
+            const int cols = ((tile.n - 1) >> log_p) - col0 + 1, last = ((tile.pos0 / kBlock + 1) * kBlock - 1) >> log_p;
+            for (int x = tid - C::kWarpLoad * 32; x < min(min(cols, last - col0 + 1), kChunkPages); x += C::kLoad * 32) s_page[x] = p.seqs.page(tile.s, col0 + x);
+            if (C::kLoad == 1) __syncwarp();
+            else asm volatile("bar.sync 1, %0;" ::"n"(C::kLoad * 32) : "memory");
+        }
+        int slot = 0;
+        uint32_t free_par = 1u;
+        bool first_round = true, ok = true;
+        auto advance = [&]() {
+            if (++slot == NS) {
+                slot = 0;
+                free_par ^= 1u;
+                first_round = false;
+            }
+        };
+        auto far_tile = [&](int it, bool is_v, int arrive_bytes) {
+            uint8_t *dst = smem + C::kRing + slot * C::kTile;
+            mbar_expect_tx(&kv_full[slot], arrive_bytes);
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                if (is_v) tma_load_3d(dst + h * kHalfBytes, &tm_vs, &kv_full[slot], 64 * h, work.block(it) * kBlock, tile.snap * p.Hkv + hk);
+                else tma_load_3d(dst + h * kHalfBytes, &tm_cb, &kv_full[slot], 64 * h, work.block(it) * kBlock, hk);
+            }
+        };
+        if constexpr (!Q8) {
+            if (leader) {
+                auto load = [&](int it, bool is_v) {
+                    if (!ok) return;
+                    if (!first_round && !mbar_wait(&kv_empty[slot], free_par, p.wait_limit)) {
+                        ok = false;
+                        return;
+                    }
+                    const int kind = work.kind(it);
+                    if (kind == kFar) {
+                        far_tile(it, is_v, C::kTile);
+                    } else {
+                        const CUtensorMap *tm = is_v ? &tm_v : (kind == kBdA ? &tm_k3 : &tm_k1);
+                        uint8_t *dst = smem + C::kRing + slot * C::kTile;
+                        const int key0 = work.block(it) * kBlock, end = min(tile.n, key0 + kBlock);
+                        int bytes = 0;                        // pages behind the end, or missing ones (reported), are not loaded
+                        for (int key = key0; key < end; key += page_size)
+                            if (page_of(key) >= 0) bytes += page_size * D * 2;
+                        mbar_expect_tx(&kv_full[slot], bytes);
+                        for (int key = key0; key < end; key += page_size) {
+                            const int page = page_of(key);
+                            if (page < 0) continue;
+#pragma unroll
+                            for (int h = 0; h < NH; ++h)
+                                tma_load_4d(dst + h * kHalfBytes + (key - key0) * 128, tm, &kv_full[slot], 64 * h, 0, hk, page);
+                        }
+                    }
+                    advance();
+                };
+                for (int j = 0; j < NB && j < n; ++j) load(j, false);
+                for (int j = 0; j < n; ++j) {
+                    load(j, true);
+                    if (j + NB < n) load(j + NB, false);
+                }
+                if (!ok) s_err = 1;
+            }
+        } else {
+            // Codes of the next tile are fetched into registers while this one is converted.  CH lanes share a row, 16 codes each.
+            constexpr int CH = D / 16, RPI = 32 / CH, NL = 32 / RPI;       // rows per instruction, loads per thread and tile
+            const int ch = lane % CH, rsub = lane / CH;
+            const int total = 2 * n;
+            uint4 codes[NL];
+            float scale_k = 0.f, scale_v = 0.f;
+            // load number -> item, kind of tile (order K0 K1 V0 K2 V1 ... as the tensor pipe consumes them)
+            auto item_of = [&](int x, bool &is_v) {
+                if (x < NB || n <= NB) {
+                    if (x < min(NB, n)) {
+                        is_v = false;
+                        return x;
+                    }
+                    is_v = true;
+                    return x - n;
+                }
+                const int y = x - NB;                                      // V0 K(NB) V1 K(NB+1) ... until the keys run out
+                if (y < 2 * (n - NB)) {
+                    is_v = (y & 1) == 0;
+                    return is_v ? y / 2 : NB + y / 2;
+                }
+                is_v = true;
+                return y - (n - NB);
+            };
+            auto fetch = [&](int x) {
+                bool is_v;
+                const int it = item_of(x, is_v), kind = work.kind(it);
+                if (kind == kFar) return;
+                const int key0 = work.block(it) * kBlock + 32 * lw;
+                const PagedPool &pool = is_v ? p.v : (kind == kBdA ? p.k3 : p.k1);
+                const int8_t *base = static_cast<const int8_t *>(pool.ptr);
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    const int key = key0 + RPI * i + rsub;
+                    codes[i] = make_uint4(0, 0, 0, 0);
+                    if (key < tile.n) {
+                        const int page = page_of(key);
+                        if (page >= 0) codes[i] = *reinterpret_cast<const uint4 *>(base + pool.row(page, hk, key & (page_size - 1)) + 16 * ch);
+                    }
+                }
+                if (!is_v) {
+                    const int key = key0 + lane, page = key < tile.n ? page_of(key) : -1, r = key & (page_size - 1);
+                    scale_k = page >= 0 ? __ldg(pool.scale + pool.scale_at(page, hk, r)) : 0.f;
+                    scale_v = page >= 0 ? __ldg(p.v.scale + p.v.scale_at(page, hk, r)) : 0.f;
+                }
+            };
+            fetch(0);
+            for (int x = 0; x < total; ++x) {
+                bool is_v;
+                const int it = item_of(x, is_v), kind = work.kind(it);
+                if (!first_round && !mbar_wait(&kv_empty[slot], free_par, p.wait_limit)) ok = false;
+                if (!__all_sync(~0u, ok)) {
+                    ok = false;
+                    break;
+                }
+                if (kind == kFar) {
+                    if (leader) far_tile(it, is_v, C::kTile);
+                    else if (lw != 0 && lane == 0) mbar_arrive(&kv_full[slot]);
+                    if (!is_v && lane == 0) mbar_arrive(&sc_full[it % C::kScal]);   // keeps the phases of sc_full in step with the items
+                    if (x + 1 < total) fetch(x + 1);
+                } else {
+                    if (!is_v) {
+                        const int b = it % C::kScal, col = 32 * lw + lane;
+                        s_ks[b][col] = scale_k * p.scale_log2;
+                        if constexpr (F16) s_vs[b][col] = half_weight_factor(scale_v, s_p2[b][col]);
+                        else s_vs[b][col] = scale_v;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sc_full[b]);
+                    }
+                    uint8_t *dst = smem + C::kRing + slot * C::kTile + (ch >> 2) * kHalfBytes;
+                    const int flip = D == 128 ? ch >> 2 : 0;                  // the two halves of a row take turns: no bank is asked for twice
+#pragma unroll
+                    for (int i = 0; i < NL; ++i) {
+                        const int row = 32 * lw + RPI * i + rsub;
+                        uint4 a, b;
+                        if (F16 && is_v) {
+                            if constexpr (F16) {
+                                const __half2 p2 = __float2half2_rn(s_p2[it % C::kScal][row]);
+                                Codes8<T>::expand_scaled(codes[i].x, p2, a.x, a.y);
+                                Codes8<T>::expand_scaled(codes[i].y, p2, a.z, a.w);
+                                Codes8<T>::expand_scaled(codes[i].z, p2, b.x, b.y);
+                                Codes8<T>::expand_scaled(codes[i].w, p2, b.z, b.w);
+                            }
+                        } else {
+                            Codes8<T>::expand(codes[i].x, a.x, a.y);
+                            Codes8<T>::expand(codes[i].y, a.z, a.w);
+                            Codes8<T>::expand(codes[i].z, b.x, b.y);
+                            Codes8<T>::expand(codes[i].w, b.z, b.w);
+                        }
+                        uint8_t *line = dst + row * 128;
+                        const int c0 = (2 * (ch & 3)) ^ (row & 7);            // 128-byte swizzle: 16-byte piece j of row r lies at j ^ (r % 8)
+                        *reinterpret_cast<uint4 *>(line + 16 * (c0 ^ flip)) = flip ? b : a;
+                        *reinterpret_cast<uint4 *>(line + 16 * (c0 ^ flip ^ 1)) = flip ? a : b;
+                    }
+                    if (x + 1 < total) fetch(x + 1);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&kv_full[slot]);
+                }
+                advance();
+            }
+            if (!ok) s_err = 1;
+        }
+    } else if (warp == C::kWarpMma) {
+        // ================================================================== products
+        if (elect_one()) {
+            constexpr uint32_t idesc_qk = idesc_f16kind(128, kBlock, 0, 0, F16 ? 0u : 1u);
+            constexpr uint32_t idesc_pv = idesc_f16kind(128, D, 0, 1, F16 ? 0u : 1u);
+            const uint64_t d_q = smem_desc_sw128(smem_u32(smem + C::kQ), 16, 1024);
+            const uint64_t d_k0 = smem_desc_sw128(smem_u32(smem + C::kRing), 16, 1024);
+            const uint64_t d_v0 = smem_desc_sw128(smem_u32(smem + C::kRing), kHalfBytes, 1024);
+            bool ok = mbar_wait(&bar_q, 0, p.wait_limit);
+            int slot = 0;
+            uint32_t slot_par = 0;
+            int sbuf = 0, pbuf = 0;
+            uint32_t p_par = 0;
+            auto next_slot = [&]() {
+                if (++slot == NS) {
+                    slot = 0;
+                    slot_par ^= 1u;
+                }
+            };
+            auto qk = [&](int it) {
+                if (!ok) return;
+                if (!mbar_wait(&kv_full[slot], slot_par, p.wait_limit)) {
+                    ok = false;
+                    return;
+                }
+                tc_fence_after();
+                const uint64_t db = d_k0 + static_cast<uint64_t>((slot * C::kTile) >> 4);
+                const uint64_t da = d_q + static_cast<uint64_t>((it < n_q2 ? C::kTile : 0) >> 4);
+                const uint32_t sdst = tmem + C::kColS + kBlock * sbuf;
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+#pragma unroll
+                    for (int k4 = 0; k4 < 4; ++k4) {
+                        const uint64_t off = static_cast<uint64_t>((h * kHalfBytes + k4 * 32) >> 4);
+                        if (h == 0 && k4 == 0) mma_ss_first(sdst, da + off, db + off, idesc_qk);
+                        else mma_ss_acc(sdst, da + off, db + off, idesc_qk);
+                    }
+                tc_commit(&kv_empty[slot]);
+                tc_commit(&s_full[sbuf]);
+                next_slot();
+                if (++sbuf == NB) sbuf = 0;
+            };
+            auto pv = [&](int it) {
+                if (!ok) return;
+                if (!mbar_wait(&p_full[pbuf], p_par, p.wait_limit) || !mbar_wait(&kv_full[slot], slot_par, p.wait_limit)) {
+                    ok = false;
+                    return;
+                }
+                tc_fence_after();
+                const uint64_t dv = d_v0 + static_cast<uint64_t>((slot * C::kTile) >> 4);
+                const uint32_t odst = tmem + C::kColO, psrc = tmem + C::kColS + kBlock * pbuf;
+                if (it == 0) mma_ts_first(odst, psrc, dv, idesc_pv);
+                else mma_ts_acc(odst, psrc, dv, idesc_pv);
+#pragma unroll
+                for (int kk = 1; kk < kBlock / 16; ++kk) mma_ts_acc(odst, psrc + 8 * kk, dv + static_cast<uint64_t>((kk * 2048) >> 4), idesc_pv);
+                tc_commit(&kv_empty[slot]);
+                tc_commit(&pv_done[pbuf]);
+                next_slot();
+                if (++pbuf == NB) {
+                    pbuf = 0;
+                    p_par ^= 1u;
+                }
+            };
+            for (int j = 0; j < NB && j < n; ++j) qk(j);
+            for (int j = 0; j < n; ++j) {
+                pv(j);
+                if (j + NB < n) qk(j + NB);
+            }
+            if (!ok) s_err = 1;
+        }
+    } else {
+        // ================================================================== softmax
+        constexpr unsigned kAll = 0xffffffffu;
+        const int g = warp >> 2, lq = warp & 3;
+        const int row = lq * 32 + lane;
+        const int rpos = tile.pos0 % kBlock + row / p.G;      // position of the row's token inside its block (rows without a token: behind it)
+        const uint32_t lane_off = static_cast<uint32_t>(lq * 32) << 16;
+        const uint32_t sa = tmem + lane_off + C::kColS + kBlock * g;
+        const uint32_t o_addr = tmem + lane_off + C::kColO;
+        float my_ref = -INFINITY, l_part = 0.f;
+        bool ok = true;
+        constexpr int NCW = kBlock / 32;
+        const float *cnt_base = p.cnt + (static_cast<int64_t>(max(tile.snap, 0)) * p.Hkv + hk) * p.MK + lane;
+        float *cw = &s_cw[warp][0];
+        float cnt_reg[NCW];
+#pragma unroll
+        for (int i = 0; i < NCW; ++i) cnt_reg[i] = g < work.n_far ? __ldg(cnt_base + g * kBlock + 32 * i) : 0.f;
+#pragma unroll 1
+        for (int it = g; it < n; it += NB) {
+            const int par = (it / NB) & 1;
+            const int kind = work.kind(it);
+            const bool q8 = Q8 && kind != kFar;
+            const int sb = it % C::kScal;
+            bool has_empty = false;
+            if (kind == kFar) {
+                __syncwarp();
+                bool full = true;
+#pragma unroll
+                for (int i = 0; i < NCW; ++i) {
+                    cw[32 * i + lane] = cnt_reg[i];
+                    full = full && cnt_reg[i] > 0.f;
+                }
+                has_empty = __any_sync(kAll, !full);
+                __syncwarp();
+                if (it + NB < work.n_far) {
+#pragma unroll
+                    for (int i = 0; i < NCW; ++i) cnt_reg[i] = __ldg(cnt_base + (it + NB) * kBlock + 32 * i);
+                }
+            }
+            const int lo = kind == kBdB ? rpos : 0, hi = kind == kDiag ? rpos + 1 : kind == kBdA ? rpos : kBlock;
+            if (q8 && !__all_sync(kAll, mbar_wait(&sc_full[sb], (it / C::kScal) & 1, p.wait_limit))) {
+                ok = false;
+                break;
+            }
+            if (!__all_sync(kAll, mbar_wait(&s_full[g], par, p.wait_limit))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            uint32_t r[64];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < kBlock; c += 64) {
+                if (Q8 && q8) {
+                    q8_scores(sa + c, kind, lo - c, hi - c, &s_ks[sb][c], r);
+                    mx = fmaxf(mx, t4_max(r));
+                } else {
+                    t4_scores(sa + c, kind, has_empty, lo - c, hi - c, cw + c, r);
+                    mx = fmaxf(mx, t4_max(r));
+                }
+            }
+            const float m_tile = q8 ? mx : mx * p.scale_log2;
+            if (it > 0 && !__all_sync(kAll, mbar_wait(&refbar[(g + NB - 1) % NB][lq], ((it - 1) / NB) & 1, p.wait_limit))) {
+                ok = false;
+                break;
+            }
+            const float ref = s_ref[row];
+            float m_use = ref;
+            if (m_tile > ref + kT4Lazy || ref == -INFINITY) m_use = fmaxf(ref, m_tile);
+            if (m_use != ref) s_ref[row] = m_use;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&refbar[g][lq]);
+            const float m_safe = (m_use == -INFINITY) ? 0.f : m_use;
+            const bool rescale = (m_use != ref) && (ref != -INFINITY);
+            if (__any_sync(kAll, rescale)) {
+                if (!__all_sync(kAll, mbar_wait(&pv_done[(it - 1) % NB], ((it - 1) / NB) & 1, p.wait_limit))) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const float alpha = rescale ? ex2(ref - m_safe) : 1.f;
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    uint32_t o[16];
+                    tmem_ld16(o_addr + 16 * c, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                    tmem_st16(o_addr + 16 * c, o);
+                }
+            }
+            if (my_ref != m_use) {
+                l_part *= ex2(my_ref - m_safe);
+                my_ref = m_use;
+            }
+            float ls = 0.f;
+#pragma unroll
+            for (int c = 0; c < kBlock; c += 64) {
+                if (Q8 && q8) {
+                    q8_scores(sa + c, kind, lo - c, hi - c, &s_ks[sb][c], r);
+                    ls = q8_exp<F16>(r, sa + c / 2, kind != kFull, &s_vs[sb][c], -m_safe, ls);
+                } else {
+                    t4_scores(sa + c, kind, has_empty, lo - c, hi - c, cw + c, r);
+                    ls = kind == kFar ? t4_exp<true, F16>(r, sa + c / 2, cw + c, p.scale_log2, -m_safe, ls)
+                                      : t4_exp<false, F16>(r, sa + c / 2, cw + c, p.scale_log2, -m_safe, ls);
+                }
+            }
+            l_part += ls;
+            if (!Q8 && it == n - 1) {
+                // The value rows behind the sequence's end: the weights there are zero, what the page holds need not be a number.
+                const int valid = tile.n - tile.pos0 / kBlock * kBlock;
+                if (valid < kBlock) {
+                    constexpr int per = 2;                    // the last load of the ring is this item's value tile
+                    const int vslot = (per * n - 1) % NS;
+                    if (!__all_sync(kAll, mbar_wait(&kv_full[vslot], ((per * n - 1) / NS) & 1, p.wait_limit))) {
+                        ok = false;
+                        break;
+                    }
+                    if (row >= valid) {
+#pragma unroll
+                        for (int h = 0; h < NH; ++h)
+#pragma unroll
+                            for (int x = 0; x < 8; ++x)
+                                *reinterpret_cast<uint4 *>(smem + C::kRing + vslot * C::kTile + h * kHalfBytes + row * 128 + 16 * x) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                }
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[g]);
+        }
+        // ---- merge the partial denominators, O / l once the last product has finished
+        s_lend[g][row] = l_part;
+        s_mend[g][row] = my_ref;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&endbar);
+        if (ok && !__all_sync(kAll, mbar_wait(&endbar, 0, p.wait_limit))) ok = false;
+        if (ok && !__all_sync(kAll, mbar_wait(&pv_done[(n - 1) % NB], ((n - 1) / NB) & 1, p.wait_limit))) ok = false;
+        tc_fence_after();
+        if (!ok) s_err = 1;
+        if (ok && g < 2) {
+            const float ref = s_ref[row];
+            float den = 0.f;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const float li = s_lend[i][row];
+                if (li != 0.f) den += li * ex2(s_mend[i][row] - ref);
+            }
+            const float inv = den != 0.f ? 1.f / den : 0.f;
+            uint32_t r[C::kOq];
+#pragma unroll
+            for (int c = 0; c < C::kOq / 32; ++c) tmem_ld32(o_addr + g * C::kOq + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
+            tc_wait_ld();
+            // the warp's 32 rows through the tile ring (every read of it has finished) and out in whole lines, eight lanes a row
+            constexpr int kRowB = C::kOq * 2, kPitch = kRowB + 16;
+            uint8_t *stg = smem + C::kRing + warp * (32 * kPitch);
+#pragma unroll
+            for (int j = 0; j < C::kOq / 8; ++j) {
+                uint4 w;
+                w.x = pack16<F16>(__uint_as_float(r[8 * j]) * inv, __uint_as_float(r[8 * j + 1]) * inv);
+                w.y = pack16<F16>(__uint_as_float(r[8 * j + 2]) * inv, __uint_as_float(r[8 * j + 3]) * inv);
+                w.z = pack16<F16>(__uint_as_float(r[8 * j + 4]) * inv, __uint_as_float(r[8 * j + 5]) * inv);
+                w.w = pack16<F16>(__uint_as_float(r[8 * j + 6]) * inv, __uint_as_float(r[8 * j + 7]) * inv);
+                *reinterpret_cast<uint4 *>(stg + lane * kPitch + 16 * j) = w;
+            }
+            __syncwarp();
+            constexpr int kLanesPerRow = kRowB / 16, kRowsPerIt = 32 / kLanesPerRow;
+            const int sub = lane / kLanesPerRow, ch = lane % kLanesPerRow, valid = tile.ntok * p.G;
+            T *obase = static_cast<T *>(p.out) + g * C::kOq + 8 * ch;
+#pragma unroll
+            for (int x = 0; x < 32 / kRowsPerIt; ++x) {
+                const int rr = x * kRowsPerIt + sub, qr = lq * 32 + rr;
+                const uint4 w = *reinterpret_cast<const uint4 *>(stg + rr * kPitch + 16 * ch);
+                if (qr < valid) {
+                    const int64_t t = tile.t0 + qr / p.G, h = hk * p.G + qr % p.G;
+                    *reinterpret_cast<uint4 *>(obase + t * p.o_t + h * p.o_h) = w;
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (s_err && tid == 0) {
+        if (p.seqs.status) atomicExch(p.seqs.status, VQ_WORD_TIMEOUT);
+        // a bounded wait expired: give tile loads still in flight time to land before leaving
+#pragma unroll 1
+        for (int w = 0; w < (1 << 14); ++w) __nanosleep(256);
+    }
+    __syncthreads();
+    if (warp == C::kWarpLoad) {
+        __syncwarp();
+        tmem_dealloc(tmem, C::kCols);
+    }
+}
+
+// tokens [T, Hq, D] in boxes of 64 columns x G heads x TQ tokens
+static bool map_tokens(CUtensorMap *out, const void *ptr, int64_t T, const PagedAttnParams &p, int64_t s_t, int64_t s_h, int TQ, bool f16)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dim[3] = {static_cast<cuuint64_t>(p.D), static_cast<cuuint64_t>(p.Hq), static_cast<cuuint64_t>(T)};
+    // a dimension of one element may come with any stride: give the map one it accepts
+    const cuuint64_t str[2] = {static_cast<cuuint64_t>(p.Hq > 1 ? s_h * 2 : p.D * 2), static_cast<cuuint64_t>(T > 1 ? s_t * 2 : p.Hq * p.D * 2)};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.G), static_cast<cuuint32_t>(TQ)}, es[3] = {1, 1, 1};
+    return fn(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(ptr), dim, str, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// pool [NP, Hkv, P, D] in boxes of 64 columns x one page
+static bool map_pool(CUtensorMap *out, const PagedPool &pool, const PagedAttnParams &p, bool f16)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return false;
+    const int P = 1 << p.seqs.log_p;
+    const cuuint64_t dim[4] = {static_cast<cuuint64_t>(p.D), static_cast<cuuint64_t>(P), static_cast<cuuint64_t>(p.Hkv), static_cast<cuuint64_t>(p.seqs.NP)};
+    const cuuint64_t str[3] = {static_cast<cuuint64_t>(pool.s_row * 2), static_cast<cuuint64_t>(p.Hkv > 1 ? pool.s_head * 2 : pool.s_row * 2),
+                               static_cast<cuuint64_t>(p.seqs.NP > 1 ? pool.s_page * 2 : pool.s_row * 2)};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(P), 1, 1}, es[4] = {1, 1, 1, 1};
+    return fn(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(pool.ptr), dim, str, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool F16, bool Q8>
+static int launch_chunk(const PagedAttnParams &a, cudaStream_t stream)
+{
+    using C = ChunkCfg<D, Q8>;
+    ChunkParams cp;
+    cp.a = a;
+    cp.TQ = kBlock / a.G;
+    TcMaps m;
+    if (!map_tokens(&m.q1, a.q1, a.seqs.T, a, a.q1_t, a.q1_h, cp.TQ, F16) || !map_tokens(&m.q2, a.q2, a.seqs.T, a, a.q2_t, a.q2_h, cp.TQ, F16)) return VQ_ELAUNCH;
+    if (Q8) {
+        m.k1 = m.k3 = m.v = m.q1;   // not used: codes are fetched by plain loads
+    } else if (!map_pool(&m.k1, a.k1, a, F16) || !map_pool(&m.k3, a.k3, a, F16) || !map_pool(&m.v, a.v, a, F16)) {
+        return VQ_ELAUNCH;
+    }
+    if (a.cb != nullptr) {
+        const uint64_t MK = a.MK, cd[3] = {D, MK, static_cast<uint64_t>(a.Hkv)}, cs[3] = {1, D, MK * D}, vd[3] = {D, MK, static_cast<uint64_t>(a.NS) * a.Hkv};
+        if (!make_map(&m.cb, a.cb, 3, cd, cs, kBlock, F16) || !make_map(&m.vs, a.vsum, 3, vd, cs, kBlock, F16)) return VQ_ELAUNCH;
+    } else {
+        m.cb = m.vs = m.q1;         // never read: no tile has codes
+    }
+    auto kern = paged_chunk_kernel<D, F16, Q8>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kTotal) != cudaSuccess) return VQ_ELAUNCH;
+    // tiles: every block of positions that a sequence touches rounds its tokens up to whole tiles
+    int64_t tiles = a.seqs.T / cp.TQ + a.seqs.T / kBlock + 2 * static_cast<int64_t>(a.seqs.S);
+    if (tiles > a.seqs.T) tiles = a.seqs.T;
+    kern<<<dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.Hkv)), C::kThreads, C::kTotal, stream>>>(m.q1, m.q2, m.k1, m.k3, m.v, m.cb, m.vs, cp);
+    return launch_status();
+}
+
+template <bool F16>
+static int launch_chunk_type(const PagedAttnParams &p, bool q8, cudaStream_t stream)
+{
+    if (p.D == 64) return q8 ? launch_chunk<64, F16, true>(p, stream) : launch_chunk<64, F16, false>(p, stream);
+    return q8 ? launch_chunk<128, F16, true>(p, stream) : launch_chunk<128, F16, false>(p, stream);
+}
+
+int launch_paged_chunk(const PagedAttnParams &p, int dtype, bool q8, cudaStream_t stream)
+{
+    return dtype == VQ_F16 ? launch_chunk_type<true>(p, q8, stream) : launch_chunk_type<false>(p, q8, stream);
+}
+
+}  // namespace vq

@@ -17,6 +17,7 @@
 // partial sums through distributed shared memory: no workspace, no second launch, the same order of additions every time.
 #include <cooperative_groups.h>
 
+#include "codes8.cuh"
 #include "paged_attn.cuh"
 #include "tc_ptx.cuh"
 
@@ -79,38 +80,6 @@ struct FewCfg {
     static constexpr int MT = D / 16;
 };
 
-template <typename T> struct IsBf16 { static constexpr bool value = false; };
-template <> struct IsBf16<__nv_bfloat16> { static constexpr bool value = true; };
-
-// Four 8-bit codes -> two packed pairs of 16-bit floats, exactly.
-template <typename T> struct Codes8;
-template <> struct Codes8<__half> {
-    // 0x6400 | (x + 128) is the half 1024 + x + 128
-    static __device__ __forceinline__ void expand(uint32_t w, uint32_t &lo, uint32_t &hi)
-    {
-        w ^= 0x80808080u;
-        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
-        const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2 *>(&b), bias);
-        lo = *reinterpret_cast<const uint32_t *>(&x);
-        hi = *reinterpret_cast<const uint32_t *>(&y);
-    }
-};
-template <> struct Codes8<__nv_bfloat16> {
-    // 0x4300 | (x & 127) is the bf16 128 + (x & 127), 0x4300 | (x & 128) is 128 or 256: their difference is x
-    static __device__ __forceinline__ uint32_t pair(uint32_t e)
-    {
-        const uint32_t a = e & 0xff7fff7fu, b = e & 0xff80ff80u;
-        const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
-        return *reinterpret_cast<const uint32_t *>(&x);
-    }
-    static __device__ __forceinline__ void expand(uint32_t w, uint32_t &lo, uint32_t &hi)
-    {
-        lo = pair(__byte_perm(w, 0x43434343u, 0x4140));
-        hi = pair(__byte_perm(w, 0x43434343u, 0x4342));
-    }
-};
-
 struct FewSteps {
     int n_far, n_old, n_near;       // steps of codes, of raw keys before the exact window, of rotated keys
     int old0, near0;                // first key of the latter two (multiples of 16)
@@ -148,6 +117,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAt
     const int rows = (i1 - i0 + 1) * p.G;
     const int bd = p.boundary(i0), snap = p.snapshot(s, bd);
     FewSteps st;
+    constexpr bool kHalf = Q8 && !IsBf16<T>::value;
     constexpr int KEYS = Q8 ? 32 : 16;                               // keys per step of window rows
     st.n_far = snap >= 0 ? p.MK / 16 : 0;
     st.old0 = bd;
@@ -273,16 +243,13 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAt
     // sc: scores of keys r and r + 8 (c0 c1 | c2 c3) in log2 units, -inf where excluded -> weights; w: denominator weights of the two keys,
     // f: factors of their value rows.  Raises the references, adds to l, returns the packed weights as B operands.
     auto softmax = [&](float (&sc)[NT][4], float w0, float w1, float f0, float f1, uint32_t (&pb)[NT][2]) {
-        // half weights carry the value's scale: the reference is that of score + log2(scale), so that they stay below 2^8 whatever the scale
-        constexpr bool kShift = Q8 && sizeof(T) == 2 && !IsBf16<T>::value;
-        const float sh0 = kShift ? __log2f(fmaxf(f0, 9.094947e-13f)) : 0.f, sh1 = kShift ? __log2f(fmaxf(f1, 9.094947e-13f)) : 0.f;
         bool above = false;
         float mx[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                mx[nt][x] = fmaxf(sc[nt][x] + sh0, sc[nt][2 + x] + sh1);
+                mx[nt][x] = fmaxf(sc[nt][x], sc[nt][2 + x]);
                 above |= mx[nt][x] > m[nt][x] + kFewLazy || (m[nt][x] == -INFINITY && mx[nt][x] > -INFINITY);
             }
         if (__any_sync(~0u, above)) {
@@ -361,7 +328,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAt
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) sc[nt][x] = 0.f;
-            float w0 = 1.f, w1 = 1.f, f0 = 1.f, f1 = 1.f, k0 = p.scale_log2, k1 = p.scale_log2;
+            float w0 = 1.f, w1 = 1.f, f0 = 1.f, f1 = 1.f, k0 = p.scale_log2, k1 = p.scale_log2, e0 = 1.f, e1 = 1.f;
             const uint8_t *kst = stg;
             if (far || !Q8) {
 #pragma unroll
@@ -397,6 +364,10 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAt
                 k1 *= s4[32];
                 f0 = s4[64];
                 f1 = s4[96];
+                if constexpr (kHalf) {
+                    f0 = half_weight_factor(f0, e0);
+                    f1 = half_weight_factor(f1, e1);
+                }
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -458,13 +429,24 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAt
                         v[a][0] = x.x; v[a][1] = x.y;
                     }
                 }
+                __half2 pa, pc;                                      // the powers of two that go with this thread's pairs of keys
+                if constexpr (kHalf) {
+                    pa = __floats2half2_rn(__shfl_sync(~0u, e0, 8 * c), __shfl_sync(~0u, e0, 8 * c + 4));
+                    pc = __floats2half2_rn(__shfl_sync(~0u, e1, 8 * c), __shfl_sync(~0u, e1, 8 * c + 4));
+                }
 #pragma unroll
                 for (int w = 0; w < D / 32; ++w)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {           // bytes 0, 1 and 2, 3 of the word: m-tiles 2 w, 2 w + 1
                         uint32_t a0, a1, a2, a3;
-                        Codes8<T>::expand(__byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140), a0, a1);
-                        Codes8<T>::expand(__byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140), a2, a3);
+                        const uint32_t u = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140), x = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
+                        if constexpr (kHalf) {
+                            Codes8<T>::expand_scaled(u, pa, a0, a1);
+                            Codes8<T>::expand_scaled(x, pc, a2, a3);
+                        } else {
+                            Codes8<T>::expand(u, a0, a1);
+                            Codes8<T>::expand(x, a2, a3);
+                        }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) M::mma(o[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
                     }
