@@ -96,3 +96,32 @@ def test_errors_are_exceptions_and_the_operators_trace(ops, api):
     eager = step(q, k, v, out).item()
     traced = torch.compile(step, backend="eager", fullgraph=True)(q, k, v, torch.empty_like(out)).item()
     assert eager == traced
+
+
+def test_paged_operators_through_the_dispatcher_equal_the_api(ops, api):
+    from tests.paged_cases import Case
+    for qs, lens, q8 in (((1, 3), (300, 500), False), ((140, 20), (500, 300), True)):
+        c = Case(5, qs, lens, 2, 4, 64, 32, 128, 128, torch.bfloat16, q8, True)
+        want = c.attend(api)
+        p, far = c.pages(), c.far_args()
+        q1, q2, out = c.q1.cuda(), c.q2.cuda(), torch.empty_like(want)
+        meta = (c.table.cuda(), c.cu_q.cuda(), c.seq_lens.cuda())
+        args = (q1, q2, *p, *meta, far["codebook"], far["cnt"], far["vsum"], far["snap_table"], c.W)
+        ops.paged_attention(*args, max(qs), 0.0, out, None)
+        assert torch.equal(out, want)
+        with pytest.raises(RuntimeError, match="status -7"):
+            ops.paged_attention(*args, 0, 0.0, out, None)
+        assert ops.paged_attention_status(*args, 0, 0.0, out, None) == -7
+        back = torch.empty(2, 2, 40, 64, dtype=torch.bfloat16, device="cuda")
+        start = (meta[2] - 40).contiguous()
+        ops.paged_read(p.v, p.v_scale, back, None, None, None, None, None, None, meta[0], start, meta[2], None)
+        assert torch.equal(back, api.paged_read([(p.v, p.v_scale)], meta[0], start, meta[2], 40, torch.bfloat16)[0])
+        k, v = (torch.randn(sum(qs), 2, 64, device="cuda").bfloat16() for _ in range(2))
+        other = type(p)(*(None if t is None else t.clone() for t in p))
+        cos, sin = api.rope_tables(1024, 64, "cuda")
+        r1 = torch.empty_like(q1)
+        ops.paged_append(k, v, *p, *meta, q1, r1, None, cos, sin, 0, None)
+        w1, _ = api.paged_append(k, v, other, *meta, q=q1)
+        assert torch.equal(r1, w1) and all(a is None or torch.equal(a.nan_to_num(9.0) if a.is_floating_point() else a, b.nan_to_num(9.0) if b.is_floating_point() else b)
+                                           for a, b in zip(p, other))
+    api.check_status()

@@ -14,8 +14,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import native
-from .native import (BLOCK, VqDecodeArgs, VqPagedAppendArgs, VqPagedAttentionArgs, VqPagedReadArgs, VqPrefillArgs, check, desc, lib,
-                     stream_ptr)
+from .native import BLOCK, VqDecodeArgs, VqPrefillArgs, check, desc, lib, stream_ptr
 
 _IMPL = {"auto": native.IMPL_AUTO, "simt": native.IMPL_SIMT, "tensor": native.IMPL_TENSOR}
 
@@ -471,12 +470,23 @@ class PagedKV(NamedTuple):
         return cls(pool(), pool(), pool() if raw_keys else None, scale(), scale(), scale() if raw_keys else None)
 
 
-def _paged_kv(kv, pages: PagedKV, block_table, cu_q, seq_lens) -> None:
-    for name, t in zip(("k1", "v", "k3", "k1_scale", "v_scale", "k3_scale"), pages):
-        desc(t, getattr(kv, name))
-    desc(block_table, kv.table)
-    desc(cu_q, kv.cu_q)
-    desc(seq_lens, kv.lens)
+def _paged(which: int, *args) -> None:
+    """One of the paged operators (append, read, attention) through the dispatcher; its first argument is a tensor."""
+    global _PAGED_CALLS
+    if _PAGED_CALLS is None:
+        from . import torch_ops
+        _PAGED_CALLS = torch_ops.paged_calls()
+    word = _STATUS.get(args[0].get_device())
+    if word is None:
+        word = device_status_word(_require_cuda(args[0]))
+    status = _PAGED_CALLS[which](*args, word)
+    if status != 0:
+        if status == -4:                                    # VQ_EDEVICE: host tensors and mixed devices are reported as everywhere here
+            _require_cuda(*(t for t in args if isinstance(t, torch.Tensor)))
+        check(status, ("vqattn_paged_append", "vqattn_paged_read", "vqattn_paged_attention")[which])
+
+
+_PAGED_CALLS = None
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, pages: PagedKV, block_table: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor,
@@ -489,25 +499,19 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pages: PagedKV, block_table: 
     block_table int32 [S,MB]: page of tokens [P*c, P*(c+1)) of a sequence; cu_q int32 [S+1]: sequence s brings rows cu_q[s] ..
     cu_q[s+1]-1; seq_lens int32 [S]: its length with them.  rotate=False stores keys (and returns queries) as they are.
     n_pos: an upper bound of the positions + 1 (None: what the table can address)."""
-    dev = _require_cuda(k, v, *pages, block_table, cu_q, seq_lens, q)
-    T, _, D = k.shape
-    new = lambda: torch.empty(q.shape, dtype=q.dtype, device=dev)
-    q1 = new() if q is not None else None
-    q2 = new() if q is not None and const_pos is not None else None
-    if T == 0:
+    q1 = q.new_empty(q.shape) if q is not None else None
+    q2 = q.new_empty(q.shape) if q is not None and const_pos is not None else None
+    if k.shape[0] == 0:
         return q1, q2
-    a = VqPagedAppendArgs()
-    _paged_kv(a.kv, pages, block_table, cu_q, seq_lens)
-    for name, t in (("k", k), ("v", v), ("q", q), ("q1", q1), ("q2", q2)):
-        desc(t, getattr(a, name))
+    if not k.is_cuda:
+        _require_cuda(k)
+    cos = sin = None
+    const = const_pos or 0
     if rotate:
         n = n_pos if n_pos is not None else block_table.shape[1] * pages.k1.shape[2]
-        cos, sin = rope_tables(max(n, (const_pos or 0) + 1), D, dev, base)
-        a.cos_tab, a.sin_tab, a.n_pos = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    a.const_pos = int(const_pos or 0)
-    a.status_word = device_status_word(dev).data_ptr()
-    with torch.cuda.device(dev):
-        check(lib.vqattn_paged_append(ctypes.byref(a), stream_ptr(dev)), "vqattn_paged_append")
+        cos, sin = rope_tables(max(n, const + 1), k.shape[2], k.device, base)
+    k1, vp, k3, k1_scale, v_scale, k3_scale = pages
+    _paged(0, k, v, k1, vp, k3, k1_scale, v_scale, k3_scale, block_table, cu_q, seq_lens, q, q1, q2, cos, sin, const)
     return q1, q2
 
 
@@ -521,24 +525,14 @@ def paged_read(pools, block_table: torch.Tensor, starts: torch.Tensor, seq_lens:
     pools = [p if isinstance(p, tuple) else (p, None) for p in pools]
     if not 1 <= len(pools) <= 3:
         raise ValueError("one to three pools")
-    dev = _require_cuda(*(t for p in pools for t in p), block_table, starts, seq_lens)
     first = pools[0][0]
     dt = out_dtype or (torch.float32 if first.dtype == torch.int8 else first.dtype)
-    S = block_table.shape[0]
-    outs = [torch.empty((S, first.shape[1], n, first.shape[3]), dtype=dt, device=dev) for _ in pools]
-    if S == 0 or n == 0:
+    shape = (block_table.shape[0], first.shape[1], n, first.shape[3])
+    outs = [first.new_empty(shape, dtype=dt) for _ in pools]
+    if shape[0] == 0 or n == 0:
         return outs
-    a = VqPagedReadArgs()
-    for i, ((pool, scale), out) in enumerate(zip(pools, outs)):
-        desc(pool, a.pool[i])
-        desc(scale, a.scale[i])
-        desc(out, a.out[i])
-    desc(block_table, a.table)
-    desc(starts, a.start)
-    desc(seq_lens, a.lens)
-    a.status_word = device_status_word(dev).data_ptr()
-    with torch.cuda.device(dev):
-        check(lib.vqattn_paged_read(ctypes.byref(a), stream_ptr(dev)), "vqattn_paged_read")
+    args = [x for (pool, scale), out in zip(pools, outs) for x in (pool, scale, out)]
+    _paged(1, *args, *(None,) * (9 - len(args)), block_table, starts, seq_lens)
     return outs
 
 
@@ -556,20 +550,15 @@ def paged_attention(q1: torch.Tensor, q2: torch.Tensor, pages: PagedKV, block_ta
     far = (codebook, cnt, vsum, snap_table)
     if codebook is not None and any(t is None for t in far):
         raise ValueError("codebook, cnt, vsum and snap_table go together")
-    dev = _require_cuda(q1, q2, *pages, block_table, cu_q, seq_lens, *far, out)
     if out is None:
-        out = torch.empty(q1.shape, dtype=q1.dtype, device=dev)
+        out = q1.new_empty(q1.shape)
     if q1.shape[0] == 0:
         return out
-    a = VqPagedAttentionArgs()
-    _paged_kv(a.kv, pages, block_table, cu_q, seq_lens)
-    for name, t in zip(("q1", "q2", "out", "codebook", "cnt", "vsum", "snap_table"), (q1, q2, out) + (far if codebook is not None else (None,) * 4)):
-        desc(t, getattr(a, name))
-    a.window, a.max_q = int(window), int(max_q)
-    a.scale = float(scale) if scale else 0.0
-    a.status_word = device_status_word(dev).data_ptr()
-    with torch.cuda.device(dev):
-        check(lib.vqattn_paged_attention(ctypes.byref(a), stream_ptr(dev)), "vqattn_paged_attention")
+    if codebook is None:
+        far = (None,) * 4
+    k1, vp, k3, k1_scale, v_scale, k3_scale = pages
+    _paged(2, q1, q2, k1, vp, k3, k1_scale, v_scale, k3_scale, block_table, cu_q, seq_lens, *far, int(window), int(max_q),
+           float(scale) if scale else 0.0, out)
     return out
 
 

@@ -14,6 +14,7 @@
 #include <torch/library.h>
 
 #include <optional>
+#include <utility>
 
 #include "vqattn.h"
 
@@ -25,6 +26,7 @@ int32_t dtype_of(const at::Tensor &t)
         case at::kFloat: return VQ_F32;
         case at::kBFloat16: return VQ_BF16;
         case at::kHalf: return VQ_F16;
+        case at::kChar: return VQ_I8;
         case at::kByte: return VQ_U8;
         case at::kUInt16: return VQ_U16;
         case at::kInt: return VQ_I32;
@@ -189,6 +191,107 @@ void cache_advance(const at::Tensor &codes, const at::Tensor &v_new, int64_t K, 
           "vqattn::cache_advance");
 }
 
+// ---- the paged cache.  The *_status forms return the C status (what vqtree_b200/api.py turns into its own exception); the others raise.
+
+VqTensorDesc any_desc(const at::Tensor &t)         // host tensors too: the C function answers VQ_EDEVICE for them
+{
+    if (t.is_cuda()) return desc(t);
+    VqTensorDesc d{};
+    TORCH_CHECK(t.dim() <= VQATTN_MAX_DIMS, "vqattn: at most ", VQATTN_MAX_DIMS, " dimensions");
+    d.ptr = t.numel() > 0 ? t.data_ptr() : reinterpret_cast<void *>(16);
+    d.dtype = dtype_of(t);
+    d.ndim = static_cast<int32_t>(t.dim());
+    for (int64_t i = 0; i < t.dim(); ++i) {
+        d.shape[i] = t.size(i);
+        d.stride[i] = t.stride(i);
+    }
+    d.device = -1;
+    return d;
+}
+VqTensorDesc any_desc(const std::optional<at::Tensor> &t)
+{
+    return t.has_value() && t->defined() ? any_desc(*t) : desc(t);
+}
+
+using OptTensor = std::optional<at::Tensor>;
+
+VqPagedKv paged_kv(const at::Tensor &k1, const at::Tensor &v, const OptTensor &k3, const OptTensor &k1_scale, const OptTensor &v_scale,
+                   const OptTensor &k3_scale, const at::Tensor &table, const at::Tensor &cu_q, const at::Tensor &lens)
+{
+    VqPagedKv kv{};
+    kv.k1 = any_desc(k1); kv.v = any_desc(v); kv.k3 = any_desc(k3);
+    kv.k1_scale = any_desc(k1_scale); kv.v_scale = any_desc(v_scale); kv.k3_scale = any_desc(k3_scale);
+    kv.table = any_desc(table); kv.cu_q = any_desc(cu_q); kv.lens = any_desc(lens);
+    return kv;
+}
+
+// pages <- new tokens k, v [T,Hkv,D] (rotated when there are tables), q1 / q2 <- q [T,Hq,D] rotated
+int64_t paged_append_status(const at::Tensor &k, const at::Tensor &v, at::Tensor k1, at::Tensor v_pages, const OptTensor &k3,
+                            const OptTensor &k1_scale, const OptTensor &v_scale, const OptTensor &k3_scale, const at::Tensor &table,
+                            const at::Tensor &cu_q, const at::Tensor &lens, const OptTensor &q, const OptTensor &q1, const OptTensor &q2,
+                            const OptTensor &cos_tab, const OptTensor &sin_tab, int64_t const_pos, const OptTensor &status_word)
+{
+    if (!k.is_cuda()) return VQ_EDEVICE;
+    const c10::cuda::CUDAGuard guard(k.device());
+    VqPagedAppendArgs a{};
+    a.kv = paged_kv(k1, v_pages, k3, k1_scale, v_scale, k3_scale, table, cu_q, lens);
+    a.k = any_desc(k); a.v = any_desc(v); a.q = any_desc(q); a.q1 = any_desc(q1); a.q2 = any_desc(q2);
+    if (cos_tab.has_value() && cos_tab->defined()) {
+        TORCH_CHECK(sin_tab.has_value() && cos_tab->is_cuda() && sin_tab->is_cuda() && cos_tab->scalar_type() == at::kFloat &&
+                        sin_tab->scalar_type() == at::kFloat && cos_tab->is_contiguous() && sin_tab->is_contiguous() &&
+                        cos_tab->sizes() == sin_tab->sizes() && cos_tab->dim() == 2 && 2 * cos_tab->size(1) == k.size(-1),
+                    "vqattn: cos / sin tables are contiguous CUDA float32 [n_pos, D / 2]");
+        a.cos_tab = cos_tab->data_ptr<float>();
+        a.sin_tab = sin_tab->data_ptr<float>();
+        a.n_pos = cos_tab->size(0);
+    }
+    a.const_pos = const_pos;
+    a.status_word = word_of(status_word);
+    return vqattn_paged_append(&a, stream_of(k));
+}
+
+// out [S,Hkv,n,D] <- rows [start, start + n) of every sequence in a pool; up to three pools
+int64_t paged_read_status(const at::Tensor &pool0, const OptTensor &scale0, at::Tensor out0, const OptTensor &pool1, const OptTensor &scale1,
+                          const OptTensor &out1, const OptTensor &pool2, const OptTensor &scale2, const OptTensor &out2, const at::Tensor &table,
+                          const at::Tensor &start, const at::Tensor &lens, const OptTensor &status_word)
+{
+    if (!pool0.is_cuda()) return VQ_EDEVICE;
+    const c10::cuda::CUDAGuard guard(pool0.device());
+    VqPagedReadArgs a{};
+    a.pool[0] = any_desc(pool0); a.pool[1] = any_desc(pool1); a.pool[2] = any_desc(pool2);
+    a.scale[0] = any_desc(scale0); a.scale[1] = any_desc(scale1); a.scale[2] = any_desc(scale2);
+    a.out[0] = any_desc(out0); a.out[1] = any_desc(out1); a.out[2] = any_desc(out2);
+    a.table = any_desc(table); a.start = any_desc(start); a.lens = any_desc(lens);
+    a.status_word = word_of(status_word);
+    return vqattn_paged_read(&a, stream_of(pool0));
+}
+
+// out [T,Hq,D] <- attention of the new tokens over their pages and, before the boundary, over the snapshots
+int64_t paged_attention_status(const at::Tensor &q1, const at::Tensor &q2, const at::Tensor &k1, const at::Tensor &v_pages, const OptTensor &k3,
+                               const OptTensor &k1_scale, const OptTensor &v_scale, const OptTensor &k3_scale, const at::Tensor &table,
+                               const at::Tensor &cu_q, const at::Tensor &lens, const OptTensor &codebook, const OptTensor &cnt,
+                               const OptTensor &vsum, const OptTensor &snap_table, int64_t window, int64_t max_q, double scale, at::Tensor out,
+                               const OptTensor &status_word)
+{
+    if (!q1.is_cuda()) return VQ_EDEVICE;
+    const c10::cuda::CUDAGuard guard(q1.device());
+    VqPagedAttentionArgs a{};
+    a.kv = paged_kv(k1, v_pages, k3, k1_scale, v_scale, k3_scale, table, cu_q, lens);
+    a.q1 = any_desc(q1); a.q2 = any_desc(q2); a.out = any_desc(out);
+    a.codebook = any_desc(codebook); a.cnt = any_desc(cnt); a.vsum = any_desc(vsum); a.snap_table = any_desc(snap_table);
+    a.window = window;
+    a.max_q = max_q;
+    a.scale = static_cast<float>(scale);
+    a.status_word = word_of(status_word);
+    return vqattn_paged_attention(&a, stream_of(q1));
+}
+
+// the raising forms
+template <auto F> struct Raising;
+template <typename... A, int64_t (*F)(A...)> struct Raising<F> {
+    static void call(A... args) { check(static_cast<int>(F(std::forward<A>(args)...)), "vqattn::paged"); }
+};
+
 int64_t abi_version() { return vqattn_version(); }
 
 }  // namespace
@@ -208,6 +311,22 @@ TORCH_LIBRARY(vqattn, m)
           "int n_valid, int n_bd, float scale, Tensor(a!) workspace, Tensor(b!) out, Tensor(c!)? status_word) -> ()");
     m.def("cache_advance(Tensor codes, Tensor v_new, int K, Tensor(a!) cnt, Tensor(b!) vsum_f32, Tensor(c!)? vsum_act, "
           "Tensor(d!)? status_word) -> ()");
+    m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k1, Tensor(b!) v_pages, Tensor(c!)? k3, Tensor(d!)? k1_scale, Tensor(e!)? v_scale, "
+          "Tensor(f!)? k3_scale, Tensor table, Tensor cu_q, Tensor lens, Tensor? q, Tensor(g!)? q1, Tensor(h!)? q2, Tensor? cos_tab, "
+          "Tensor? sin_tab, int const_pos, Tensor(i!)? status_word) -> ()");
+    m.def("paged_append_status(Tensor k, Tensor v, Tensor(a!) k1, Tensor(b!) v_pages, Tensor(c!)? k3, Tensor(d!)? k1_scale, Tensor(e!)? v_scale, "
+          "Tensor(f!)? k3_scale, Tensor table, Tensor cu_q, Tensor lens, Tensor? q, Tensor(g!)? q1, Tensor(h!)? q2, Tensor? cos_tab, "
+          "Tensor? sin_tab, int const_pos, Tensor(i!)? status_word) -> int");
+    m.def("paged_read(Tensor pool0, Tensor? scale0, Tensor(a!) out0, Tensor? pool1, Tensor? scale1, Tensor(b!)? out1, Tensor? pool2, Tensor? scale2, "
+          "Tensor(c!)? out2, Tensor table, Tensor start, Tensor lens, Tensor(d!)? status_word) -> ()");
+    m.def("paged_read_status(Tensor pool0, Tensor? scale0, Tensor(a!) out0, Tensor? pool1, Tensor? scale1, Tensor(b!)? out1, Tensor? pool2, Tensor? scale2, "
+          "Tensor(c!)? out2, Tensor table, Tensor start, Tensor lens, Tensor(d!)? status_word) -> int");
+    m.def("paged_attention(Tensor q1, Tensor q2, Tensor k1, Tensor v_pages, Tensor? k3, Tensor? k1_scale, Tensor? v_scale, Tensor? k3_scale, Tensor table, "
+          "Tensor cu_q, Tensor lens, Tensor? codebook, Tensor? cnt, Tensor? vsum, Tensor? snap_table, int window, int max_q, float scale, "
+          "Tensor(a!) out, Tensor(b!)? status_word) -> ()");
+    m.def("paged_attention_status(Tensor q1, Tensor q2, Tensor k1, Tensor v_pages, Tensor? k3, Tensor? k1_scale, Tensor? v_scale, Tensor? k3_scale, Tensor table, "
+          "Tensor cu_q, Tensor lens, Tensor? codebook, Tensor? cnt, Tensor? vsum, Tensor? snap_table, int window, int max_q, float scale, "
+          "Tensor(a!) out, Tensor(b!)? status_word) -> int");
 }
 
 TORCH_LIBRARY_IMPL(vqattn, CUDA, m)
@@ -217,4 +336,10 @@ TORCH_LIBRARY_IMPL(vqattn, CUDA, m)
     m.impl("prefill", &prefill);
     m.impl("decode", &decode);
     m.impl("cache_advance", &cache_advance);
+    m.impl("paged_append", &Raising<&paged_append_status>::call);
+    m.impl("paged_append_status", &paged_append_status);
+    m.impl("paged_read", &Raising<&paged_read_status>::call);
+    m.impl("paged_read_status", &paged_read_status);
+    m.impl("paged_attention", &Raising<&paged_attention_status>::call);
+    m.impl("paged_attention_status", &paged_attention_status);
 }

@@ -17,6 +17,12 @@ that kernels raise on an expired bounded wait or a bad code):
     prefill(q1, q2, k1, k3, v, codebook?, cnt?, vsum?, window, scale, impl, out!, lse2!?, status_word?)
     decode(q1, q2, k1_win, k3_win, v_win, codebook?, cnt?, vsum?, n_valid, n_bd, scale, workspace!, out!, status_word?)
     cache_advance(codes, v_new, K, cnt!, vsum_f32!, vsum_act!?, status_word?)
+    paged_append(k, v, k1!, v_pages!, k3!?, k1_scale!?, v_scale!?, k3_scale!?, table, cu_q, lens, q?, q1!?, q2!?, cos_tab?, sin_tab?,
+                 const_pos, status_word?)
+    paged_read(pool0, scale0?, out0!, pool1?, scale1?, out1!?, pool2?, scale2?, out2!?, table, start, lens, status_word?)
+    paged_attention(q1, q2, k1, v_pages, k3?, k1_scale?, v_scale?, k3_scale?, table, cu_q, lens, codebook?, cnt?, vsum?, snap_table?,
+                    window, max_q, scale, out!, status_word?)
+    paged_*_status(...): the same, returning the C status instead of raising
     abi_version(), assign_workspace_bytes(...), aggregates_workspace_bytes(...), decode_workspace_bytes(...)
 """
 from __future__ import annotations
@@ -28,7 +34,8 @@ import torch
 from . import native  # loads libvqattn.so first and fails loudly when it is missing
 
 LIB = Path(__file__).resolve().parent / "lib" / "libvqattn_torch.so"
-_MUTATING = ("assign_codes", "build_aggregates", "prefill", "decode", "cache_advance")
+_PAGED = ("paged_append", "paged_read", "paged_attention")
+_MUTATING = ("assign_codes", "build_aggregates", "prefill", "decode", "cache_advance") + _PAGED
 _loaded = False
 
 
@@ -44,9 +51,28 @@ def load():
         # shape propagation for tracing: the operators return nothing and only write into their arguments
         for name in _MUTATING:
             torch.library.register_fake(f"vqattn::{name}")(_nothing)
+        for name in _PAGED:
+            torch.library.register_fake(f"vqattn::{name}_status")(_ok)
         _loaded = True
     return torch.ops.vqattn
 
 
 def _nothing(*args, **kwargs):
     return None
+
+
+def _ok(*args, **kwargs):
+    return 0
+
+
+def paged_calls():
+    """The status forms of the paged operators, loaded once: what ``api.paged_*`` calls (describing some fifteen tensors in C++ takes 1 us,
+    from Python 30)."""
+    global _calls
+    if _calls is None:
+        ops = load()
+        _calls = tuple(getattr(ops, f"{name}_status").default for name in _PAGED)
+    return _calls
+
+
+_calls = None
