@@ -5,20 +5,24 @@
 // matrix product only has to keep out of its way: mma.sync with the KEYS on the M axis (16 per instruction) and 8 query rows on N, for
 // which a tile of 128 rows of tcgen05 would be nearly empty.  A warp takes steps of 16 keys (32 of 8-bit rows) and keeps its own online
 // softmax: no barrier in the loop.
-//   - Both products may permute their reduction index: a thread reads 16 contiguous bytes of a key row, which hold its operands of
-//     several k-steps, and q is read in the same order.  Values enter as V^T (D on M): pairs of keys are interleaved by byte permutes.
-//     So every thread copies exactly the bytes it will use (cp.async, a private FIFO in shared memory): no shared layout, no ldmatrix, not
-//     even a warp barrier between copy and use.
+//   - A warp's keys and values arrive by TMA, 16 rows a box, in a FIFO of its own (barriers of its own, no CTA barrier).  Both products may
+//     permute their reduction index: a thread reads 16 contiguous bytes of a swizzled key row, which hold its operands of several k-steps, and q
+//     is read in the same order.  Values enter as V^T (D on M): pairs of keys are interleaved by byte permutes.
 //   - S^T (keys x rows) becomes the B operand of the second product by movmatrix, 8 x 8 at a time.
-//   - 8-bit codes become 16-bit floats exactly (byte permutes and one subtraction); a key's scale multiplies its score, a value's scale its
-//     weight.
+//   - 8-bit keys stay bytes: the query rows become 16-bit fixed point numbers (largest element 32639), high and low byte each a factor of an
+//     integer product, which is exact.  An element of q is off by 2^-16 of its row's largest at most - bf16 already rounds elements
+//     near the largest by 2^-9 of it - and the keys need no conversion, which was a third of the kernel's instructions.
+//     8-bit values become 16-bit floats exactly (byte permutes and one subtraction).  A key's scale multiplies its score, a value's
+//     scale its weight.
 //   - Counts multiply the weights of codes in the denominator; codes without members are excluded.
 // One unit = (sequence, block of positions, kv head); its steps are dealt out to the warps of a cluster of 1 - 8 CTAs, which merge their
 // partial sums through distributed shared memory: no workspace, no second launch, the same order of additions every time.
 #include <cooperative_groups.h>
+#include <type_traits>
 
 #include "codes8.cuh"
 #include "paged_attn.cuh"
+#include "prefill_tc_common.cuh"
 #include "tc_ptx.cuh"
 
 namespace vq {
@@ -50,32 +54,24 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x)
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// copies N bytes, or zeros when !some
-template <int N>
-__device__ __forceinline__ void cp_async(void *dst, const void *src, bool some)
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    if constexpr (N == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(some ? 16 : 0) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(ptx::smem_u32(dst)), "l"(src), "n"(N), "r"(some ? N : 0) : "memory");
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 template <typename T, bool Q8, int D, int NT>
 struct FewCfg {
     static constexpr int kCols = 8 * NT;                         // query rows, padded
-    static constexpr int KC = D / 32, VC = D / 64;               // 16-byte pieces of a 16-bit key / value row per thread
-    static constexpr int kSlots16 = 2 * KC + 4 * VC;             // 16-byte slots per thread: 16 keys of 16-bit rows
-    static constexpr int kSlots8 = 2 * (2 * VC + 4);             // 32 keys of 8-bit rows
-    static constexpr int kSlots = Q8 && kSlots8 > kSlots16 ? kSlots8 : kSlots16;
-    static constexpr int kStage = kSlots * 32 * 16;              // bytes of a stage: 16 keys, or 32 of 8-bit rows
-    static constexpr int kScal = (Q8 ? 8 : 2) * 32 * 4;          // counts, or scales of keys and values
-    static constexpr int kWarpBytes = kFewStages * (kStage + kScal);
-    static constexpr int kQ = 2 * kCols * D * 2;                 // q1 and q2 rows
-    static constexpr int kPages = Q8 ? 64 : 512;                 // page table entries kept in shared memory (the rest is read where it is
-                                                                 // needed): 8-bit rows leave no more if two CTAs are to share an SM
-    static constexpr int kTotal = kFewWarps * kWarpBytes + kQ + kPages * 4;
+    static constexpr int VC = D / 64;                            // boxes of 64 columns of a 16-bit row
+    static constexpr int kBox = 16 * 128;                        // bytes of 16 rows x 64 columns of 16 bits
+    static constexpr int kBox8 = 16 * D;                         // 16 rows of 8 bits
+    static constexpr int kStage = 2 * VC * kBox;                 // 16 keys with their values, or 32 of 8 bits
+    static_assert(4 * kBox8 == kStage, "a stage holds twice as many 8-bit rows");
+    static constexpr int kWarpBytes = kFewStages * kStage;
+    static constexpr int kQ8 = kCols * D;                        // one byte plane of the rows
+    static constexpr int kQ = Q8 ? kCols * D * 2 + 4 * kQ8 : 2 * kCols * D * 2;   // 16-bit rows q1, q2; or q2, and both kinds in two planes
+    static constexpr int kPages = 256;                           // page table entries kept in shared memory; the rest is read where it is needed
+    static constexpr int kTotal = kFewWarps * kWarpBytes + kQ + kPages * 4 + 1024;   // + slack for 1024-byte alignment
     static_assert(kCols * D * 4 <= kFewStages * kStage, "a warp's sums fit into its FIFO");
     static constexpr int MT = D / 16;
 };
@@ -86,17 +82,23 @@ struct FewSteps {
 };
 
 template <typename T, bool Q8, int D, int NT>
-__global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAttnParams p, int groups, int nsplit)
+__global__ void __launch_bounds__(kFewWarps * 32, 2) paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constant__ CUtensorMap tm_k3, const __grid_constant__ CUtensorMap tm_v,
+                 const __grid_constant__ CUtensorMap tm_cb, const __grid_constant__ CUtensorMap tm_vs, const PagedAttnParams p, int groups, int nsplit)
 {
     using C = FewCfg<T, Q8, D, NT>;
     using M = Mma16816<T>;
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ __align__(8) uint64_t s_bar[kFewWarps][kFewStages];
+    __shared__ int s_bad;                                            // some page of the unit is missing, or not kept in shared memory
     __shared__ float s_m[kFewWarps][C::kCols], s_l[kFewWarps][C::kCols];
     __shared__ float s_cm[C::kCols], s_cl[C::kCols];
+    __shared__ float s_unit[2][Q8 ? C::kCols : 1];                   // what the fixed point rows count in
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int r = lane >> 2, c = lane & 3;
     uint8_t *fifo = smem + warp * C::kWarpBytes;
     T *s_q = reinterpret_cast<T *>(smem + kFewWarps * C::kWarpBytes);        // [2][kCols][D]
+    uint8_t *s_q8 = smem + kFewWarps * C::kWarpBytes + C::kCols * D * 2;     // 8-bit rows: [q1, q2][high, low byte][kCols][D]
     int *s_page = reinterpret_cast<int *>(smem + kFewWarps * C::kWarpBytes + C::kQ);
 
     const int split = blockIdx.x % nsplit;
@@ -128,16 +130,62 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAt
     const int total = st.n_far + st.n_old + st.n_near;
     const int col0 = bd >> p.seqs.log_p, cols = (i1 >> p.seqs.log_p) - col0 + 1;
 
-    for (int x = tid; x < min(cols, C::kPages); x += kFewWarps * 32) s_page[x] = p.seqs.page(s, col0 + x);
-    for (int x = tid; x < 2 * C::kCols * D / 8; x += kFewWarps * 32) {
-        const int which = x / (C::kCols * D / 8), row = x / (D / 8) % C::kCols, d = x % (D / 8) * 8;
+    if (tid == 0) {
+        for (int w = 0; w < kFewWarps; ++w)
+            for (int x = 0; x < kFewStages; ++x) ptx::mbar_init(&s_bar[w][x], 1);
+        ptx::fence_mbar_init();
+        s_bad = cols > C::kPages;
+    }
+    __syncthreads();
+    for (int x = tid; x < min(cols, C::kPages); x += kFewWarps * 32) {
+        s_page[x] = p.seqs.page(s, col0 + x);
+        if (s_page[x] < 0) s_bad = 1;
+    }
+    // ---- query rows.  Rows behind `rows` are zeros.
+    auto q_row = [&](int which, int row) {
+        const int64_t t = t0 + row / p.G, h = hk * p.G + row % p.G;
+        return which ? static_cast<const T *>(p.q2) + t * p.q2_t + h * p.q2_h : static_cast<const T *>(p.q1) + t * p.q1_t + h * p.q1_h;
+    };
+    for (int x = tid; x < (Q8 ? 1 : 2) * C::kCols * D / 8; x += kFewWarps * 32) {
+        const int which = Q8 ? 1 : x / (C::kCols * D / 8), row = x / (D / 8) % C::kCols, d = x % (D / 8) * 8;
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < rows) {
-            const int64_t t = t0 + row / p.G, h = hk * p.G + row % p.G;
-            const T *src = which ? static_cast<const T *>(p.q2) + t * p.q2_t + h * p.q2_h : static_cast<const T *>(p.q1) + t * p.q1_t + h * p.q1_h;
-            v = *reinterpret_cast<const uint4 *>(src + d);
-        }
+        if (row < rows) v = *reinterpret_cast<const uint4 *>(q_row(which, row) + d);
         reinterpret_cast<uint4 *>(s_q)[x] = v;
+    }
+    if constexpr (Q8) {                                              // fixed point: v = 256 hi + lo
+        for (int x = warp; x < 2 * C::kCols; x += kFewWarps) {
+            const int which = x / C::kCols, row = x % C::kCols;
+            float e[D / 32], top = 0.f, unit = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) e[i] = row < rows ? to_f32(q_row(which, row)[lane * (D / 32) + i]) : 0.f;
+            bool finite = true;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                top = fmaxf(top, fabsf(e[i]));
+                finite = finite && fabsf(e[i]) < INFINITY;
+            }
+#pragma unroll
+            for (int y = 16; y; y >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, y));
+            unit = top * (1.f / 32639.f);
+            const float inv = unit >= 1.17549435e-38f ? __frcp_rn(unit) : 0.f;
+            uint32_t hi = 0, lo = 0;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                const int v = min(32639, max(-32639, __float2int_rn(e[i] * inv))), h = (v + 128) >> 8;
+                hi |= (static_cast<uint32_t>(h) & 255u) << (8 * i);
+                lo |= (static_cast<uint32_t>(v - 256 * h) & 255u) << (8 * i);
+            }
+            uint8_t *dst = s_q8 + 2 * which * C::kQ8 + row * D + lane * (D / 32);
+            if constexpr (D == 128) {
+                *reinterpret_cast<uint32_t *>(dst) = hi;
+                *reinterpret_cast<uint32_t *>(dst + C::kQ8) = lo;
+            } else {
+                *reinterpret_cast<uint16_t *>(dst) = static_cast<uint16_t>(hi);
+                *reinterpret_cast<uint16_t *>(dst + C::kQ8) = static_cast<uint16_t>(lo);
+            }
+            if (lane == 0) s_unit[which][row] = __all_sync(~0u, finite) ? unit : __int_as_float(0x7fffffff);
+            else __all_sync(~0u, finite);
+        }
     }
     __syncthreads();
 
@@ -147,110 +195,97 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAt
         const int x = (j >> p.seqs.log_p) - col0;
         return x < C::kPages ? s_page[x] : p.seqs.page(s, x + col0);
     };
-    // ---- the thread's share of a step, into stage `slot`
+    const bool bad = s_bad;
+    auto first_key = [&](int step) {
+        return step < st.n_far + st.n_old ? st.old0 + (step - st.n_far) * KEYS : st.near0 + (step - st.n_far - st.n_old) * KEYS;
+    };
+    // ---- keys and values of a step into stage `slot`, by one thread.  Missing pages (reported) bring nothing.
     auto fill = [&](int step, int slot) {
         uint8_t *dst = fifo + slot * C::kStage;
-        float *sc = reinterpret_cast<float *>(fifo + kFewStages * C::kStage + slot * C::kScal);
+        uint64_t *bar = &s_bar[warp][slot];
         if (step < st.n_far) {
-            const int r0 = step * 16;
-            const T *kb = static_cast<const T *>(p.cb) + (static_cast<int64_t>(hk) * p.MK + r0) * D;
-            const T *vb = static_cast<const T *>(p.vsum) + (far_base + r0) * D;
-            int x = 0;
+            ptx::mbar_expect_tx(bar, C::kStage);
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int j = 0; j < C::KC; ++j, ++x) cp_async<16>(dst + (x * 32 + lane) * 16, kb + (r + 8 * a) * D + 32 * j + 8 * c, true);
-#pragma unroll
-            for (int a = 0; a < 4; ++a)
-#pragma unroll
-                for (int j = 0; j < C::VC; ++j, ++x)
-                    cp_async<16>(dst + (x * 32 + lane) * 16, vb + (2 * c + (a & 1) + 8 * (a >> 1)) * D + 64 * j + 8 * r, true);
-#pragma unroll
-            for (int a = 0; a < 2; ++a) cp_async<4>(sc + a * 32 + lane, p.cnt + far_base + r0 + r + 8 * a, true);
+            for (int h = 0; h < C::VC; ++h) {
+                ptx::tma_load_3d(dst + h * C::kBox, &tm_cb, bar, 64 * h, step * 16, hk);
+                ptx::tma_load_3d(dst + (C::VC + h) * C::kBox, &tm_vs, bar, 64 * h, step * 16, snap * p.Hkv + hk);
+            }
             return;
         }
-        const bool old = step < st.n_far + st.n_old;
-        const int key0 = old ? st.old0 + (step - st.n_far) * KEYS : st.near0 + (step - st.n_far - st.n_old) * KEYS;
-        const PagedPool &kp = old ? p.k3 : p.k1;
-        int x = 0;
+        const CUtensorMap *tm = step < st.n_far + st.n_old ? &tm_k3 : &tm_k1;
+        const int key0 = first_key(step);
+        int pg[KEYS / 16], some = 0;
 #pragma unroll
-        for (int sub = 0; sub < KEYS / 16; ++sub) {
-            const int j0 = key0 + 16 * sub;
-            const int pg = j0 <= i1 ? page_of(j0) : -1;               // none: zeros, whose keys are masked (or reported)
-            const bool have = pg >= 0;
-            const int pr = j0 & page_mask, page = have ? pg : 0;
-            if constexpr (!Q8) {
-                const T *kb = static_cast<const T *>(kp.ptr) + kp.row(page, hk, pr), *vb = static_cast<const T *>(p.v.ptr) + p.v.row(page, hk, pr);
+        for (int u = 0; u < KEYS / 16; ++u) {
+            pg[u] = key0 + 16 * u <= i1 ? page_of(key0 + 16 * u) : -1;
+            some += pg[u] >= 0;
+        }
+        ptx::mbar_expect_tx(bar, some * (C::kStage / (KEYS / 16)));
 #pragma unroll
-                for (int a = 0; a < 2; ++a)
-#pragma unroll
-                    for (int j = 0; j < C::KC; ++j, ++x) cp_async<16>(dst + (x * 32 + lane) * 16, kb + (r + 8 * a) * kp.s_row + 32 * j + 8 * c, have);
-#pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const int key = 2 * c + (a & 1) + 8 * (a >> 1);
-#pragma unroll
-                    for (int j = 0; j < C::VC; ++j, ++x)              // behind the sequence's end a page may hold anything: zeros instead
-                        cp_async<16>(dst + (x * 32 + lane) * 16, vb + key * p.v.s_row + 64 * j + 8 * r, have && j0 + key < n);
-                }
+        for (int u = 0; u < KEYS / 16; ++u) {
+            const int pr = (key0 + 16 * u) & page_mask;
+            if (pg[u] < 0) continue;
+            if constexpr (Q8) {
+                ptx::tma_load_4d(dst + 2 * u * C::kBox8, tm, bar, 0, pr, hk, pg[u]);
+                ptx::tma_load_4d(dst + (2 * u + 1) * C::kBox8, &tm_v, bar, 0, pr, hk, pg[u]);
             } else {
-                const int8_t *kb = static_cast<const int8_t *>(kp.ptr) + kp.row(page, hk, pr), *vb = static_cast<const int8_t *>(p.v.ptr) + p.v.row(page, hk, pr);
 #pragma unroll
-                for (int a = 0; a < 2; ++a)
-#pragma unroll
-                    for (int j = 0; j < D / 64; ++j, ++x) cp_async<16>(dst + (x * 32 + lane) * 16, kb + (r + 8 * a) * kp.s_row + 64 * j + 16 * c, have);
-#pragma unroll
-                for (int a = 0; a < 4; ++a, ++x) {
-                    const int key = 2 * c + (a & 1) + 8 * (a >> 1);
-#pragma unroll
-                    for (int j = 0; j < C::VC; ++j) cp_async<8>(dst + (x * 32 + lane) * 16 + 8 * j, vb + key * p.v.s_row + 64 * j + 8 * r, have);
-                }
-                const float *ks = kp.scale + kp.scale_at(page, hk, pr), *vs = p.v.scale + p.v.scale_at(page, hk, pr);
-#pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const bool in = have && j0 + r + 8 * a < n;
-                    cp_async<4>(sc + (4 * sub + a) * 32 + lane, ks + (r + 8 * a) * kp.c_row, in);
-                    cp_async<4>(sc + (4 * sub + 2 + a) * 32 + lane, vs + (r + 8 * a) * p.v.c_row, in);
+                for (int h = 0; h < C::VC; ++h) {
+                    ptx::tma_load_4d(dst + h * C::kBox, tm, bar, 64 * h, pr, hk, pg[u]);
+                    ptx::tma_load_4d(dst + (C::VC + h) * C::kBox, &tm_v, bar, 64 * h, pr, hk, pg[u]);
                 }
             }
         }
     };
+    // ---- what goes with the rows: lane l has the count of code l, or the scales of key l and of its value
+    auto extras = [&](int step, float &x, float &y) {
+        x = y = 0.f;
+        if (step >= total) return;
+        if (step < st.n_far) {
+            x = __ldg(p.cnt + far_base + step * 16 + (lane & 15));
+        } else if constexpr (Q8) {
+            const int j = first_key(step) + lane, pg = j < n && j <= (i1 | 15) ? page_of(j) : -1, pr = j & page_mask;
+            const PagedPool &kp = step < st.n_far + st.n_old ? p.k3 : p.k1;
+            if (pg >= 0) {
+                x = __ldg(kp.scale + kp.scale_at(pg, hk, pr));
+                y = __ldg(p.v.scale + p.v.scale_at(pg, hk, pr));
+            }
+        }
+    };
 
-    float o[NT][C::MT][4], m[NT][2], l[NT][2];
+    float o[NT][C::MT][4], m[NT][2], lim[NT][2], l[NT][2], qu[NT][2];   // lim: the score that raises the reference m
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int mt = 0; mt < C::MT; ++mt)
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[nt][mt][x] = 0.f;
-        m[nt][0] = m[nt][1] = -INFINITY;
+        m[nt][0] = m[nt][1] = lim[nt][0] = lim[nt][1] = -INFINITY;
+        qu[nt][0] = qu[nt][1] = 0.f;
         l[nt][0] = l[nt][1] = 0.f;
     }
     uint32_t qf[NT][D / 8];
 
     const int stride = nsplit * kFewWarps, first = split * kFewWarps + warp;
 #pragma unroll
-    for (int x = 0; x < kFewStages - 1; ++x) {
-        if (first + x * stride < total) fill(first + x * stride, x);
-        cp_commit();
-    }
-    // positions of the thread's columns
-    int pos[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) pos[nt][x] = i0 + (8 * nt + 2 * c + x) / p.G;
-
-    // sc: scores of keys r and r + 8 (c0 c1 | c2 c3) in log2 units, -inf where excluded -> weights; w: denominator weights of the two keys,
-    // f: factors of their value rows.  Raises the references, adds to l, returns the packed weights as B operands.
-    auto softmax = [&](float (&sc)[NT][4], float w0, float w1, float f0, float f1, uint32_t (&pb)[NT][2]) {
+    for (int x = 0; x < kFewStages - 1; ++x)
+        if (first + x * stride < total && ptx::elect_one()) fill(first + x * stride, x);
+    float next_x, next_y;
+    extras(first, next_x, next_y);
+    // sc: scores of keys r and r + 8 of each group of 16 (c0 c1 | c2 c3) in log2 units, -inf where excluded -> weights; w: denominator weights of
+    // the two keys, f: factors of their value rows.  Raises the references, adds to l, returns the packed weights as B operands.
+    auto softmax = [&](auto &sc, const auto &w, const auto &f, auto &pb) {
+        constexpr int SUBS = sizeof(sc) / sizeof(sc[0]);
         bool above = false;
         float mx[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                mx[nt][x] = fmaxf(sc[nt][x], sc[nt][2 + x]);
-                above |= mx[nt][x] > m[nt][x] + kFewLazy || (m[nt][x] == -INFINITY && mx[nt][x] > -INFINITY);
+                mx[nt][x] = fmaxf(sc[0][nt][x], sc[0][nt][2 + x]);
+#pragma unroll
+                for (int u = 1; u < SUBS; ++u) mx[nt][x] = ptx::fmax3(mx[nt][x], sc[u][nt][x], sc[u][nt][2 + x]);
+                above |= mx[nt][x] > lim[nt][x];
             }
         if (__any_sync(~0u, above)) {
 #pragma unroll
@@ -263,6 +298,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAt
                     if (v > m[nt][x]) {
                         const float a = m[nt][x] == -INFINITY ? 0.f : ptx::ex2(m[nt][x] - v);
                         m[nt][x] = v;
+                        lim[nt][x] = v + kFewLazy;
                         l[nt][x] *= a;
 #pragma unroll
                         for (int mt = 0; mt < C::MT; ++mt) {
@@ -275,185 +311,235 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAt
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const float ma = m[nt][0] == -INFINITY ? 0.f : m[nt][0], mb = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-            const float p0 = ptx::ex2(sc[nt][0] - ma), p1 = ptx::ex2(sc[nt][1] - mb), p2 = ptx::ex2(sc[nt][2] - ma), p3 = ptx::ex2(sc[nt][3] - mb);
-            l[nt][0] += p0 * w0 + p2 * w1;
-            l[nt][1] += p1 * w0 + p3 * w1;
-            pb[nt][0] = movmatrix(Pair16<T>::pack(p0 * f0, p1 * f0));
-            pb[nt][1] = movmatrix(Pair16<T>::pack(p2 * f1, p3 * f1));
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) {
+                const float p0 = ptx::ex2(sc[u][nt][0] - ma), p1 = ptx::ex2(sc[u][nt][1] - mb), p2 = ptx::ex2(sc[u][nt][2] - ma), p3 = ptx::ex2(sc[u][nt][3] - mb);
+                l[nt][0] += p0 * w[u][0] + p2 * w[u][1];
+                l[nt][1] += p1 * w[u][0] + p3 * w[u][1];
+                pb[u][nt][0] = movmatrix(Pair16<T>::pack(p0 * f[u][0], p1 * f[u][0]));
+                pb[u][nt][1] = movmatrix(Pair16<T>::pack(p2 * f[u][1], p3 * f[u][1]));
+            }
         }
+    };
+    // excluded keys of the 16 from j0 on; true: there is no such page
+    auto mask = [&](float (&sc)[NT][4], int j0, bool old) {
+        if (bad && j0 <= i1 && page_of(j0) < 0) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) sc[nt][x] = -INFINITY;
+            return true;
+        }
+        // what every row of the group sees: raw keys below i0 - W, rotated ones in [i1 - W, i0]
+        const bool all = old ? j0 + 15 < i0 - p.W : j0 + 15 <= i0 && (!p.rerope || j0 >= i1 - p.W);
+        if (all) return false;
+        const int ja = j0 + r, jb = ja + 8;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int i = i0 + (8 * nt + 2 * c + x) / p.G, hi = old ? i - p.W - 1 : i, lo = old || !p.rerope ? bd : i - p.W;
+                if (ja < lo || ja > hi || ja >= n) sc[nt][x] = -INFINITY;
+                if (jb < lo || jb > hi || jb >= n) sc[nt][2 + x] = -INFINITY;
+            }
+        return false;
     };
 
     int phase = -1, slot = 0;
+    uint32_t par = 0;
+    bool failed = false;
     for (int step = first; step < total; step += stride) {
+        __syncwarp();                                                // the stage of the step before has been consumed by every lane
         {
-            const int next = step + (kFewStages - 1) * stride;
-            int ns = slot + kFewStages - 1;
-            if (ns >= kFewStages) ns -= kFewStages;
-            if (next < total) fill(next, ns);
-            cp_commit();
+            const int next = step + (kFewStages - 1) * stride, ns = slot == 0 ? kFewStages - 1 : slot - 1;
+            if (next < total && ptx::elect_one()) fill(next, ns);
         }
         const bool far = step < st.n_far, old = !far && step < st.n_far + st.n_old;
         const int ph = far ? 0 : old ? 1 : 2;
         if (ph != phase) {                                           // q in the order of this phase's key rows
             phase = ph;
-            const T *src = s_q + ((far || old) ? C::kCols * D : 0);
+            if (Q8 && !far) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const T *row = src + (8 * nt + r) * D;
-                if (far || !Q8) {
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint8_t *row = s_q8 + (old ? 2 * C::kQ8 : 0) + (8 * nt + r) * D + 16 * C::VC * c;
 #pragma unroll
-                    for (int j = 0; j < C::KC; ++j) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(row + 32 * j + 8 * c);
-                        qf[nt][4 * j] = v.x; qf[nt][4 * j + 1] = v.y; qf[nt][4 * j + 2] = v.z; qf[nt][4 * j + 3] = v.w;
+                    for (int j = 0; j < C::VC; ++j) {
+                        const uint4 h = *reinterpret_cast<const uint4 *>(row + 16 * j), e = *reinterpret_cast<const uint4 *>(row + C::kQ8 + 16 * j);
+                        qf[nt][8 * j] = h.x; qf[nt][8 * j + 1] = h.y; qf[nt][8 * j + 2] = h.z; qf[nt][8 * j + 3] = h.w;
+                        qf[nt][8 * j + 4] = e.x; qf[nt][8 * j + 5] = e.y; qf[nt][8 * j + 6] = e.z; qf[nt][8 * j + 7] = e.w;
                     }
-                } else {
 #pragma unroll
-                    for (int j = 0; j < C::KC; ++j) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(row + 64 * (j / 2) + 16 * c + 8 * (j % 2));
-                        qf[nt][4 * j] = v.x; qf[nt][4 * j + 1] = v.y; qf[nt][4 * j + 2] = v.z; qf[nt][4 * j + 3] = v.w;
-                    }
+                    for (int x = 0; x < 2; ++x) qu[nt][x] = s_unit[old][8 * nt + 2 * c + x] * p.scale_log2;
                 }
+            } else {
+                const T *src = s_q + (!Q8 && (far || old) ? C::kCols * D : 0);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 2 * C::VC; ++j) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(src + (8 * nt + r) * D + 64 * (j / 2) + 16 * c + 8 * (j % 2));
+                        qf[nt][4 * j] = v.x; qf[nt][4 * j + 1] = v.y; qf[nt][4 * j + 2] = v.z; qf[nt][4 * j + 3] = v.w;
+                    }
             }
         }
-        cp_wait<kFewStages - 1>();
-        const uint8_t *stg = fifo + slot * C::kStage + lane * 16;
-        const float *scal = reinterpret_cast<const float *>(fifo + kFewStages * C::kStage + slot * C::kScal) + lane;
-        if (++slot == kFewStages) slot = 0;
-        const int subs = far || !Q8 ? 1 : 2;
-#pragma unroll 1
-        for (int sub = 0; sub < subs; ++sub) {
-            // ---- S^T = K Q^T
-            float sc[NT][4];
+        const float my_x = next_x, my_y = next_y;
+        extras(step + stride, next_x, next_y);
+        const uint8_t *stg = fifo + slot * C::kStage;
+        if (!__all_sync(~0u, ptx::mbar_wait(&s_bar[warp][slot], par, p.wait_limit))) {
+            failed = true;
+            break;
+        }
+        if (++slot == kFewStages) {
+            slot = 0;
+            par ^= 1u;
+        }
+        const int key0 = first_key(step);
+        if (far || !Q8) {
+            // ---- S^T = K Q^T, even and odd k-steps by themselves.  Piece j of row k lies at j ^ (k % 8); four lanes share a row, each
+            // takes two neighbouring pieces of its 128 bytes: the eight lanes that read together ask for different banks.
+            float sc[1][NT][4], s2[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) sc[nt][x] = 0.f;
-            float w0 = 1.f, w1 = 1.f, f0 = 1.f, f1 = 1.f, k0 = p.scale_log2, k1 = p.scale_log2, e0 = 1.f, e1 = 1.f;
-            const uint8_t *kst = stg;
-            if (far || !Q8) {
+                for (int x = 0; x < 4; ++x) sc[0][nt][x] = s2[nt][x] = 0.f;
 #pragma unroll
-                for (int j = 0; j < C::KC; ++j) {
-                    const uint4 a = *reinterpret_cast<const uint4 *>(kst + j * 512), b = *reinterpret_cast<const uint4 *>(kst + (C::KC + j) * 512);
+            for (int h = 0; h < C::VC; ++h)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const uint8_t *at = stg + h * C::kBox + r * 128 + (((2 * c + y) ^ r) << 4);
+                    const uint4 a = *reinterpret_cast<const uint4 *>(at), b = *reinterpret_cast<const uint4 *>(at + 8 * 128);
+                    const int j = 2 * h + y;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        M::mma(sc[nt], a.x, b.x, a.y, b.y, qf[nt][4 * j], qf[nt][4 * j + 1]);
-                        M::mma(sc[nt], a.z, b.z, a.w, b.w, qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
+                        M::mma(sc[0][nt], a.x, b.x, a.y, b.y, qf[nt][4 * j], qf[nt][4 * j + 1]);
+                        M::mma(s2[nt], a.z, b.z, a.w, b.w, qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
                     }
                 }
-                if (far) {
-                    w0 = scal[0];
-                    w1 = scal[32];
-                }
-            } else {
-                kst += sub * (2 * (D / 64) + 4) * 512;
 #pragma unroll
-                for (int j = 0; j < D / 64; ++j) {
-                    const uint4 a4 = *reinterpret_cast<const uint4 *>(kst + j * 512), b4 = *reinterpret_cast<const uint4 *>(kst + (D / 64 + j) * 512);
-                    const uint32_t a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t al, ah, bl, bh;
-                        Codes8<T>::expand(a[w], al, ah);
-                        Codes8<T>::expand(b[w], bl, bh);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) M::mma(sc[nt], al, bl, ah, bh, qf[nt][8 * j + 2 * w], qf[nt][8 * j + 2 * w + 1]);
-                    }
-                }
-                const float *s4 = scal + 4 * sub * 32;
-                k0 *= s4[0];
-                k1 *= s4[32];
-                f0 = s4[64];
-                f1 = s4[96];
-                if constexpr (kHalf) {
-                    f0 = half_weight_factor(f0, e0);
-                    f1 = half_weight_factor(f1, e1);
-                }
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                sc[nt][0] *= k0; sc[nt][1] *= k0; sc[nt][2] *= k1; sc[nt][3] *= k1;
-            }
-            // ---- excluded keys
+                for (int x = 0; x < 4; ++x) sc[0][nt][x] = (sc[0][nt][x] + s2[nt][x]) * p.scale_log2;
+            float w[1][2] = {{1.f, 1.f}};
+            const float f[1][2] = {{1.f, 1.f}};
+            bool hole = false;
             if (far) {
+                w[0][0] = __shfl_sync(~0u, my_x, r);
+                w[0][1] = __shfl_sync(~0u, my_x, r + 8);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    if (!(w0 > 0.f)) sc[nt][0] = sc[nt][1] = -INFINITY;
-                    if (!(w1 > 0.f)) sc[nt][2] = sc[nt][3] = -INFINITY;
+                    if (!(w[0][0] > 0.f)) sc[0][nt][0] = sc[0][nt][1] = -INFINITY;
+                    if (!(w[0][1] > 0.f)) sc[0][nt][2] = sc[0][nt][3] = -INFINITY;
                 }
             } else {
-                const int j0 = (old ? st.old0 + (step - st.n_far) * KEYS : st.near0 + (step - st.n_far - st.n_old) * KEYS) + 16 * sub;
-                // keys every row of the group sees: raw ones below i0 - W, rotated ones in [i1 - W, i0]
-                const bool all = old ? j0 + 15 < i0 - p.W : j0 + 15 <= i0 && (!p.rerope || j0 >= i1 - p.W);
-                if (!all) {
-                    const int ja = j0 + r, jb = ja + 8;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const int i = pos[nt][x], hi = old ? i - p.W - 1 : i, lo = old || !p.rerope ? bd : i - p.W;
-                            if (ja < lo || ja > hi || ja >= n) sc[nt][x] = -INFINITY;
-                            if (jb < lo || jb > hi || jb >= n) sc[nt][2 + x] = -INFINITY;
-                        }
-                }
+                hole = mask(sc[0], key0, old);
             }
-            uint32_t pb[NT][2];
-            softmax(sc, w0, w1, f0, f1, pb);
+            uint32_t pb[1][NT][2];
+            softmax(sc, w, f, pb);
             // ---- O^T += V^T P^T
-            if (far || !Q8) {
-                const uint8_t *vst = stg + 2 * C::KC * 512;
 #pragma unroll
-                for (int j = 0; j < C::VC; ++j) {
-                    uint4 v4[4];
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) v4[a] = *reinterpret_cast<const uint4 *>(vst + (a * C::VC + j) * 512);
-                    const uint32_t v0[4] = {v4[0].x, v4[0].y, v4[0].z, v4[0].w}, v1[4] = {v4[1].x, v4[1].y, v4[1].z, v4[1].w};
-                    const uint32_t v2[4] = {v4[2].x, v4[2].y, v4[2].z, v4[2].w}, v3[4] = {v4[3].x, v4[3].y, v4[3].z, v4[3].w};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t a0 = __byte_perm(v0[w], v1[w], 0x5410), a1 = __byte_perm(v0[w], v1[w], 0x7632);
-                        const uint32_t a2 = __byte_perm(v2[w], v3[w], 0x5410), a3 = __byte_perm(v2[w], v3[w], 0x7632);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) M::mma(o[nt][4 * j + w], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-                    }
-                }
-            } else {
-                const uint8_t *vst = stg + (sub * (2 * (D / 64) + 4) + 2 * (D / 64)) * 512;
-                uint32_t v[4][D / 32];
+            for (int h = 0; h < C::VC; ++h) {
+                uint4 v4[4];
 #pragma unroll
                 for (int a = 0; a < 4; ++a) {
-                    if constexpr (D == 128) {
-                        const uint4 x = *reinterpret_cast<const uint4 *>(vst + a * 512);
-                        v[a][0] = x.x; v[a][1] = x.y; v[a][2] = x.z; v[a][3] = x.w;
-                    } else {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(vst + a * 512);
-                        v[a][0] = x.x; v[a][1] = x.y;
+                    const int k = 2 * c + (a & 1) + 8 * (a >> 1);
+                    v4[a] = *reinterpret_cast<const uint4 *>(stg + (C::VC + h) * C::kBox + k * 128 + ((r ^ (k & 7)) << 4));
+                }
+                if (!far && (hole || key0 + 16 > n)) {               // behind the sequence's end a page may hold anything: zeros instead
+#pragma unroll
+                    for (int a = 0; a < 4; ++a)
+                        if (hole || key0 + 2 * c + (a & 1) + 8 * (a >> 1) >= n) v4[a] = make_uint4(0, 0, 0, 0);
+                }
+                const uint32_t v0[4] = {v4[0].x, v4[0].y, v4[0].z, v4[0].w}, v1[4] = {v4[1].x, v4[1].y, v4[1].z, v4[1].w};
+                const uint32_t v2[4] = {v4[2].x, v4[2].y, v4[2].z, v4[2].w}, v3[4] = {v4[3].x, v4[3].y, v4[3].z, v4[3].w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t a0 = __byte_perm(v0[x], v1[x], 0x5410), a1 = __byte_perm(v0[x], v1[x], 0x7632);
+                    const uint32_t a2 = __byte_perm(v2[x], v3[x], 0x5410), a3 = __byte_perm(v2[x], v3[x], 0x7632);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) M::mma(o[nt][4 * h + x], a0, a1, a2, a3, pb[0][nt][0], pb[0][nt][1]);
+                }
+            }
+        } else {
+            // 8-bit rows of 128 (64) bytes: piece j of row k lies at j ^ (k % 8)  (j ^ (k / 2 % 4))
+            auto piece = [&](int k, int j) { return D == 128 ? k * 128 + ((j ^ (k & 7)) << 4) : k * 64 + ((j ^ ((k >> 1) & 3)) << 4); };
+            float sc[2][NT][4], f[2][2], e[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
+            const float w[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                int hi[NT][4], lo[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) hi[nt][x] = lo[nt][x] = 0;
+#pragma unroll
+                for (int j = 0; j < C::VC; ++j) {
+                    const uint8_t *at = stg + 2 * u * C::kBox8;
+                    const uint4 a = *reinterpret_cast<const uint4 *>(at + piece(r, C::VC * c + j)), b = *reinterpret_cast<const uint4 *>(at + piece(r + 8, C::VC * c + j));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_s8(hi[nt], a.x, b.x, a.y, b.y, qf[nt][8 * j], qf[nt][8 * j + 1]);
+                        mma_s8(lo[nt], a.x, b.x, a.y, b.y, qf[nt][8 * j + 4], qf[nt][8 * j + 5]);
+                        mma_s8(hi[nt], a.z, b.z, a.w, b.w, qf[nt][8 * j + 2], qf[nt][8 * j + 3]);
+                        mma_s8(lo[nt], a.z, b.z, a.w, b.w, qf[nt][8 * j + 6], qf[nt][8 * j + 7]);
                     }
                 }
-                __half2 pa, pc;                                      // the powers of two that go with this thread's pairs of keys
+                const float k0 = __shfl_sync(~0u, my_x, 16 * u + r), k1 = __shfl_sync(~0u, my_x, 16 * u + 8 + r);
+                f[u][0] = __shfl_sync(~0u, my_y, 16 * u + r);
+                f[u][1] = __shfl_sync(~0u, my_y, 16 * u + 8 + r);
                 if constexpr (kHalf) {
-                    pa = __floats2half2_rn(__shfl_sync(~0u, e0, 8 * c), __shfl_sync(~0u, e0, 8 * c + 4));
-                    pc = __floats2half2_rn(__shfl_sync(~0u, e1, 8 * c), __shfl_sync(~0u, e1, 8 * c + 4));
+                    f[u][0] = half_weight_factor(f[u][0], e[u][0]);
+                    f[u][1] = half_weight_factor(f[u][1], e[u][1]);
                 }
 #pragma unroll
-                for (int w = 0; w < D / 32; ++w)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {           // bytes 0, 1 and 2, 3 of the word: m-tiles 2 w, 2 w + 1
+                    for (int x = 0; x < 2; ++x) {
+                        sc[u][nt][x] = static_cast<float>(256 * hi[nt][x] + lo[nt][x]) * (qu[nt][x] * k0);
+                        sc[u][nt][2 + x] = static_cast<float>(256 * hi[nt][2 + x] + lo[nt][2 + x]) * (qu[nt][x] * k1);
+                    }
+                mask(sc[u], key0 + 16 * u, old);
+            }
+            uint32_t pb[2][NT][2];
+            softmax(sc, w, f, pb);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t v[4][D / 32];
+#pragma unroll
+                for (int a = 0; a < 4; ++a)
+#pragma unroll
+                    for (int h = 0; h < C::VC; ++h) {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(stg + (2 * u + 1) * C::kBox8 + piece(2 * c + (a & 1) + 8 * (a >> 1), 4 * h + (r >> 1)) + 8 * (r & 1));
+                        v[a][2 * h] = x.x; v[a][2 * h + 1] = x.y;
+                    }
+                __half2 pa, pc;                                      // the powers of two that go with this thread's pairs of keys
+                if constexpr (kHalf) {
+                    pa = __floats2half2_rn(__shfl_sync(~0u, e[u][0], 8 * c), __shfl_sync(~0u, e[u][0], 8 * c + 4));
+                    pc = __floats2half2_rn(__shfl_sync(~0u, e[u][1], 8 * c), __shfl_sync(~0u, e[u][1], 8 * c + 4));
+                }
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {           // bytes 0, 1 and 2, 3 of the word: m-tiles 2 x, 2 x + 1
                         uint32_t a0, a1, a2, a3;
-                        const uint32_t u = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140), x = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
+                        const uint32_t y = __byte_perm(v[0][x], v[1][x], half ? 0x7362 : 0x5140), z = __byte_perm(v[2][x], v[3][x], half ? 0x7362 : 0x5140);
                         if constexpr (kHalf) {
-                            Codes8<T>::expand_scaled(u, pa, a0, a1);
-                            Codes8<T>::expand_scaled(x, pc, a2, a3);
+                            Codes8<T>::expand_scaled(y, pa, a0, a1);
+                            Codes8<T>::expand_scaled(z, pc, a2, a3);
                         } else {
-                            Codes8<T>::expand(u, a0, a1);
-                            Codes8<T>::expand(x, a2, a3);
+                            Codes8<T>::expand(y, a0, a1);
+                            Codes8<T>::expand(z, a2, a3);
                         }
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) M::mma(o[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                        for (int nt = 0; nt < NT; ++nt) M::mma(o[nt][2 * x + half], a0, a1, a2, a3, pb[u][nt][0], pb[u][nt][1]);
                     }
             }
         }
     }
-    cp_wait<0>();
+    if (failed) {
+        p.seqs.raise(VQ_WORD_TIMEOUT);
+#pragma unroll 1
+        for (int x = 0; x < (1 << 14); ++x) __nanosleep(256);        // tile loads still in flight get time to land
+    }
 
     // ---- merge: warps, then the CTAs of the cluster
     float *sum = reinterpret_cast<float *>(fifo);                    // [kCols][D]
@@ -531,6 +617,24 @@ __global__ void __launch_bounds__(kFewWarps * 32) paged_few_kernel(const PagedAt
     cluster.sync();                                                  // nobody leaves while others read its sums
 }
 
+// pool [NP, Hkv, P, D] in boxes of 16 rows x 64 columns of 16 bits, or whole rows of 8 bits
+template <bool Q8>
+static bool map_rows(CUtensorMap *out, const PagedPool &pool, const PagedAttnParams &p, bool f16)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return false;
+    const int P = 1 << p.seqs.log_p, e = Q8 ? 1 : 2;
+    const cuuint64_t dim[4] = {static_cast<cuuint64_t>(p.D), static_cast<cuuint64_t>(P), static_cast<cuuint64_t>(p.Hkv), static_cast<cuuint64_t>(p.seqs.NP)};
+    // a dimension of one element may come with any stride: give the map one it accepts
+    const cuuint64_t str[3] = {static_cast<cuuint64_t>(pool.s_row * e), static_cast<cuuint64_t>((p.Hkv > 1 ? pool.s_head : pool.s_row) * e),
+                               static_cast<cuuint64_t>((p.seqs.NP > 1 ? pool.s_page : pool.s_row) * e)};
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(Q8 ? p.D : 64), 16, 1, 1}, es[4] = {1, 1, 1, 1};
+    return fn(out, Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+              const_cast<void *>(pool.ptr), dim, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              Q8 && p.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, bool Q8, int D, int NT>
 static int launch_few(const PagedAttnParams &p, cudaStream_t stream)
 {
@@ -544,6 +648,15 @@ static int launch_few(const PagedAttnParams &p, cudaStream_t stream)
     int nsplit = 1;
     while (nsplit < 8 && units * nsplit < 2 * sms) nsplit *= 2;
     if (units * nsplit > 0x7fffffff) return VQ_EUNSUPPORTED;
+    constexpr bool f16 = !IsBf16<T>::value;
+    CUtensorMap k1, k3, v, cb, vs;
+    if (!map_rows<Q8>(&k1, p.k1, p, f16) || !map_rows<Q8>(&k3, p.k3, p, f16) || !map_rows<Q8>(&v, p.v, p, f16)) return VQ_ELAUNCH;
+    if (p.cb != nullptr) {
+        const uint64_t MK = p.MK, cd[3] = {D, MK, static_cast<uint64_t>(p.Hkv)}, cs[3] = {1, D, MK * D}, vd[3] = {D, MK, static_cast<uint64_t>(p.NS) * p.Hkv};
+        if (!make_map(&cb, p.cb, 3, cd, cs, 16, f16) || !make_map(&vs, p.vsum, 3, vd, cs, 16, f16)) return VQ_ELAUNCH;
+    } else {
+        cb = vs = k1;               // never read
+    }
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = static_cast<unsigned>(nsplit);
@@ -555,7 +668,7 @@ static int launch_few(const PagedAttnParams &p, cudaStream_t stream)
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, p, groups, nsplit) == cudaSuccess ? launch_status() : (cudaGetLastError(), VQ_ELAUNCH);
+    return cudaLaunchKernelEx(&cfg, kern, k1, k3, v, cb, vs, p, groups, nsplit) == cudaSuccess ? launch_status() : (cudaGetLastError(), VQ_ELAUNCH);
 }
 
 template <typename T, bool Q8, int D>
