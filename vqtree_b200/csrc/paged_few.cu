@@ -5,15 +5,13 @@
 // matrix product only has to keep out of its way: mma.sync with the KEYS on the M axis (16 per instruction) and 8 query rows on N, for
 // which a tile of 128 rows of tcgen05 would be nearly empty.  A warp takes steps of 16 keys (32 of 8-bit rows) and keeps its own online
 // softmax: no barrier in the loop.
-//   - A warp's keys and values arrive by TMA, 16 rows a box, in a FIFO of its own (barriers of its own, no CTA barrier).  Both products may
+//   - A warp's keys and values arrive by TMA, 16 rows a box, in a FIFO of its own, filled by one lane of a fifth warp (no CTA barrier).  Both products may
 //     permute their reduction index: a thread reads 16 contiguous bytes of a swizzled key row, which hold its operands of several k-steps, and q
 //     is read in the same order.  Values enter as V^T (D on M): pairs of keys are interleaved by byte permutes.
 //   - S^T (keys x rows) becomes the B operand of the second product by movmatrix, 8 x 8 at a time.
-//   - 8-bit keys stay bytes: the query rows become 16-bit fixed point numbers (largest element 32639), high and low byte each a factor of an
-//     integer product, which is exact.  An element of q is off by 2^-16 of its row's largest at most - bf16 already rounds elements
-//     near the largest by 2^-9 of it - and the keys need no conversion, which was a third of the kernel's instructions.
-//     8-bit values become 16-bit floats exactly (byte permutes and one subtraction).  A key's scale multiplies its score, a value's
-//     scale its weight.
+//   - 8-bit codes become halves exactly (byte permutes and a subtraction).  A key's scale multiplies its score.  A bf16 query row is brought into
+//     the range of a half by a power of two (its largest element to 2^10 .. 2^11; elements above 2^-24 of it stay exact).  Weights carry the
+//     scale of their value.
 //   - Counts multiply the weights of codes in the denominator; codes without members are excluded.
 // One unit = (sequence, block of positions, kv head); its steps are dealt out to the warps of a cluster of 1 - 8 CTAs, which merge their
 // partial sums through distributed shared memory: no workspace, no second launch, the same order of additions every time.
@@ -30,7 +28,9 @@ namespace vq {
 namespace cg = cooperative_groups;
 
 constexpr int kFewWarps = 4;
+constexpr int kFewThreads = (kFewWarps + 1) * 32;   // and the warp that issues the loads
 constexpr int kFewStages = 3;
+constexpr int kFewSplit = 16;           // CTAs of a cluster at most (more than 8 are opt-in on this architecture)
 constexpr float kFewLazy = 8.f;         // log2 units a score may exceed its row's reference before the sums are rescaled
 
 template <typename T> struct Mma16816;
@@ -54,11 +54,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x)
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
-{
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 template <typename T, bool Q8, int D, int NT>
 struct FewCfg {
     static constexpr int kCols = 8 * NT;                         // query rows, padded
@@ -68,8 +63,7 @@ struct FewCfg {
     static constexpr int kStage = 2 * VC * kBox;                 // 16 keys with their values, or 32 of 8 bits
     static_assert(4 * kBox8 == kStage, "a stage holds twice as many 8-bit rows");
     static constexpr int kWarpBytes = kFewStages * kStage;
-    static constexpr int kQ8 = kCols * D;                        // one byte plane of the rows
-    static constexpr int kQ = Q8 ? kCols * D * 2 + 4 * kQ8 : 2 * kCols * D * 2;   // 16-bit rows q1, q2; or q2, and both kinds in two planes
+    static constexpr int kQ = (Q8 ? 3 : 2) * kCols * D * 2;      // rows q1, q2; 8-bit rows: q2, and both as halves
     static constexpr int kPages = 256;                           // page table entries kept in shared memory; the rest is read where it is needed
     static constexpr int kTotal = kFewWarps * kWarpBytes + kQ + kPages * 4 + 1024;   // + slack for 1024-byte alignment
     static_assert(kCols * D * 4 <= kFewStages * kStage, "a warp's sums fit into its FIFO");
@@ -82,23 +76,23 @@ struct FewSteps {
 };
 
 template <typename T, bool Q8, int D, int NT>
-__global__ void __launch_bounds__(kFewWarps * 32, 2) paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constant__ CUtensorMap tm_k3, const __grid_constant__ CUtensorMap tm_v,
+__global__ void __launch_bounds__(kFewThreads, NT == 4 ? 1 : 2)
+paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constant__ CUtensorMap tm_k3, const __grid_constant__ CUtensorMap tm_v,
                  const __grid_constant__ CUtensorMap tm_cb, const __grid_constant__ CUtensorMap tm_vs, const PagedAttnParams p, int groups, int nsplit)
 {
     using C = FewCfg<T, Q8, D, NT>;
     using M = Mma16816<T>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ __align__(8) uint64_t s_bar[kFewWarps][kFewStages];
+    __shared__ __align__(8) uint64_t s_bar[kFewWarps][kFewStages], s_free[kFewWarps][kFewStages];
     __shared__ int s_bad;                                            // some page of the unit is missing, or not kept in shared memory
     __shared__ float s_m[kFewWarps][C::kCols], s_l[kFewWarps][C::kCols];
     __shared__ float s_cm[C::kCols], s_cl[C::kCols];
-    __shared__ float s_unit[2][Q8 ? C::kCols : 1];                   // what the fixed point rows count in
+    __shared__ float s_unit[2][Q8 ? C::kCols : 1];                   // 8-bit rows: the power of two a query row was divided by
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int r = lane >> 2, c = lane & 3;
-    uint8_t *fifo = smem + warp * C::kWarpBytes;
     T *s_q = reinterpret_cast<T *>(smem + kFewWarps * C::kWarpBytes);        // [2][kCols][D]
-    uint8_t *s_q8 = smem + kFewWarps * C::kWarpBytes + C::kCols * D * 2;     // 8-bit rows: [q1, q2][high, low byte][kCols][D]
+    __half *s_qh = reinterpret_cast<__half *>(s_q + C::kCols * D);           // 8-bit rows: [q1, q2][kCols][D]
     int *s_page = reinterpret_cast<int *>(smem + kFewWarps * C::kWarpBytes + C::kQ);
 
     const int split = blockIdx.x % nsplit;
@@ -107,6 +101,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) paged_few_kernel(const __gr
     unit /= p.Hkv;
     const int grp = unit % groups, s = unit / groups;
     int t0, q, n;
+    grid_dependency_launch();
+    grid_dependency_wait();
     if (!p.seqs.seq(s, t0, q, n, p.max_q) || q == 0) return;         // the whole cluster leaves
     int i0 = n - q, i1 = n - 1;                                      // positions of the group's tokens: those of one 128-block
     if (grp == 0) i1 = min(i1, i0 / kBlock * kBlock + kBlock - 1);
@@ -132,12 +128,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) paged_few_kernel(const __gr
 
     if (tid == 0) {
         for (int w = 0; w < kFewWarps; ++w)
-            for (int x = 0; x < kFewStages; ++x) ptx::mbar_init(&s_bar[w][x], 1);
+            for (int x = 0; x < kFewStages; ++x) {
+                ptx::mbar_init(&s_bar[w][x], 1);
+                ptx::mbar_init(&s_free[w][x], 1);
+            }
         ptx::fence_mbar_init();
         s_bad = cols > C::kPages;
     }
     __syncthreads();
-    for (int x = tid; x < min(cols, C::kPages); x += kFewWarps * 32) {
+    for (int x = tid; x < min(cols, C::kPages); x += kFewThreads) {
         s_page[x] = p.seqs.page(s, col0 + x);
         if (s_page[x] < 0) s_bad = 1;
     }
@@ -146,45 +145,33 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) paged_few_kernel(const __gr
         const int64_t t = t0 + row / p.G, h = hk * p.G + row % p.G;
         return which ? static_cast<const T *>(p.q2) + t * p.q2_t + h * p.q2_h : static_cast<const T *>(p.q1) + t * p.q1_t + h * p.q1_h;
     };
-    for (int x = tid; x < (Q8 ? 1 : 2) * C::kCols * D / 8; x += kFewWarps * 32) {
+    for (int x = tid; x < (Q8 ? 1 : 2) * C::kCols * D / 8; x += kFewThreads) {
         const int which = Q8 ? 1 : x / (C::kCols * D / 8), row = x / (D / 8) % C::kCols, d = x % (D / 8) * 8;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (row < rows) v = *reinterpret_cast<const uint4 *>(q_row(which, row) + d);
         reinterpret_cast<uint4 *>(s_q)[x] = v;
     }
-    if constexpr (Q8) {                                              // fixed point: v = 256 hi + lo
-        for (int x = warp; x < 2 * C::kCols; x += kFewWarps) {
+    if constexpr (Q8) {
+        for (int x = warp; x < 2 * C::kCols; x += kFewWarps + 1) {
             const int which = x / C::kCols, row = x % C::kCols;
-            float e[D / 32], top = 0.f, unit = 0.f;
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) e[i] = row < rows ? to_f32(q_row(which, row)[lane * (D / 32) + i]) : 0.f;
-            bool finite = true;
+            float e[D / 32], top = 0.f;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
+                e[i] = row < rows ? to_f32(q_row(which, row)[lane * (D / 32) + i]) : 0.f;
                 top = fmaxf(top, fabsf(e[i]));
-                finite = finite && fabsf(e[i]) < INFINITY;
             }
+            int shift = 0;
+            if constexpr (IsBf16<T>::value) {
 #pragma unroll
-            for (int y = 16; y; y >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, y));
-            unit = top * (1.f / 32639.f);
-            const float inv = unit >= 1.17549435e-38f ? __frcp_rn(unit) : 0.f;
-            uint32_t hi = 0, lo = 0;
+                for (int y = 16; y; y >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, y));
+                const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+                if (top > 0.f && ex < 128) shift = max(-100, ex) - 10;
+            }
+            const float mul = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                const int v = min(32639, max(-32639, __float2int_rn(e[i] * inv))), h = (v + 128) >> 8;
-                hi |= (static_cast<uint32_t>(h) & 255u) << (8 * i);
-                lo |= (static_cast<uint32_t>(v - 256 * h) & 255u) << (8 * i);
-            }
-            uint8_t *dst = s_q8 + 2 * which * C::kQ8 + row * D + lane * (D / 32);
-            if constexpr (D == 128) {
-                *reinterpret_cast<uint32_t *>(dst) = hi;
-                *reinterpret_cast<uint32_t *>(dst + C::kQ8) = lo;
-            } else {
-                *reinterpret_cast<uint16_t *>(dst) = static_cast<uint16_t>(hi);
-                *reinterpret_cast<uint16_t *>(dst + C::kQ8) = static_cast<uint16_t>(lo);
-            }
-            if (lane == 0) s_unit[which][row] = __all_sync(~0u, finite) ? unit : __int_as_float(0x7fffffff);
-            else __all_sync(~0u, finite);
+            for (int i = 0; i < D / 32; i += 2)
+                *reinterpret_cast<__half2 *>(s_qh + (which * C::kCols + row) * D + lane * (D / 32) + i) = __floats2half2_rn(e[i] * mul, e[i + 1] * mul);
+            if (lane == 0) s_unit[which][row] = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
         }
     }
     __syncthreads();
@@ -199,10 +186,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) paged_few_kernel(const __gr
     auto first_key = [&](int step) {
         return step < st.n_far + st.n_old ? st.old0 + (step - st.n_far) * KEYS : st.near0 + (step - st.n_far - st.n_old) * KEYS;
     };
-    // ---- keys and values of a step into stage `slot`, by one thread.  Missing pages (reported) bring nothing.
-    auto fill = [&](int step, int slot) {
-        uint8_t *dst = fifo + slot * C::kStage;
-        uint64_t *bar = &s_bar[warp][slot];
+    // ---- keys and values of a step into stage `slot` of warp w, by one thread.  Missing pages (reported) bring nothing.
+    auto fill = [&](int w, int step, int slot) {
+        uint8_t *dst = smem + w * C::kWarpBytes + slot * C::kStage;
+        uint64_t *bar = &s_bar[w][slot];
         if (step < st.n_far) {
             ptx::mbar_expect_tx(bar, C::kStage);
 #pragma unroll
@@ -253,318 +240,343 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) paged_few_kernel(const __gr
         }
     };
 
-    float o[NT][C::MT][4], m[NT][2], lim[NT][2], l[NT][2], qu[NT][2];   // lim: the score that raises the reference m
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[nt][mt][x] = 0.f;
-        m[nt][0] = m[nt][1] = lim[nt][0] = lim[nt][1] = -INFINITY;
-        qu[nt][0] = qu[nt][1] = 0.f;
-        l[nt][0] = l[nt][1] = 0.f;
-    }
-    uint32_t qf[NT][D / 8];
-
-    const int stride = nsplit * kFewWarps, first = split * kFewWarps + warp;
-#pragma unroll
-    for (int x = 0; x < kFewStages - 1; ++x)
-        if (first + x * stride < total && ptx::elect_one()) fill(first + x * stride, x);
-    float next_x, next_y;
-    extras(first, next_x, next_y);
-    // sc: scores of keys r and r + 8 of each group of 16 (c0 c1 | c2 c3) in log2 units, -inf where excluded -> weights; w: denominator weights of
-    // the two keys, f: factors of their value rows.  Raises the references, adds to l, returns the packed weights as B operands.
-    auto softmax = [&](auto &sc, const auto &w, const auto &f, auto &pb) {
-        constexpr int SUBS = sizeof(sc) / sizeof(sc[0]);
-        bool above = false;
-        float mx[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                mx[nt][x] = fmaxf(sc[0][nt][x], sc[0][nt][2 + x]);
-#pragma unroll
-                for (int u = 1; u < SUBS; ++u) mx[nt][x] = ptx::fmax3(mx[nt][x], sc[u][nt][x], sc[u][nt][2 + x]);
-                above |= mx[nt][x] > lim[nt][x];
+    const int stride = nsplit * kFewWarps;
+    bool failed = false;
+    if (warp == kFewWarps) {
+        // lane w keeps warp w's FIFO full
+        if (lane < kFewWarps) {
+            int slot = 0;
+            uint32_t par = 1u;
+            for (int step = split * kFewWarps + lane, x = 0; step < total; step += stride, ++x) {
+                if (x >= kFewStages && !ptx::mbar_wait(&s_free[lane][slot], par, p.wait_limit)) {
+                    failed = true;
+                    break;
+                }
+                fill(lane, step, slot);
+                if (++slot == kFewStages) {
+                    slot = 0;
+                    par ^= 1u;
+                }
             }
-        if (__any_sync(~0u, above)) {
+        }
+    } else {
+        float o[NT][C::MT][4], m[NT][2], lim[NT][2], l[NT][2], qu[NT][2];   // lim: the score that raises the reference m
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int mt = 0; mt < C::MT; ++mt)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[nt][mt][x] = 0.f;
+            m[nt][0] = m[nt][1] = lim[nt][0] = lim[nt][1] = -INFINITY;
+            qu[nt][0] = qu[nt][1] = 0.f;
+            l[nt][0] = l[nt][1] = 0.f;
+        }
+        uint32_t qf[NT][D / 8];
+        uint8_t *const fifo = smem + warp * C::kWarpBytes;
+        const int first = split * kFewWarps + warp;
+        float next_x, next_y;
+        extras(first, next_x, next_y);
+        // sc: scores of keys r and r + 8 of each group of 16 (c0 c1 | c2 c3) in log2 units, -inf where excluded -> weights; w: denominator weights of
+        // the two keys, f: factors of their value rows.  Raises the references, adds to l, returns the packed weights as B operands.
+        auto softmax = [&](auto &sc, const auto &w, const auto &f, auto &pb, bool half) {
+            constexpr int SUBS = sizeof(sc) / sizeof(sc[0]);
+            bool above = false;
+            float mx[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    float v = mx[nt][x];
+                    mx[nt][x] = fmaxf(sc[0][nt][x], sc[0][nt][2 + x]);
 #pragma unroll
-                    for (int y = 4; y < 32; y <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, y));
-                    if (v > m[nt][x]) {
-                        const float a = m[nt][x] == -INFINITY ? 0.f : ptx::ex2(m[nt][x] - v);
-                        m[nt][x] = v;
-                        lim[nt][x] = v + kFewLazy;
-                        l[nt][x] *= a;
-#pragma unroll
-                        for (int mt = 0; mt < C::MT; ++mt) {
-                            o[nt][mt][x] *= a;
-                            o[nt][mt][2 + x] *= a;
-                        }
-                    }
+                    for (int u = 1; u < SUBS; ++u) mx[nt][x] = ptx::fmax3(mx[nt][x], sc[u][nt][x], sc[u][nt][2 + x]);
+                    above |= mx[nt][x] > lim[nt][x];
                 }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const float ma = m[nt][0] == -INFINITY ? 0.f : m[nt][0], mb = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-#pragma unroll
-            for (int u = 0; u < SUBS; ++u) {
-                const float p0 = ptx::ex2(sc[u][nt][0] - ma), p1 = ptx::ex2(sc[u][nt][1] - mb), p2 = ptx::ex2(sc[u][nt][2] - ma), p3 = ptx::ex2(sc[u][nt][3] - mb);
-                l[nt][0] += p0 * w[u][0] + p2 * w[u][1];
-                l[nt][1] += p1 * w[u][0] + p3 * w[u][1];
-                pb[u][nt][0] = movmatrix(Pair16<T>::pack(p0 * f[u][0], p1 * f[u][0]));
-                pb[u][nt][1] = movmatrix(Pair16<T>::pack(p2 * f[u][1], p3 * f[u][1]));
-            }
-        }
-    };
-    // excluded keys of the 16 from j0 on; true: there is no such page
-    auto mask = [&](float (&sc)[NT][4], int j0, bool old) {
-        if (bad && j0 <= i1 && page_of(j0) < 0) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) sc[nt][x] = -INFINITY;
-            return true;
-        }
-        // what every row of the group sees: raw keys below i0 - W, rotated ones in [i1 - W, i0]
-        const bool all = old ? j0 + 15 < i0 - p.W : j0 + 15 <= i0 && (!p.rerope || j0 >= i1 - p.W);
-        if (all) return false;
-        const int ja = j0 + r, jb = ja + 8;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int i = i0 + (8 * nt + 2 * c + x) / p.G, hi = old ? i - p.W - 1 : i, lo = old || !p.rerope ? bd : i - p.W;
-                if (ja < lo || ja > hi || ja >= n) sc[nt][x] = -INFINITY;
-                if (jb < lo || jb > hi || jb >= n) sc[nt][2 + x] = -INFINITY;
-            }
-        return false;
-    };
-
-    int phase = -1, slot = 0;
-    uint32_t par = 0;
-    bool failed = false;
-    for (int step = first; step < total; step += stride) {
-        __syncwarp();                                                // the stage of the step before has been consumed by every lane
-        {
-            const int next = step + (kFewStages - 1) * stride, ns = slot == 0 ? kFewStages - 1 : slot - 1;
-            if (next < total && ptx::elect_one()) fill(next, ns);
-        }
-        const bool far = step < st.n_far, old = !far && step < st.n_far + st.n_old;
-        const int ph = far ? 0 : old ? 1 : 2;
-        if (ph != phase) {                                           // q in the order of this phase's key rows
-            phase = ph;
-            if (Q8 && !far) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const uint8_t *row = s_q8 + (old ? 2 * C::kQ8 : 0) + (8 * nt + r) * D + 16 * C::VC * c;
-#pragma unroll
-                    for (int j = 0; j < C::VC; ++j) {
-                        const uint4 h = *reinterpret_cast<const uint4 *>(row + 16 * j), e = *reinterpret_cast<const uint4 *>(row + C::kQ8 + 16 * j);
-                        qf[nt][8 * j] = h.x; qf[nt][8 * j + 1] = h.y; qf[nt][8 * j + 2] = h.z; qf[nt][8 * j + 3] = h.w;
-                        qf[nt][8 * j + 4] = e.x; qf[nt][8 * j + 5] = e.y; qf[nt][8 * j + 6] = e.z; qf[nt][8 * j + 7] = e.w;
-                    }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) qu[nt][x] = s_unit[old][8 * nt + 2 * c + x] * p.scale_log2;
-                }
-            } else {
-                const T *src = s_q + (!Q8 && (far || old) ? C::kCols * D : 0);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int j = 0; j < 2 * C::VC; ++j) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(src + (8 * nt + r) * D + 64 * (j / 2) + 16 * c + 8 * (j % 2));
-                        qf[nt][4 * j] = v.x; qf[nt][4 * j + 1] = v.y; qf[nt][4 * j + 2] = v.z; qf[nt][4 * j + 3] = v.w;
-                    }
-            }
-        }
-        const float my_x = next_x, my_y = next_y;
-        extras(step + stride, next_x, next_y);
-        const uint8_t *stg = fifo + slot * C::kStage;
-        if (!__all_sync(~0u, ptx::mbar_wait(&s_bar[warp][slot], par, p.wait_limit))) {
-            failed = true;
-            break;
-        }
-        if (++slot == kFewStages) {
-            slot = 0;
-            par ^= 1u;
-        }
-        const int key0 = first_key(step);
-        if (far || !Q8) {
-            // ---- S^T = K Q^T, even and odd k-steps by themselves.  Piece j of row k lies at j ^ (k % 8); four lanes share a row, each
-            // takes two neighbouring pieces of its 128 bytes: the eight lanes that read together ask for different banks.
-            float sc[1][NT][4], s2[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) sc[0][nt][x] = s2[nt][x] = 0.f;
-#pragma unroll
-            for (int h = 0; h < C::VC; ++h)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const uint8_t *at = stg + h * C::kBox + r * 128 + (((2 * c + y) ^ r) << 4);
-                    const uint4 a = *reinterpret_cast<const uint4 *>(at), b = *reinterpret_cast<const uint4 *>(at + 8 * 128);
-                    const int j = 2 * h + y;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        M::mma(sc[0][nt], a.x, b.x, a.y, b.y, qf[nt][4 * j], qf[nt][4 * j + 1]);
-                        M::mma(s2[nt], a.z, b.z, a.w, b.w, qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
-                    }
-                }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) sc[0][nt][x] = (sc[0][nt][x] + s2[nt][x]) * p.scale_log2;
-            float w[1][2] = {{1.f, 1.f}};
-            const float f[1][2] = {{1.f, 1.f}};
-            bool hole = false;
-            if (far) {
-                w[0][0] = __shfl_sync(~0u, my_x, r);
-                w[0][1] = __shfl_sync(~0u, my_x, r + 8);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (!(w[0][0] > 0.f)) sc[0][nt][0] = sc[0][nt][1] = -INFINITY;
-                    if (!(w[0][1] > 0.f)) sc[0][nt][2] = sc[0][nt][3] = -INFINITY;
-                }
-            } else {
-                hole = mask(sc[0], key0, old);
-            }
-            uint32_t pb[1][NT][2];
-            softmax(sc, w, f, pb);
-            // ---- O^T += V^T P^T
-#pragma unroll
-            for (int h = 0; h < C::VC; ++h) {
-                uint4 v4[4];
-#pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const int k = 2 * c + (a & 1) + 8 * (a >> 1);
-                    v4[a] = *reinterpret_cast<const uint4 *>(stg + (C::VC + h) * C::kBox + k * 128 + ((r ^ (k & 7)) << 4));
-                }
-                if (!far && (hole || key0 + 16 > n)) {               // behind the sequence's end a page may hold anything: zeros instead
-#pragma unroll
-                    for (int a = 0; a < 4; ++a)
-                        if (hole || key0 + 2 * c + (a & 1) + 8 * (a >> 1) >= n) v4[a] = make_uint4(0, 0, 0, 0);
-                }
-                const uint32_t v0[4] = {v4[0].x, v4[0].y, v4[0].z, v4[0].w}, v1[4] = {v4[1].x, v4[1].y, v4[1].z, v4[1].w};
-                const uint32_t v2[4] = {v4[2].x, v4[2].y, v4[2].z, v4[2].w}, v3[4] = {v4[3].x, v4[3].y, v4[3].z, v4[3].w};
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const uint32_t a0 = __byte_perm(v0[x], v1[x], 0x5410), a1 = __byte_perm(v0[x], v1[x], 0x7632);
-                    const uint32_t a2 = __byte_perm(v2[x], v3[x], 0x5410), a3 = __byte_perm(v2[x], v3[x], 0x7632);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) M::mma(o[nt][4 * h + x], a0, a1, a2, a3, pb[0][nt][0], pb[0][nt][1]);
-                }
-            }
-        } else {
-            // 8-bit rows of 128 (64) bytes: piece j of row k lies at j ^ (k % 8)  (j ^ (k / 2 % 4))
-            auto piece = [&](int k, int j) { return D == 128 ? k * 128 + ((j ^ (k & 7)) << 4) : k * 64 + ((j ^ ((k >> 1) & 3)) << 4); };
-            float sc[2][NT][4], f[2][2], e[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
-            const float w[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                int hi[NT][4], lo[NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) hi[nt][x] = lo[nt][x] = 0;
-#pragma unroll
-                for (int j = 0; j < C::VC; ++j) {
-                    const uint8_t *at = stg + 2 * u * C::kBox8;
-                    const uint4 a = *reinterpret_cast<const uint4 *>(at + piece(r, C::VC * c + j)), b = *reinterpret_cast<const uint4 *>(at + piece(r + 8, C::VC * c + j));
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma_s8(hi[nt], a.x, b.x, a.y, b.y, qf[nt][8 * j], qf[nt][8 * j + 1]);
-                        mma_s8(lo[nt], a.x, b.x, a.y, b.y, qf[nt][8 * j + 4], qf[nt][8 * j + 5]);
-                        mma_s8(hi[nt], a.z, b.z, a.w, b.w, qf[nt][8 * j + 2], qf[nt][8 * j + 3]);
-                        mma_s8(lo[nt], a.z, b.z, a.w, b.w, qf[nt][8 * j + 6], qf[nt][8 * j + 7]);
-                    }
-                }
-                const float k0 = __shfl_sync(~0u, my_x, 16 * u + r), k1 = __shfl_sync(~0u, my_x, 16 * u + 8 + r);
-                f[u][0] = __shfl_sync(~0u, my_y, 16 * u + r);
-                f[u][1] = __shfl_sync(~0u, my_y, 16 * u + 8 + r);
-                if constexpr (kHalf) {
-                    f[u][0] = half_weight_factor(f[u][0], e[u][0]);
-                    f[u][1] = half_weight_factor(f[u][1], e[u][1]);
-                }
+            if (__any_sync(~0u, above)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        sc[u][nt][x] = static_cast<float>(256 * hi[nt][x] + lo[nt][x]) * (qu[nt][x] * k0);
-                        sc[u][nt][2 + x] = static_cast<float>(256 * hi[nt][2 + x] + lo[nt][2 + x]) * (qu[nt][x] * k1);
+                        float v = mx[nt][x];
+#pragma unroll
+                        for (int y = 4; y < 32; y <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, y));
+                        if (v > m[nt][x]) {
+                            const float a = m[nt][x] == -INFINITY ? 0.f : ptx::ex2(m[nt][x] - v);
+                            m[nt][x] = v;
+                            lim[nt][x] = v + kFewLazy;
+                            l[nt][x] *= a;
+#pragma unroll
+                            for (int mt = 0; mt < C::MT; ++mt) {
+                                o[nt][mt][x] *= a;
+                                o[nt][mt][2 + x] *= a;
+                            }
+                        }
                     }
-                mask(sc[u], key0 + 16 * u, old);
             }
-            uint32_t pb[2][NT][2];
-            softmax(sc, w, f, pb);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                uint32_t v[4][D / 32];
+            for (int nt = 0; nt < NT; ++nt) {
+                const float ma = m[nt][0] == -INFINITY ? 0.f : m[nt][0], mb = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
 #pragma unroll
-                for (int a = 0; a < 4; ++a)
-#pragma unroll
-                    for (int h = 0; h < C::VC; ++h) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(stg + (2 * u + 1) * C::kBox8 + piece(2 * c + (a & 1) + 8 * (a >> 1), 4 * h + (r >> 1)) + 8 * (r & 1));
-                        v[a][2 * h] = x.x; v[a][2 * h + 1] = x.y;
-                    }
-                __half2 pa, pc;                                      // the powers of two that go with this thread's pairs of keys
-                if constexpr (kHalf) {
-                    pa = __floats2half2_rn(__shfl_sync(~0u, e[u][0], 8 * c), __shfl_sync(~0u, e[u][0], 8 * c + 4));
-                    pc = __floats2half2_rn(__shfl_sync(~0u, e[u][1], 8 * c), __shfl_sync(~0u, e[u][1], 8 * c + 4));
+                for (int u = 0; u < SUBS; ++u) {
+                    const float p0 = ptx::ex2(sc[u][nt][0] - ma), p1 = ptx::ex2(sc[u][nt][1] - mb), p2 = ptx::ex2(sc[u][nt][2] - ma), p3 = ptx::ex2(sc[u][nt][3] - mb);
+                    l[nt][0] += p0 * w[u][0] + p2 * w[u][1];
+                    l[nt][1] += p1 * w[u][0] + p3 * w[u][1];
+                    const float a0 = p0 * f[u][0], a1 = p1 * f[u][0], a2 = p2 * f[u][1], a3 = p3 * f[u][1];
+                    pb[u][nt][0] = movmatrix(half ? ptx::pack_f16(a0, a1) : Pair16<T>::pack(a0, a1));
+                    pb[u][nt][1] = movmatrix(half ? ptx::pack_f16(a2, a3) : Pair16<T>::pack(a2, a3));
                 }
+            }
+        };
+        // excluded keys of the 16 from j0 on; true: there is no such page
+        auto mask = [&](float (&sc)[NT][4], int j0, bool old) {
+            if (bad && j0 <= i1 && page_of(j0) < 0) {
 #pragma unroll
-                for (int x = 0; x < D / 32; ++x)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {           // bytes 0, 1 and 2, 3 of the word: m-tiles 2 x, 2 x + 1
-                        uint32_t a0, a1, a2, a3;
-                        const uint32_t y = __byte_perm(v[0][x], v[1][x], half ? 0x7362 : 0x5140), z = __byte_perm(v[2][x], v[3][x], half ? 0x7362 : 0x5140);
-                        if constexpr (kHalf) {
-                            Codes8<T>::expand_scaled(y, pa, a0, a1);
-                            Codes8<T>::expand_scaled(z, pc, a2, a3);
-                        } else {
-                            Codes8<T>::expand(y, a0, a1);
-                            Codes8<T>::expand(z, a2, a3);
+                    for (int x = 0; x < 4; ++x) sc[nt][x] = -INFINITY;
+                return true;
+            }
+            // what every row of the group sees: raw keys below i0 - W, rotated ones in [i1 - W, i0]
+            const bool all = old ? j0 + 15 < i0 - p.W : j0 + 15 <= i0 && (!p.rerope || j0 >= i1 - p.W);
+            if (all) return false;
+            const int ja = j0 + r, jb = ja + 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int i = i0 + (8 * nt + 2 * c + x) / p.G, hi = old ? i - p.W - 1 : i, lo = old || !p.rerope ? bd : i - p.W;
+                    if (ja < lo || ja > hi || ja >= n) sc[nt][x] = -INFINITY;
+                    if (jb < lo || jb > hi || jb >= n) sc[nt][2 + x] = -INFINITY;
+                }
+            return false;
+        };
+
+        int phase = -1, slot = 0;
+        uint32_t par = 0;
+        for (int step = first; step < total; step += stride) {
+            const bool far = step < st.n_far, old = !far && step < st.n_far + st.n_old;
+            const int ph = far ? 0 : old ? 1 : 2;
+            if (ph != phase) {                                           // q in the order of this phase's key rows
+                phase = ph;
+                if (Q8 && !far) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const __half *row = s_qh + ((old ? C::kCols : 0) + 8 * nt + r) * D + 16 * C::VC * c;
+#pragma unroll
+                        for (int j = 0; j < 2 * C::VC; ++j) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(row + 8 * j);
+                            qf[nt][4 * j] = v.x; qf[nt][4 * j + 1] = v.y; qf[nt][4 * j + 2] = v.z; qf[nt][4 * j + 3] = v.w;
                         }
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) M::mma(o[nt][2 * x + half], a0, a1, a2, a3, pb[u][nt][0], pb[u][nt][1]);
+                        for (int x = 0; x < 2; ++x) qu[nt][x] = s_unit[old][8 * nt + 2 * c + x] * p.scale_log2;
                     }
+                } else {
+                    const T *src = s_q + (!Q8 && (far || old) ? C::kCols * D : 0);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < 2 * C::VC; ++j) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(src + (8 * nt + r) * D + 64 * (j / 2) + 16 * c + 8 * (j % 2));
+                            qf[nt][4 * j] = v.x; qf[nt][4 * j + 1] = v.y; qf[nt][4 * j + 2] = v.z; qf[nt][4 * j + 3] = v.w;
+                        }
+                }
+            }
+            const float my_x = next_x, my_y = next_y;
+            extras(step + stride, next_x, next_y);
+            const uint8_t *stg = fifo + slot * C::kStage;
+            if (!__all_sync(~0u, ptx::mbar_wait(&s_bar[warp][slot], par, p.wait_limit))) {
+                failed = true;
+                break;
+            }
+            const int key0 = first_key(step);
+            if (far || !Q8) {
+                // ---- S^T = K Q^T, even and odd k-steps by themselves.  Piece j of row k lies at j ^ (k % 8); four lanes share a row, each
+                // takes two neighbouring pieces of its 128 bytes: the eight lanes that read together ask for different banks.
+                float sc[1][NT][4], s2[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) sc[0][nt][x] = s2[nt][x] = 0.f;
+#pragma unroll
+                for (int h = 0; h < C::VC; ++h)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const uint8_t *at = stg + h * C::kBox + r * 128 + (((2 * c + y) ^ r) << 4);
+                        const uint4 a = *reinterpret_cast<const uint4 *>(at), b = *reinterpret_cast<const uint4 *>(at + 8 * 128);
+                        const int j = 2 * h + y;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            M::mma(sc[0][nt], a.x, b.x, a.y, b.y, qf[nt][4 * j], qf[nt][4 * j + 1]);
+                            M::mma(s2[nt], a.z, b.z, a.w, b.w, qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
+                        }
+                    }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) sc[0][nt][x] = (sc[0][nt][x] + s2[nt][x]) * p.scale_log2;
+                float w[1][2] = {{1.f, 1.f}};
+                const float f[1][2] = {{1.f, 1.f}};
+                bool hole = false;
+                if (far) {
+                    w[0][0] = __shfl_sync(~0u, my_x, r);
+                    w[0][1] = __shfl_sync(~0u, my_x, r + 8);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (!(w[0][0] > 0.f)) sc[0][nt][0] = sc[0][nt][1] = -INFINITY;
+                        if (!(w[0][1] > 0.f)) sc[0][nt][2] = sc[0][nt][3] = -INFINITY;
+                    }
+                } else {
+                    hole = mask(sc[0], key0, old);
+                }
+                uint32_t pb[1][NT][2];
+                softmax(sc, w, f, pb, false);
+                // ---- O^T += V^T P^T
+#pragma unroll
+                for (int h = 0; h < C::VC; ++h) {
+                    uint4 v4[4];
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        const int k = 2 * c + (a & 1) + 8 * (a >> 1);
+                        v4[a] = *reinterpret_cast<const uint4 *>(stg + (C::VC + h) * C::kBox + k * 128 + ((r ^ (k & 7)) << 4));
+                    }
+                    if (!far && (hole || key0 + 16 > n)) {               // behind the sequence's end a page may hold anything: zeros instead
+#pragma unroll
+                        for (int a = 0; a < 4; ++a)
+                            if (hole || key0 + 2 * c + (a & 1) + 8 * (a >> 1) >= n) v4[a] = make_uint4(0, 0, 0, 0);
+                    }
+                    const uint32_t v0[4] = {v4[0].x, v4[0].y, v4[0].z, v4[0].w}, v1[4] = {v4[1].x, v4[1].y, v4[1].z, v4[1].w};
+                    const uint32_t v2[4] = {v4[2].x, v4[2].y, v4[2].z, v4[2].w}, v3[4] = {v4[3].x, v4[3].y, v4[3].z, v4[3].w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const uint32_t a0 = __byte_perm(v0[x], v1[x], 0x5410), a1 = __byte_perm(v0[x], v1[x], 0x7632);
+                        const uint32_t a2 = __byte_perm(v2[x], v3[x], 0x5410), a3 = __byte_perm(v2[x], v3[x], 0x7632);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) M::mma(o[nt][4 * h + x], a0, a1, a2, a3, pb[0][nt][0], pb[0][nt][1]);
+                    }
+                }
+            } else {
+                // 8-bit rows of 128 (64) bytes: piece j of row k lies at j ^ (k % 8)  (j ^ (k / 2 % 4))
+                auto piece = [&](int k, int j) { return D == 128 ? k * 128 + ((j ^ (k & 7)) << 4) : k * 64 + ((j ^ ((k >> 1) & 3)) << 4); };
+                float sc[2][NT][4], f[2][2], e[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
+                const float w[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
+                // Weights and values as halves: codes become halves in five instructions per four, bf16 in eight.  bf16 caches whose scales
+                // leave the range of a half take the latter.
+                const bool hv = kHalf || __all_sync(~0u, (my_y >= 5.9604645e-8f && my_y < 32.f) || my_y == 0.f);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) sc[u][nt][x] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < C::VC; ++j) {
+                        const uint8_t *at = stg + 2 * u * C::kBox8;
+                        const uint4 a4 = *reinterpret_cast<const uint4 *>(at + piece(r, C::VC * c + j));
+                        const uint4 b4 = *reinterpret_cast<const uint4 *>(at + piece(r + 8, C::VC * c + j));
+                        const uint32_t a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            uint32_t al, ah, bl, bh;
+                            Codes8<__half>::expand(a[x], al, ah);
+                            Codes8<__half>::expand(b[x], bl, bh);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) Mma16816<__half>::mma(sc[u][nt], al, bl, ah, bh, qf[nt][8 * j + 2 * x], qf[nt][8 * j + 2 * x + 1]);
+                        }
+                    }
+                    const float k0 = __shfl_sync(~0u, my_x, 16 * u + r), k1 = __shfl_sync(~0u, my_x, 16 * u + 8 + r);
+                    f[u][0] = __shfl_sync(~0u, my_y, 16 * u + r);
+                    f[u][1] = __shfl_sync(~0u, my_y, 16 * u + 8 + r);
+                    if (hv) {
+                        f[u][0] = half_weight_factor(f[u][0], e[u][0]);
+                        f[u][1] = half_weight_factor(f[u][1], e[u][1]);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            sc[u][nt][x] *= qu[nt][x] * k0;
+                            sc[u][nt][2 + x] *= qu[nt][x] * k1;
+                        }
+                    mask(sc[u], key0 + 16 * u, old);
+                }
+                uint32_t pb[2][NT][2];
+                softmax(sc, w, f, pb, hv);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t v[4][D / 32];
+#pragma unroll
+                    for (int a = 0; a < 4; ++a)
+#pragma unroll
+                        for (int h = 0; h < C::VC; ++h) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(stg + (2 * u + 1) * C::kBox8 + piece(2 * c + (a & 1) + 8 * (a >> 1), 4 * h + (r >> 1)) + 8 * (r & 1));
+                            v[a][2 * h] = x.x; v[a][2 * h + 1] = x.y;
+                        }
+                    // bytes 0, 1 (y = 0) and 2, 3 of word x: m-tiles 2 x, 2 x + 1
+                    auto pairs = [&](int x, int y, int a) { return __byte_perm(v[a][x], v[a + 1][x], y ? 0x7362 : 0x5140); };
+                    if (hv) {
+                        const __half2 pa = __floats2half2_rn(__shfl_sync(~0u, e[u][0], 8 * c), __shfl_sync(~0u, e[u][0], 8 * c + 4));
+                        const __half2 pc = __floats2half2_rn(__shfl_sync(~0u, e[u][1], 8 * c), __shfl_sync(~0u, e[u][1], 8 * c + 4));
+#pragma unroll
+                        for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                uint32_t a0, a1, a2, a3;
+                                Codes8<__half>::expand_scaled(pairs(x, y, 0), pa, a0, a1);
+                                Codes8<__half>::expand_scaled(pairs(x, y, 2), pc, a2, a3);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) Mma16816<__half>::mma(o[nt][2 * x + y], a0, a1, a2, a3, pb[u][nt][0], pb[u][nt][1]);
+                            }
+                    } else if constexpr (!kHalf) {
+#pragma unroll
+                        for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                uint32_t a0, a1, a2, a3;
+                                Codes8<T>::expand(pairs(x, y, 0), a0, a1);
+                                Codes8<T>::expand(pairs(x, y, 2), a2, a3);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) M::mma(o[nt][2 * x + y], a0, a1, a2, a3, pb[u][nt][0], pb[u][nt][1]);
+                            }
+                    }
+                }
+            }
+            __syncwarp();                                                // every lane has used what it read
+            if (lane == 0) ptx::mbar_arrive(&s_free[warp][slot]);
+            if (++slot == kFewStages) {
+                slot = 0;
+                par ^= 1u;
             }
         }
+
+        // ---- merge: warps, then the CTAs of the cluster
+        float *sum = reinterpret_cast<float *>(fifo);                    // [kCols][D]
+        __syncwarp();                                                    // the warp's last reads of its FIFO
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int col = 8 * nt + 2 * c + x;
+                float v = l[nt][x];
+#pragma unroll
+                for (int y = 4; y < 32; y <<= 1) v += __shfl_xor_sync(~0u, v, y);
+                if (r == 0) {
+                    s_m[warp][col] = m[nt][x];
+                    s_l[warp][col] = v;
+                }
+            }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int mt = 0; mt < C::MT; ++mt)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)                              // m-tile mt: columns 64 (mt / 4) + 8 r + 2 (mt % 4) and the next
+                    *reinterpret_cast<float2 *>(sum + (8 * nt + 2 * c + x) * D + 64 * (mt / 4) + 8 * r + 2 * (mt % 4)) =
+                        make_float2(o[nt][mt][x], o[nt][mt][2 + x]);
     }
     if (failed) {
         p.seqs.raise(VQ_WORD_TIMEOUT);
 #pragma unroll 1
         for (int x = 0; x < (1 << 14); ++x) __nanosleep(256);        // tile loads still in flight get time to land
     }
-
-    // ---- merge: warps, then the CTAs of the cluster
-    float *sum = reinterpret_cast<float *>(fifo);                    // [kCols][D]
-    __syncwarp();                                                    // the warp's last reads of its FIFO
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int col = 8 * nt + 2 * c + x;
-            float v = l[nt][x];
-#pragma unroll
-            for (int y = 4; y < 32; y <<= 1) v += __shfl_xor_sync(~0u, v, y);
-            if (r == 0) {
-                s_m[warp][col] = m[nt][x];
-                s_l[warp][col] = v;
-            }
-        }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt)
-#pragma unroll
-            for (int x = 0; x < 2; ++x)                              // m-tile mt: columns 64 (mt / 4) + 8 r + 2 (mt % 4) and the next
-                *reinterpret_cast<float2 *>(sum + (8 * nt + 2 * c + x) * D + 64 * (mt / 4) + 8 * r + 2 * (mt % 4)) =
-                    make_float2(o[nt][mt][x], o[nt][mt][2 + x]);
     __syncthreads();
     const auto sum_of = [&](int w) { return reinterpret_cast<float *>(smem + w * C::kWarpBytes); };
     T *out = static_cast<T *>(p.out);
@@ -573,7 +585,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) paged_few_kernel(const __gr
         const int64_t t = t0 + col / p.G, h = hk * p.G + col % p.G;
         *reinterpret_cast<uint2 *>(out + t * p.o_t + h * p.o_h + d) = make_uint2(Pair16<T>::pack(v.x * inv, v.y * inv), Pair16<T>::pack(v.z * inv, v.w * inv));
     };
-    for (int x = tid; x < rows * (D / 4); x += kFewWarps * 32) {
+    for (int x = tid; x < rows * (D / 4); x += kFewThreads) {
         const int col = x / (D / 4), d = x % (D / 4) * 4;
         float mm = -INFINITY;
 #pragma unroll
@@ -600,7 +612,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) paged_few_kernel(const __gr
     if (nsplit == 1) return;
     const cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    for (int x = split * (kFewWarps * 32) + tid; x < rows * (D / 4); x += nsplit * (kFewWarps * 32)) {
+    for (int x = split * kFewThreads + tid; x < rows * (D / 4); x += nsplit * kFewThreads) {
         const int col = x / (D / 4), d = x % (D / 4) * 4;
         float mm = -INFINITY;
         for (int k = 0; k < nsplit; ++k) mm = fmaxf(mm, *cluster.map_shared_rank(&s_cm[col], k));
@@ -642,11 +654,13 @@ static int launch_few(const PagedAttnParams &p, cudaStream_t stream)
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return VQ_EDEVICE;
     auto kern = paged_few_kernel<T, Q8, D, NT>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kTotal) != cudaSuccess) return VQ_ELAUNCH;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kTotal) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return VQ_ELAUNCH;
     const int groups = p.max_q > 1 ? 2 : 1;                          // tokens of one sequence lie in at most two blocks of positions
     const int64_t units = static_cast<int64_t>(p.seqs.S) * groups * p.Hkv;
     int nsplit = 1;
-    while (nsplit < 8 && units * nsplit < 2 * sms) nsplit *= 2;
+    while (nsplit < kFewSplit && units * nsplit < 2 * sms) nsplit *= 2;
     if (units * nsplit > 0x7fffffff) return VQ_EUNSUPPORTED;
     constexpr bool f16 = !IsBf16<T>::value;
     CUtensorMap k1, k3, v, cb, vs;
@@ -657,17 +671,19 @@ static int launch_few(const PagedAttnParams &p, cudaStream_t stream)
     } else {
         cb = vs = k1;               // never read
     }
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(nsplit);
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(nsplit);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // see launch_overlapped
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(units * nsplit));
-    cfg.blockDim = dim3(kFewWarps * 32);
+    cfg.blockDim = dim3(kFewThreads);
     cfg.dynamicSmemBytes = C::kTotal;
     cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kern, k1, k3, v, cb, vs, p, groups, nsplit) == cudaSuccess ? launch_status() : (cudaGetLastError(), VQ_ELAUNCH);
 }
 
