@@ -231,12 +231,13 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
         if (step < st.n_far) {
             x = __ldg(p.cnt + far_base + step * 16 + (lane & 15));
         } else if constexpr (Q8) {
-            const int j = first_key(step) + lane, pg = j < n && j <= (i1 | 15) ? page_of(j) : -1, pr = j & page_mask;
-            const PagedPool &kp = step < st.n_far + st.n_old ? p.k3 : p.k1;
-            if (pg >= 0) {
-                x = __ldg(kp.scale + kp.scale_at(pg, hk, pr));
-                y = __ldg(p.v.scale + p.v.scale_at(pg, hk, pr));
-            }
+            const int j = first_key(step) + lane;
+            const bool in = j < n && j <= (i1 | 15), old = step < st.n_far + st.n_old;
+            const int pg = in ? page_of(j) : -1, page = max(pg, 0), pr = j & page_mask;
+            const float *ks = old ? p.k3.scale + p.k3.scale_at(page, hk, pr) : p.k1.scale + p.k1.scale_at(page, hk, pr);
+            x = __ldg(ks);
+            y = __ldg(p.v.scale + p.v.scale_at(page, hk, pr));
+            if (pg < 0) x = y = 0.f;
         }
     };
 
@@ -326,7 +327,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
                 }
             }
         };
-        // excluded keys of the 16 from j0 on; true: there is no such page
+        // excluded keys of the 16 from j0 on; true: there is no such page (bad: some page is missing)
         auto mask = [&](float (&sc)[NT][4], int j0, bool old) {
             if (bad && j0 <= i1 && page_of(j0) < 0) {
 #pragma unroll
@@ -391,60 +392,62 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
             if (far || !Q8) {
                 // ---- S^T = K Q^T, even and odd k-steps by themselves.  Piece j of row k lies at j ^ (k % 8); four lanes share a row, each
                 // takes two neighbouring pieces of its 128 bytes: the eight lanes that read together ask for different banks.
+                // All reads come first: what follows is code without branches but for the rare ones.
+                uint4 ka[2 * C::VC], kb[2 * C::VC], v4[C::VC][4];
+#pragma unroll
+                for (int j = 0; j < 2 * C::VC; ++j) {
+                    const uint8_t *at = stg + (j / 2) * C::kBox + r * 128 + (((2 * c + j % 2) ^ r) << 4);
+                    ka[j] = *reinterpret_cast<const uint4 *>(at);
+                    kb[j] = *reinterpret_cast<const uint4 *>(at + 8 * 128);
+                }
+#pragma unroll
+                for (int h = 0; h < C::VC; ++h)
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        const int k = 2 * c + (a & 1) + 8 * (a >> 1);
+                        v4[h][a] = *reinterpret_cast<const uint4 *>(stg + (C::VC + h) * C::kBox + k * 128 + ((r ^ (k & 7)) << 4));
+                    }
                 float sc[1][NT][4], s2[NT][4];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) sc[0][nt][x] = s2[nt][x] = 0.f;
 #pragma unroll
-                for (int h = 0; h < C::VC; ++h)
+                for (int j = 0; j < 2 * C::VC; ++j)
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const uint8_t *at = stg + h * C::kBox + r * 128 + (((2 * c + y) ^ r) << 4);
-                        const uint4 a = *reinterpret_cast<const uint4 *>(at), b = *reinterpret_cast<const uint4 *>(at + 8 * 128);
-                        const int j = 2 * h + y;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            M::mma(sc[0][nt], a.x, b.x, a.y, b.y, qf[nt][4 * j], qf[nt][4 * j + 1]);
-                            M::mma(s2[nt], a.z, b.z, a.w, b.w, qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
-                        }
+                    for (int nt = 0; nt < NT; ++nt) {
+                        M::mma(sc[0][nt], ka[j].x, kb[j].x, ka[j].y, kb[j].y, qf[nt][4 * j], qf[nt][4 * j + 1]);
+                        M::mma(s2[nt], ka[j].z, kb[j].z, ka[j].w, kb[j].w, qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
                     }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) sc[0][nt][x] = (sc[0][nt][x] + s2[nt][x]) * p.scale_log2;
-                float w[1][2] = {{1.f, 1.f}};
-                const float f[1][2] = {{1.f, 1.f}};
-                bool hole = false;
-                if (far) {
-                    w[0][0] = __shfl_sync(~0u, my_x, r);
-                    w[0][1] = __shfl_sync(~0u, my_x, r + 8);
+                // codes: counts as denominator weights, those without members excluded
+                const float cnt0 = __shfl_sync(~0u, my_x, r), cnt1 = __shfl_sync(~0u, my_x, r + 8);
+                const float w[1][2] = {{far ? cnt0 : 1.f, far ? cnt1 : 1.f}}, f[1][2] = {{1.f, 1.f}};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        if (!(w[0][0] > 0.f)) sc[0][nt][0] = sc[0][nt][1] = -INFINITY;
-                        if (!(w[0][1] > 0.f)) sc[0][nt][2] = sc[0][nt][3] = -INFINITY;
+                for (int nt = 0; nt < NT; ++nt) {
+                    if (!(w[0][0] > 0.f)) sc[0][nt][0] = sc[0][nt][1] = -INFINITY;
+                    if (!(w[0][1] > 0.f)) sc[0][nt][2] = sc[0][nt][3] = -INFINITY;
+                }
+                if (!far) {
+                    const bool hole = mask(sc[0], key0, old);
+                    if (hole || key0 + 16 > n) {                     // behind the sequence's end a page may hold anything: zeros instead
+#pragma unroll
+                        for (int h = 0; h < C::VC; ++h)
+#pragma unroll
+                            for (int a = 0; a < 4; ++a)
+                                if (hole || key0 + 2 * c + (a & 1) + 8 * (a >> 1) >= n) v4[h][a] = make_uint4(0, 0, 0, 0);
                     }
-                } else {
-                    hole = mask(sc[0], key0, old);
                 }
                 uint32_t pb[1][NT][2];
                 softmax(sc, w, f, pb, false);
                 // ---- O^T += V^T P^T
 #pragma unroll
                 for (int h = 0; h < C::VC; ++h) {
-                    uint4 v4[4];
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) {
-                        const int k = 2 * c + (a & 1) + 8 * (a >> 1);
-                        v4[a] = *reinterpret_cast<const uint4 *>(stg + (C::VC + h) * C::kBox + k * 128 + ((r ^ (k & 7)) << 4));
-                    }
-                    if (!far && (hole || key0 + 16 > n)) {               // behind the sequence's end a page may hold anything: zeros instead
-#pragma unroll
-                        for (int a = 0; a < 4; ++a)
-                            if (hole || key0 + 2 * c + (a & 1) + 8 * (a >> 1) >= n) v4[a] = make_uint4(0, 0, 0, 0);
-                    }
-                    const uint32_t v0[4] = {v4[0].x, v4[0].y, v4[0].z, v4[0].w}, v1[4] = {v4[1].x, v4[1].y, v4[1].z, v4[1].w};
-                    const uint32_t v2[4] = {v4[2].x, v4[2].y, v4[2].z, v4[2].w}, v3[4] = {v4[3].x, v4[3].y, v4[3].z, v4[3].w};
+                    const uint32_t v0[4] = {v4[h][0].x, v4[h][0].y, v4[h][0].z, v4[h][0].w}, v1[4] = {v4[h][1].x, v4[h][1].y, v4[h][1].z, v4[h][1].w};
+                    const uint32_t v2[4] = {v4[h][2].x, v4[h][2].y, v4[h][2].z, v4[h][2].w}, v3[4] = {v4[h][3].x, v4[h][3].y, v4[h][3].z, v4[h][3].w};
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const uint32_t a0 = __byte_perm(v0[x], v1[x], 0x5410), a1 = __byte_perm(v0[x], v1[x], 0x7632);
@@ -456,87 +459,96 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
             } else {
                 // 8-bit rows of 128 (64) bytes: piece j of row k lies at j ^ (k % 8)  (j ^ (k / 2 % 4))
                 auto piece = [&](int k, int j) { return D == 128 ? k * 128 + ((j ^ (k & 7)) << 4) : k * 64 + ((j ^ ((k >> 1) & 3)) << 4); };
-                float sc[2][NT][4], f[2][2], e[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
-                const float w[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
+                uint4 ka[2][C::VC], kb[2][C::VC];
+                uint32_t v[2][4][D / 32];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint8_t *kat = stg + 2 * u * C::kBox8, *vat = kat + C::kBox8 + 8 * (r & 1);
+#pragma unroll
+                    for (int j = 0; j < C::VC; ++j) {
+                        ka[u][j] = *reinterpret_cast<const uint4 *>(kat + piece(r, C::VC * c + j));
+                        kb[u][j] = *reinterpret_cast<const uint4 *>(kat + piece(r + 8, C::VC * c + j));
+                    }
+#pragma unroll
+                    for (int a = 0; a < 4; ++a)
+#pragma unroll
+                        for (int h = 0; h < C::VC; ++h) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(vat + piece(2 * c + (a & 1) + 8 * (a >> 1), 4 * h + (r >> 1)));
+                            v[u][a][2 * h] = x.x; v[u][a][2 * h + 1] = x.y;
+                        }
+                }
                 // Weights and values as halves: codes become halves in five instructions per four, bf16 in eight.  bf16 caches whose scales
                 // leave the range of a half take the latter.
                 const bool hv = kHalf || __all_sync(~0u, (my_y >= 5.9604645e-8f && my_y < 32.f) || my_y == 0.f);
+                float my_p2 = 1.f;
+                const float my_f = hv ? half_weight_factor(my_y, my_p2) : my_y;
+                const __half2 my_pair = __floats2half2_rn(my_p2, __shfl_down_sync(~0u, my_p2, 1));   // even lanes: of keys l, l + 1
+                float sc[2][NT][4], s2[2][NT][4], f[2][2];
+                const float w[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
+                __half2 p2[2][2];                                    // the powers of two that go with this thread's pairs of keys
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) sc[u][nt][x] = 0.f;
+                        for (int x = 0; x < 4; ++x) sc[u][nt][x] = s2[u][nt][x] = 0.f;
 #pragma unroll
                     for (int j = 0; j < C::VC; ++j) {
-                        const uint8_t *at = stg + 2 * u * C::kBox8;
-                        const uint4 a4 = *reinterpret_cast<const uint4 *>(at + piece(r, C::VC * c + j));
-                        const uint4 b4 = *reinterpret_cast<const uint4 *>(at + piece(r + 8, C::VC * c + j));
-                        const uint32_t a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+                        const uint32_t a[4] = {ka[u][j].x, ka[u][j].y, ka[u][j].z, ka[u][j].w}, b[4] = {kb[u][j].x, kb[u][j].y, kb[u][j].z, kb[u][j].w};
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
                             uint32_t al, ah, bl, bh;
                             Codes8<__half>::expand(a[x], al, ah);
                             Codes8<__half>::expand(b[x], bl, bh);
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) Mma16816<__half>::mma(sc[u][nt], al, bl, ah, bh, qf[nt][8 * j + 2 * x], qf[nt][8 * j + 2 * x + 1]);
+                            for (int nt = 0; nt < NT; ++nt)
+                                Mma16816<__half>::mma(x & 1 ? s2[u][nt] : sc[u][nt], al, bl, ah, bh, qf[nt][8 * j + 2 * x], qf[nt][8 * j + 2 * x + 1]);
                         }
                     }
-                    const float k0 = __shfl_sync(~0u, my_x, 16 * u + r), k1 = __shfl_sync(~0u, my_x, 16 * u + 8 + r);
-                    f[u][0] = __shfl_sync(~0u, my_y, 16 * u + r);
-                    f[u][1] = __shfl_sync(~0u, my_y, 16 * u + 8 + r);
-                    if (hv) {
-                        f[u][0] = half_weight_factor(f[u][0], e[u][0]);
-                        f[u][1] = half_weight_factor(f[u][1], e[u][1]);
-                    }
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int x = 0; x < 2; ++x) {
+                        const float k = __shfl_sync(~0u, my_x, 16 * u + 8 * x + r);
+                        f[u][x] = __shfl_sync(~0u, my_f, 16 * u + 8 * x + r);
+                        p2[u][x] = __shfl_sync(~0u, my_pair, 16 * u + 8 * x + 2 * c);
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            sc[u][nt][x] *= qu[nt][x] * k0;
-                            sc[u][nt][2 + x] *= qu[nt][x] * k1;
+                        for (int nt = 0; nt < NT; ++nt) {
+                            sc[u][nt][2 * x] = (sc[u][nt][2 * x] + s2[u][nt][2 * x]) * (qu[nt][0] * k);
+                            sc[u][nt][2 * x + 1] = (sc[u][nt][2 * x + 1] + s2[u][nt][2 * x + 1]) * (qu[nt][1] * k);
                         }
-                    mask(sc[u], key0 + 16 * u, old);
+                    }
                 }
+                mask(sc[0], key0, old);
+                mask(sc[1], key0 + 16, old);
                 uint32_t pb[2][NT][2];
                 softmax(sc, w, f, pb, hv);
+                // bytes 0, 1 (y = 0) and 2, 3 of word x: m-tiles 2 x, 2 x + 1
+                auto pairs = [&](int u, int x, int y, int a) { return __byte_perm(v[u][a][x], v[u][a + 1][x], y ? 0x7362 : 0x5140); };
+                if (hv) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    uint32_t v[4][D / 32];
-#pragma unroll
-                    for (int a = 0; a < 4; ++a)
-#pragma unroll
-                        for (int h = 0; h < C::VC; ++h) {
-                            const uint2 x = *reinterpret_cast<const uint2 *>(stg + (2 * u + 1) * C::kBox8 + piece(2 * c + (a & 1) + 8 * (a >> 1), 4 * h + (r >> 1)) + 8 * (r & 1));
-                            v[a][2 * h] = x.x; v[a][2 * h + 1] = x.y;
-                        }
-                    // bytes 0, 1 (y = 0) and 2, 3 of word x: m-tiles 2 x, 2 x + 1
-                    auto pairs = [&](int x, int y, int a) { return __byte_perm(v[a][x], v[a + 1][x], y ? 0x7362 : 0x5140); };
-                    if (hv) {
-                        const __half2 pa = __floats2half2_rn(__shfl_sync(~0u, e[u][0], 8 * c), __shfl_sync(~0u, e[u][0], 8 * c + 4));
-                        const __half2 pc = __floats2half2_rn(__shfl_sync(~0u, e[u][1], 8 * c), __shfl_sync(~0u, e[u][1], 8 * c + 4));
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int x = 0; x < D / 32; ++x)
 #pragma unroll
                             for (int y = 0; y < 2; ++y) {
                                 uint32_t a0, a1, a2, a3;
-                                Codes8<__half>::expand_scaled(pairs(x, y, 0), pa, a0, a1);
-                                Codes8<__half>::expand_scaled(pairs(x, y, 2), pc, a2, a3);
+                                Codes8<__half>::expand_scaled(pairs(u, x, y, 0), p2[u][0], a0, a1);
+                                Codes8<__half>::expand_scaled(pairs(u, x, y, 2), p2[u][1], a2, a3);
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) Mma16816<__half>::mma(o[nt][2 * x + y], a0, a1, a2, a3, pb[u][nt][0], pb[u][nt][1]);
                             }
-                    } else if constexpr (!kHalf) {
+                } else if constexpr (!kHalf) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int x = 0; x < D / 32; ++x)
 #pragma unroll
                             for (int y = 0; y < 2; ++y) {
                                 uint32_t a0, a1, a2, a3;
-                                Codes8<T>::expand(pairs(x, y, 0), a0, a1);
-                                Codes8<T>::expand(pairs(x, y, 2), a2, a3);
+                                Codes8<T>::expand(pairs(u, x, y, 0), a0, a1);
+                                Codes8<T>::expand(pairs(u, x, y, 2), a2, a3);
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) M::mma(o[nt][2 * x + y], a0, a1, a2, a3, pb[u][nt][0], pb[u][nt][1]);
                             }
-                    }
                 }
             }
             __syncwarp();                                                // every lane has used what it read
