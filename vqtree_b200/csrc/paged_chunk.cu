@@ -189,7 +189,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
     constexpr int NH = C::NH, NS = C::kSlots, NB = C::kBufs;
     const PagedAttnParams &p = cp.a;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *smem = smem_raw + (-ptx::smem_u32(smem_raw) & 1023u);   // stays an address of shared memory for the compiler
     __shared__ __align__(8) uint64_t bar_q, kv_full[NS], kv_empty[NS], s_full[NB], p_full[NB], pv_done[NB], refbar[NB][4], endbar, sc_full[C::kScal];
     __shared__ uint32_t s_tmem;
     __shared__ int s_err, s_some;

@@ -83,7 +83,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
     using C = FewCfg<T, Q8, D, NT>;
     using M = Mma16816<T>;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *smem = smem_raw + (-ptx::smem_u32(smem_raw) & 1023u);   // stays an address of shared memory for the compiler
     __shared__ __align__(8) uint64_t s_bar[kFewWarps][kFewStages], s_free[kFewWarps][kFewStages];
     __shared__ int s_bad;                                            // some page of the unit is missing, or not kept in shared memory
     __shared__ float s_m[kFewWarps][C::kCols], s_l[kFewWarps][C::kCols];
