@@ -470,23 +470,23 @@ class PagedKV(NamedTuple):
         return cls(pool(), pool(), pool() if raw_keys else None, scale(), scale(), scale() if raw_keys else None)
 
 
-def _paged(which: int, *args) -> None:
-    """One of the paged operators (append, read, attention) through the dispatcher; its first argument is a tensor."""
+_PAGED_CALLS = None
+
+
+def _paged_calls(t: torch.Tensor):
+    """(the paged operators, the status word of t's device)"""
     global _PAGED_CALLS
     if _PAGED_CALLS is None:
         from . import torch_ops
         _PAGED_CALLS = torch_ops.paged_calls()
-    word = _STATUS.get(args[0].get_device())
-    if word is None:
-        word = device_status_word(_require_cuda(args[0]))
-    status = _PAGED_CALLS[which](*args, word)
-    if status != 0:
-        if status == -4:                                    # VQ_EDEVICE: host tensors and mixed devices are reported as everywhere here
-            _require_cuda(*(t for t in args if isinstance(t, torch.Tensor)))
-        check(status, ("vqattn_paged_append", "vqattn_paged_read", "vqattn_paged_attention")[which])
+    word = _STATUS.get(t.get_device())
+    return _PAGED_CALLS, device_status_word(_require_cuda(t)) if word is None else word
 
 
-_PAGED_CALLS = None
+def _paged_failed(status: int, where: str, *tensors) -> None:
+    if status == -4:                                        # VQ_EDEVICE: host tensors and mixed devices are reported as everywhere here
+        _require_cuda(*tensors)
+    check(status, where)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, pages: PagedKV, block_table: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor,
@@ -499,20 +499,24 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pages: PagedKV, block_table: 
     block_table int32 [S,MB]: page of tokens [P*c, P*(c+1)) of a sequence; cu_q int32 [S+1]: sequence s brings rows cu_q[s] ..
     cu_q[s+1]-1; seq_lens int32 [S]: its length with them.  rotate=False stores keys (and returns queries) as they are.
     n_pos: an upper bound of the positions + 1 (None: what the table can address)."""
-    q1 = q.new_empty(q.shape) if q is not None else None
-    q2 = q.new_empty(q.shape) if q is not None and const_pos is not None else None
     if k.shape[0] == 0:
-        return q1, q2
-    if not k.is_cuda:
-        _require_cuda(k)
+        return (None, None) if q is None else (q.new_empty(q.shape), q.new_empty(q.shape) if const_pos is not None else None)
+    calls, word = _paged_calls(k)
     cos = sin = None
     const = const_pos or 0
     if rotate:
         n = n_pos if n_pos is not None else block_table.shape[1] * pages.k1.shape[2]
         cos, sin = rope_tables(max(n, const + 1), k.shape[2], k.device, base)
     k1, vp, k3, k1_scale, v_scale, k3_scale = pages
-    _paged(0, k, v, k1, vp, k3, k1_scale, v_scale, k3_scale, block_table, cu_q, seq_lens, q, q1, q2, cos, sin, const)
-    return q1, q2
+    q1 = q2 = None
+    if q is None:
+        status = calls[0](k, v, k1, vp, k3, k1_scale, v_scale, k3_scale, block_table, cu_q, seq_lens, None, None, None, cos, sin, const, word)
+    else:
+        q1, q2, status = calls[2](k, v, k1, vp, k3, k1_scale, v_scale, k3_scale, block_table, cu_q, seq_lens, q, const_pos is not None, cos, sin,
+                                  const, word)
+    if status != 0:
+        _paged_failed(status, "vqattn_paged_append", k, v, *pages, block_table, cu_q, seq_lens, q)
+    return q1, q2 if const_pos is not None else None
 
 
 def paged_read(pools, block_table: torch.Tensor, starts: torch.Tensor, seq_lens: torch.Tensor, n: int,
@@ -527,12 +531,13 @@ def paged_read(pools, block_table: torch.Tensor, starts: torch.Tensor, seq_lens:
         raise ValueError("one to three pools")
     first = pools[0][0]
     dt = out_dtype or (torch.float32 if first.dtype == torch.int8 else first.dtype)
-    shape = (block_table.shape[0], first.shape[1], n, first.shape[3])
-    outs = [first.new_empty(shape, dtype=dt) for _ in pools]
-    if shape[0] == 0 or n == 0:
-        return outs
-    args = [x for (pool, scale), out in zip(pools, outs) for x in (pool, scale, out)]
-    _paged(1, *args, *(None,) * (9 - len(args)), block_table, starts, seq_lens)
+    if block_table.shape[0] == 0 or n == 0:
+        return [first.new_empty((block_table.shape[0], first.shape[1], n, first.shape[3]), dtype=dt) for _ in pools]
+    calls, word = _paged_calls(first)
+    tensors, scales = [p[0] for p in pools], [p[1] for p in pools]
+    outs, status = calls[3](tensors, scales, block_table, starts, seq_lens, n, dt, word)
+    if status != 0:
+        _paged_failed(status, "vqattn_paged_read", *tensors, *scales, block_table, starts, seq_lens)
     return outs
 
 
@@ -547,18 +552,22 @@ def paged_attention(q1: torch.Tensor, q2: torch.Tensor, pages: PagedKV, block_ta
     tokens of one sequence.  codebook [Hkv,MK,D], cnt [NS,Hkv,MK] f32, vsum [NS,Hkv,MK,D], snap_table int32 [S,MS]: keys before the
     boundary b of a query count through snapshot ``snap_table[s, b // 128 % MS]`` (None: the local part only).  Returns [T,Hq,D]; rows
     from cu_q[S] on are left as they are."""
-    far = (codebook, cnt, vsum, snap_table)
-    if codebook is not None and any(t is None for t in far):
-        raise ValueError("codebook, cnt, vsum and snap_table go together")
-    if out is None:
-        out = q1.new_empty(q1.shape)
-    if q1.shape[0] == 0:
-        return out
     if codebook is None:
-        far = (None,) * 4
+        cnt = vsum = snap_table = None
+    elif cnt is None or vsum is None or snap_table is None:
+        raise ValueError("codebook, cnt, vsum and snap_table go together")
+    if q1.shape[0] == 0:
+        return q1.new_empty(q1.shape) if out is None else out
+    calls, word = _paged_calls(q1)
     k1, vp, k3, k1_scale, v_scale, k3_scale = pages
-    _paged(2, q1, q2, k1, vp, k3, k1_scale, v_scale, k3_scale, block_table, cu_q, seq_lens, *far, int(window), int(max_q),
-           float(scale) if scale else 0.0, out)
+    if out is None:
+        out, status = calls[4](q1, q2, k1, vp, k3, k1_scale, v_scale, k3_scale, block_table, cu_q, seq_lens, codebook, cnt, vsum, snap_table, window,
+                               max_q, scale or 0.0, word)
+    else:
+        status = calls[1](q1, q2, k1, vp, k3, k1_scale, v_scale, k3_scale, block_table, cu_q, seq_lens, codebook, cnt, vsum, snap_table, window, max_q,
+                          scale or 0.0, out, word)
+    if status != 0:
+        _paged_failed(status, "vqattn_paged_attention", q1, q2, *pages, block_table, cu_q, seq_lens, codebook, cnt, vsum, snap_table, out)
     return out
 
 

@@ -25,10 +25,15 @@ struct PagedAttnParams {
 
     __device__ __forceinline__ int boundary(int i) const { return i > W ? (i - W) / kBlock * kBlock : 0; }
     // snapshot of boundary b of sequence s; -1: none is wanted, or the table names none (reported)
-    __device__ __forceinline__ int snapshot(int s, int b) const
+    __device__ __forceinline__ int snapshot(int s, int b) const { return checked_snapshot(b, snapshot_entry(s, b)); }
+    // the same in two parts: what the table says, and the check
+    __device__ __forceinline__ int snapshot_entry(int s, int b) const
+    {
+        return b > 0 && cb != nullptr ? __ldg(snap + s * snap_row + (b / kBlock) % MS) : -1;
+    }
+    __device__ __forceinline__ int checked_snapshot(int b, int id) const
     {
         if (b <= 0 || cb == nullptr) return -1;
-        const int id = __ldg(snap + s * snap_row + (b / kBlock) % MS);
         if (id >= 0 && id < NS) return id;
         seqs.raise(VQ_WORD_BAD_PAGE);
         return -1;

@@ -27,9 +27,6 @@ namespace vq {
 
 namespace cg = cooperative_groups;
 
-constexpr int kFewWarps = 4;
-constexpr int kFewThreads = (kFewWarps + 1) * 32;   // and the warp that issues the loads
-constexpr int kFewStages = 3;
 constexpr int kFewSplit = 16;           // CTAs of a cluster at most (more than 8 are opt-in on this architecture)
 constexpr float kFewLazy = 8.f;         // log2 units a score may exceed its row's reference before the sums are rescaled
 
@@ -56,17 +53,23 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x)
 }
 template <typename T, bool Q8, int D, int NT>
 struct FewCfg {
+    // Warps that compute (one more issues the loads), stages of their FIFOs, CTAs of an SM: what registers and shared memory allow.  Measured,
+    // us: 64 sequences of 8 kv heads, 16 bits, 3 warps x 2 stages x 4 CTAs / 4 x 3 x 2: 136 / 152 (all 512 units run at once); 16 sequences
+    // of 32 heads, 8 bits, 5 x 2 x 2 / 4 x 3 x 2 / 3 x 2 x 3: 77 / 87 / 104.
+    static constexpr int kWarps = Q8 ? 5 : NT == 1 ? 3 : 4, kThreads = (kWarps + 1) * 32;
+    static constexpr int kStages = NT == 1 ? 2 : 3;
+    static constexpr int kCtas = NT == 1 ? (Q8 ? 2 : 4) : NT == 2 ? 2 : 1;
     static constexpr int kCols = 8 * NT;                         // query rows, padded
     static constexpr int VC = D / 64;                            // boxes of 64 columns of a 16-bit row
     static constexpr int kBox = 16 * 128;                        // bytes of 16 rows x 64 columns of 16 bits
     static constexpr int kBox8 = 16 * D;                         // 16 rows of 8 bits
     static constexpr int kStage = 2 * VC * kBox;                 // 16 keys with their values, or 32 of 8 bits
     static_assert(4 * kBox8 == kStage, "a stage holds twice as many 8-bit rows");
-    static constexpr int kWarpBytes = kFewStages * kStage;
+    static constexpr int kWarpBytes = kStages * kStage;
     static constexpr int kQ = (Q8 ? 3 : 2) * kCols * D * 2;      // rows q1, q2; 8-bit rows: q2, and both as halves
     static constexpr int kPages = 256;                           // page table entries kept in shared memory; the rest is read where it is needed
-    static constexpr int kTotal = kFewWarps * kWarpBytes + kQ + kPages * 4 + 1024;   // + slack for 1024-byte alignment
-    static_assert(kCols * D * 4 <= kFewStages * kStage, "a warp's sums fit into its FIFO");
+    static constexpr int kTotal = kWarps * kWarpBytes + kQ + kPages * 4 + 1024;   // + slack for 1024-byte alignment
+    static_assert(kCols * D * 4 <= kStages * kStage, "a warp's sums fit into its FIFO");
     static constexpr int MT = D / 16;
 };
 
@@ -76,7 +79,7 @@ struct FewSteps {
 };
 
 template <typename T, bool Q8, int D, int NT>
-__global__ void __launch_bounds__(kFewThreads, NT == 4 ? 1 : 2)
+__global__ void __launch_bounds__(FewCfg<T, Q8, D, NT>::kThreads, FewCfg<T, Q8, D, NT>::kCtas)
 paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constant__ CUtensorMap tm_k3, const __grid_constant__ CUtensorMap tm_v,
                  const __grid_constant__ CUtensorMap tm_cb, const __grid_constant__ CUtensorMap tm_vs, const PagedAttnParams p, int groups, int nsplit)
 {
@@ -84,16 +87,16 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
     using M = Mma16816<T>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-ptx::smem_u32(smem_raw) & 1023u);   // stays an address of shared memory for the compiler
-    __shared__ __align__(8) uint64_t s_bar[kFewWarps][kFewStages], s_free[kFewWarps][kFewStages];
+    __shared__ __align__(8) uint64_t s_bar[C::kWarps][C::kStages], s_free[C::kWarps][C::kStages];
     __shared__ int s_bad;                                            // some page of the unit is missing, or not kept in shared memory
-    __shared__ float s_m[kFewWarps][C::kCols], s_l[kFewWarps][C::kCols];
+    __shared__ float s_m[C::kWarps][C::kCols], s_l[C::kWarps][C::kCols];
     __shared__ float s_cm[C::kCols], s_cl[C::kCols];
     __shared__ float s_unit[2][Q8 ? C::kCols : 1];                   // 8-bit rows: the power of two a query row was divided by
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int r = lane >> 2, c = lane & 3;
-    T *s_q = reinterpret_cast<T *>(smem + kFewWarps * C::kWarpBytes);        // [2][kCols][D]
+    T *s_q = reinterpret_cast<T *>(smem + C::kWarps * C::kWarpBytes);        // [2][kCols][D]
     __half *s_qh = reinterpret_cast<__half *>(s_q + C::kCols * D);           // 8-bit rows: [q1, q2][kCols][D]
-    int *s_page = reinterpret_cast<int *>(smem + kFewWarps * C::kWarpBytes + C::kQ);
+    int *s_page = reinterpret_cast<int *>(smem + C::kWarps * C::kWarpBytes + C::kQ);
 
     const int split = blockIdx.x % nsplit;
     int unit = blockIdx.x / nsplit;
@@ -113,68 +116,66 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
         if (i0 > i1) return;
     }
     const int rows = (i1 - i0 + 1) * p.G;
-    const int bd = p.boundary(i0), snap = p.snapshot(s, bd);
+    const int bd = p.boundary(i0), entry = p.snapshot_entry(s, bd);
     FewSteps st;
     constexpr bool kHalf = Q8 && !IsBf16<T>::value;
     constexpr int KEYS = Q8 ? 32 : 16;                               // keys per step of window rows
-    st.n_far = snap >= 0 ? p.MK / 16 : 0;
     st.old0 = bd;
     const int old_end = p.rerope ? max(0, i1 - p.W) : 0;             // raw keys: [bd, old_end)
     st.n_old = old_end > bd ? (old_end - bd + KEYS - 1) / KEYS : 0;
     st.near0 = (p.rerope ? max(0, i0 - p.W) : bd) & ~15;
     st.n_near = (i1 - st.near0) / KEYS + 1;
-    const int total = st.n_far + st.n_old + st.n_near;
+    int snap = -1, total = 0;
+    auto plan = [&]() {                                              // uses the table's entry, which has been under way since
+        snap = p.checked_snapshot(bd, entry);
+        st.n_far = snap >= 0 ? p.MK / 16 : 0;
+        total = st.n_far + st.n_old + st.n_near;
+    };
     const int col0 = bd >> p.seqs.log_p, cols = (i1 >> p.seqs.log_p) - col0 + 1;
 
-    if (tid == 0) {
-        for (int w = 0; w < kFewWarps; ++w)
-            for (int x = 0; x < kFewStages; ++x) {
-                ptx::mbar_init(&s_bar[w][x], 1);
-                ptx::mbar_init(&s_free[w][x], 1);
-            }
-        ptx::fence_mbar_init();
-        s_bad = cols > C::kPages;
-    }
-    __syncthreads();
-    for (int x = tid; x < min(cols, C::kPages); x += kFewThreads) {
-        s_page[x] = p.seqs.page(s, col0 + x);
-        if (s_page[x] < 0) s_bad = 1;
-    }
-    // ---- query rows.  Rows behind `rows` are zeros.
-    auto q_row = [&](int which, int row) {
-        const int64_t t = t0 + row / p.G, h = hk * p.G + row % p.G;
-        return which ? static_cast<const T *>(p.q2) + t * p.q2_t + h * p.q2_h : static_cast<const T *>(p.q1) + t * p.q1_t + h * p.q1_h;
-    };
-    for (int x = tid; x < (Q8 ? 1 : 2) * C::kCols * D / 8; x += kFewThreads) {
-        const int which = Q8 ? 1 : x / (C::kCols * D / 8), row = x / (D / 8) % C::kCols, d = x % (D / 8) * 8;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < rows) v = *reinterpret_cast<const uint4 *>(q_row(which, row) + d);
-        reinterpret_cast<uint4 *>(s_q)[x] = v;
-    }
-    if constexpr (Q8) {
-        for (int x = warp; x < 2 * C::kCols; x += kFewWarps + 1) {
-            const int which = x / C::kCols, row = x % C::kCols;
-            float e[D / 32], top = 0.f;
+    // The other warps fetch the query rows while the loading warp (below) sets up the barriers and the page table and goes ahead; they meet at a
+    // named barrier where that one does not stop.
+    if (warp != C::kWarps) {
+        // ---- query rows.  Rows behind `rows` are zeros.
+        auto q_row = [&](int which, int row) {
+            const int64_t t = t0 + row / p.G, h = hk * p.G + row % p.G;
+            return which ? static_cast<const T *>(p.q2) + t * p.q2_t + h * p.q2_h : static_cast<const T *>(p.q1) + t * p.q1_t + h * p.q1_h;
+        };
+        for (int x = tid; x < (Q8 ? 1 : 2) * C::kCols * D / 8; x += C::kWarps * 32) {
+            const int which = Q8 ? 1 : x / (C::kCols * D / 8), row = x / (D / 8) % C::kCols, d = x % (D / 8) * 8;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (row < rows) v = *reinterpret_cast<const uint4 *>(q_row(which, row) + d);
+            reinterpret_cast<uint4 *>(s_q)[x] = v;
+        }
+        if constexpr (Q8) {
+            for (int x = warp; x < 2 * C::kCols; x += C::kWarps) {
+                const int which = x / C::kCols, row = x % C::kCols;
+                float e[D / 32], top = 0.f;
+                int shift = 0;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                e[i] = row < rows ? to_f32(q_row(which, row)[lane * (D / 32) + i]) : 0.f;
-                top = fmaxf(top, fabsf(e[i]));
-            }
-            int shift = 0;
-            if constexpr (IsBf16<T>::value) {
+                for (int i = 0; i < D / 32; ++i) e[i] = 0.f;
+                if (row < rows) {
 #pragma unroll
-                for (int y = 16; y; y >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, y));
-                const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-                if (top > 0.f && ex < 128) shift = max(-100, ex) - 10;
-            }
-            const float mul = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+                    for (int i = 0; i < D / 32; ++i) {
+                        e[i] = to_f32(q_row(which, row)[lane * (D / 32) + i]);
+                        top = fmaxf(top, fabsf(e[i]));
+                    }
+                    if constexpr (IsBf16<T>::value) {
 #pragma unroll
-            for (int i = 0; i < D / 32; i += 2)
-                *reinterpret_cast<__half2 *>(s_qh + (which * C::kCols + row) * D + lane * (D / 32) + i) = __floats2half2_rn(e[i] * mul, e[i + 1] * mul);
-            if (lane == 0) s_unit[which][row] = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+                        for (int y = 16; y; y >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, y));
+                        const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+                        if (top > 0.f && ex < 128) shift = max(-100, ex) - 10;
+                    }
+                }
+                const float mul = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+#pragma unroll
+                for (int i = 0; i < D / 32; i += 2)
+                    *reinterpret_cast<__half2 *>(s_qh + (which * C::kCols + row) * D + lane * (D / 32) + i) = __floats2half2_rn(e[i] * mul, e[i + 1] * mul);
+                if (lane == 0) s_unit[which][row] = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+            }
         }
     }
-    __syncthreads();
+    plan();
 
     const int64_t far_base = (static_cast<int64_t>(snap < 0 ? 0 : snap) * p.Hkv + hk) * p.MK;
     const int page_mask = (1 << p.seqs.log_p) - 1;
@@ -182,7 +183,6 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
         const int x = (j >> p.seqs.log_p) - col0;
         return x < C::kPages ? s_page[x] : p.seqs.page(s, x + col0);
     };
-    const bool bad = s_bad;
     auto first_key = [&](int step) {
         return step < st.n_far + st.n_old ? st.old0 + (step - st.n_far) * KEYS : st.near0 + (step - st.n_far - st.n_old) * KEYS;
     };
@@ -241,23 +241,57 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
         }
     };
 
-    const int stride = nsplit * kFewWarps;
+    const int stride = nsplit * C::kWarps;
     bool failed = false;
-    if (warp == kFewWarps) {
-        // lane w keeps warp w's FIFO full
-        if (lane < kFewWarps) {
-            int slot = 0;
-            uint32_t par = 1u;
-            for (int step = split * kFewWarps + lane, x = 0; step < total; step += stride, ++x) {
-                if (x >= kFewStages && !ptx::mbar_wait(&s_free[lane][slot], par, p.wait_limit)) {
-                    failed = true;
-                    break;
+    if (warp == C::kWarps) {
+        if (lane == 0) {
+            for (int w = 0; w < C::kWarps; ++w)
+                for (int x = 0; x < C::kStages; ++x) {
+                    ptx::mbar_init(&s_bar[w][x], 1);
+                    ptx::mbar_init(&s_free[w][x], 1);
                 }
-                fill(lane, step, slot);
-                if (++slot == kFewStages) {
-                    slot = 0;
-                    par ^= 1u;
-                }
+            ptx::fence_mbar_init();
+        }
+        __syncwarp();
+        // Lane w looks after warp w's FIFO: step and stage of its next fill.  Those that find their stage free are served one after another by
+        // one elected thread; nobody waits for a warp that is behind.
+        int step = lane < C::kWarps ? split * C::kWarps + lane : total, fills = 0, slot = 0;
+        uint32_t par = 1u;
+        auto serve = [&](bool ready) {
+            for (unsigned left = __ballot_sync(~0u, ready); left; left &= left - 1) {
+                const int w = __ffs(left) - 1, at = __shfl_sync(~0u, step, w), to = __shfl_sync(~0u, slot, w);
+                if (ptx::elect_one()) fill(w, at, to);
+                __syncwarp();
+            }
+            if (!ready) return;
+            step += stride;
+            ++fills;
+            if (++slot == C::kStages) {
+                slot = 0;
+                par ^= 1u;
+            }
+        };
+#pragma unroll 1
+        for (int x = 0; x < C::kStages; ++x) serve(step < st.n_far);  // codes need no page table
+        bool miss = cols > C::kPages;
+        for (int x = lane; x < min(cols, C::kPages); x += 32) {
+            const int pg = p.seqs.page(s, col0 + x);
+            s_page[x] = pg;
+            miss = miss || pg < 0;
+        }
+        miss = __any_sync(~0u, miss);
+        if (lane == 0) s_bad = miss;
+        __syncwarp();
+        asm volatile("bar.arrive 1, %0;" ::"n"(C::kThreads) : "memory");
+        long long since = clock64();
+        while (__any_sync(~0u, step < total)) {
+            const bool ready = step < total && (fills < C::kStages || ptx::mbar_test(&s_free[lane][slot], par));
+            if (__any_sync(~0u, ready)) {
+                serve(ready);
+                since = clock64();
+            } else if (clock64() - since > p.wait_limit) {
+                failed = true;
+                break;
             }
         }
     } else {
@@ -274,7 +308,9 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
         }
         uint32_t qf[NT][D / 8];
         uint8_t *const fifo = smem + warp * C::kWarpBytes;
-        const int first = split * kFewWarps + warp;
+        const int first = split * C::kWarps + warp;
+        asm volatile("bar.sync 1, %0;" ::"n"(C::kThreads) : "memory");
+        const bool bad = s_bad;
         float next_x, next_y;
         extras(first, next_x, next_y);
         // sc: scores of keys r and r + 8 of each group of 16 (c0 c1 | c2 c3) in log2 units, -inf where excluded -> weights; w: denominator weights of
@@ -459,6 +495,12 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
             } else {
                 // 8-bit rows of 128 (64) bytes: piece j of row k lies at j ^ (k % 8)  (j ^ (k / 2 % 4))
                 auto piece = [&](int k, int j) { return D == 128 ? k * 128 + ((j ^ (k & 7)) << 4) : k * 64 + ((j ^ ((k >> 1) & 3)) << 4); };
+                // Weights and values as halves: codes become halves in five instructions per four, bf16 in eight.  bf16 caches whose scales
+                // leave the range of a half take the latter.
+                const bool hv = kHalf || __all_sync(~0u, (my_y >= 5.9604645e-8f && my_y < 32.f) || my_y == 0.f);
+                float my_p2 = 1.f;
+                const float my_f = hv ? half_weight_factor(my_y, my_p2) : my_y;
+                const __half2 my_pair = __floats2half2_rn(my_p2, __shfl_down_sync(~0u, my_p2, 1));   // even lanes: of keys l, l + 1
                 uint4 ka[2][C::VC], kb[2][C::VC];
                 uint32_t v[2][4][D / 32];
 #pragma unroll
@@ -477,15 +519,8 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
                             v[u][a][2 * h] = x.x; v[u][a][2 * h + 1] = x.y;
                         }
                 }
-                // Weights and values as halves: codes become halves in five instructions per four, bf16 in eight.  bf16 caches whose scales
-                // leave the range of a half take the latter.
-                const bool hv = kHalf || __all_sync(~0u, (my_y >= 5.9604645e-8f && my_y < 32.f) || my_y == 0.f);
-                float my_p2 = 1.f;
-                const float my_f = hv ? half_weight_factor(my_y, my_p2) : my_y;
-                const __half2 my_pair = __floats2half2_rn(my_p2, __shfl_down_sync(~0u, my_p2, 1));   // even lanes: of keys l, l + 1
-                float sc[2][NT][4], s2[2][NT][4], f[2][2];
-                const float w[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
-                __half2 p2[2][2];                                    // the powers of two that go with this thread's pairs of keys
+                float sc[2][NT][4], s2[2][NT][4], f[2][2], w[2][2];
+                __half2 p2[2][2];                                   // the powers of two that go with this thread's pairs of keys
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -508,6 +543,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const float k = __shfl_sync(~0u, my_x, 16 * u + 8 * x + r);
+                        w[u][x] = 1.f;
                         f[u][x] = __shfl_sync(~0u, my_f, 16 * u + 8 * x + r);
                         p2[u][x] = __shfl_sync(~0u, my_pair, 16 * u + 8 * x + 2 * c);
 #pragma unroll
@@ -517,8 +553,8 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
                         }
                     }
                 }
-                mask(sc[0], key0, old);
-                mask(sc[1], key0 + 16, old);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) mask(sc[u], key0 + 16 * u, old);
                 uint32_t pb[2][NT][2];
                 softmax(sc, w, f, pb, hv);
                 // bytes 0, 1 (y = 0) and 2, 3 of word x: m-tiles 2 x, 2 x + 1
@@ -553,7 +589,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
             }
             __syncwarp();                                                // every lane has used what it read
             if (lane == 0) ptx::mbar_arrive(&s_free[warp][slot]);
-            if (++slot == kFewStages) {
+            if (++slot == C::kStages) {
                 slot = 0;
                 par ^= 1u;
             }
@@ -597,15 +633,15 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
         const int64_t t = t0 + col / p.G, h = hk * p.G + col % p.G;
         *reinterpret_cast<uint2 *>(out + t * p.o_t + h * p.o_h + d) = make_uint2(Pair16<T>::pack(v.x * inv, v.y * inv), Pair16<T>::pack(v.z * inv, v.w * inv));
     };
-    for (int x = tid; x < rows * (D / 4); x += kFewThreads) {
+    for (int x = tid; x < rows * (D / 4); x += C::kThreads) {
         const int col = x / (D / 4), d = x % (D / 4) * 4;
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, s_m[w][col]);
+        for (int w = 0; w < C::kWarps; ++w) mm = fmaxf(mm, s_m[w][col]);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float den = 0.f;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) {
+        for (int w = 0; w < C::kWarps; ++w) {
             const float a = s_m[w][col] == -INFINITY ? 0.f : ptx::ex2(s_m[w][col] - mm);
             const float4 y = *reinterpret_cast<const float4 *>(sum_of(w) + col * D + d);
             v.x = fmaf(a, y.x, v.x); v.y = fmaf(a, y.y, v.y); v.z = fmaf(a, y.z, v.z); v.w = fmaf(a, y.w, v.w);
@@ -624,17 +660,33 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
     if (nsplit == 1) return;
     const cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    for (int x = split * kFewThreads + tid; x < rows * (D / 4); x += nsplit * kFewThreads) {
+    for (int x = split * C::kThreads + tid; x < rows * (D / 4); x += nsplit * C::kThreads) {
         const int col = x / (D / 4), d = x % (D / 4) * 4;
-        float mm = -INFINITY;
-        for (int k = 0; k < nsplit; ++k) mm = fmaxf(mm, *cluster.map_shared_rank(&s_cm[col], k));
+        // four CTAs at a time, their loads under way together
+        float mm = -INFINITY, den = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        float den = 0.f;
-        for (int k = 0; k < nsplit; ++k) {
-            const float mk = *cluster.map_shared_rank(&s_cm[col], k), a = mk == -INFINITY ? 0.f : ptx::ex2(mk - mm);
-            const float4 y = *cluster.map_shared_rank(reinterpret_cast<float4 *>(sum_of(0) + col * D + d), k);
-            v.x = fmaf(a, y.x, v.x); v.y = fmaf(a, y.y, v.y); v.z = fmaf(a, y.z, v.z); v.w = fmaf(a, y.w, v.w);
-            den = fmaf(a, *cluster.map_shared_rank(&s_cl[col], k), den);
+        for (int k0 = 0; k0 < nsplit; k0 += 4) {
+            float mk[4], lk[4];
+            float4 y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int from = min(k0 + k, nsplit - 1);
+                mk[k] = *cluster.map_shared_rank(&s_cm[col], from);
+                lk[k] = *cluster.map_shared_rank(&s_cl[col], from);
+                y[k] = *cluster.map_shared_rank(reinterpret_cast<float4 *>(sum_of(0) + col * D + d), from);
+                if (k0 + k >= nsplit) mk[k] = -INFINITY;
+            }
+            const float top = fmaxf(mm, fmaxf(fmaxf(mk[0], mk[1]), fmaxf(mk[2], mk[3])));
+            const float keep = mm == -INFINITY ? 0.f : ptx::ex2(mm - top);
+            v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+            den *= keep;
+            mm = top;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float a = mk[k] == -INFINITY ? 0.f : ptx::ex2(mk[k] - top);
+                v.x = fmaf(a, y[k].x, v.x); v.y = fmaf(a, y[k].y, v.y); v.z = fmaf(a, y[k].z, v.z); v.w = fmaf(a, y[k].w, v.w);
+                den = fmaf(a, lk[k], den);
+            }
         }
         store(col, d, v, den);
     }
@@ -672,7 +724,9 @@ static int launch_few(const PagedAttnParams &p, cudaStream_t stream)
     const int groups = p.max_q > 1 ? 2 : 1;                          // tokens of one sequence lie in at most two blocks of positions
     const int64_t units = static_cast<int64_t>(p.seqs.S) * groups * p.Hkv;
     int nsplit = 1;
-    while (nsplit < kFewSplit && units * nsplit < 2 * sms) nsplit *= 2;
+    // As many CTAs of a cluster as the SMs hold at once: a second round would start when the first one ends.  (The second block of positions of a
+    // sequence is hardly ever there.)
+    while (nsplit < kFewSplit && 2 * nsplit * p.seqs.S * static_cast<int64_t>(p.Hkv) <= C::kCtas * sms) nsplit *= 2;
     if (units * nsplit > 0x7fffffff) return VQ_EUNSUPPORTED;
     constexpr bool f16 = !IsBf16<T>::value;
     CUtensorMap k1, k3, v, cb, vs;
@@ -691,7 +745,7 @@ static int launch_few(const PagedAttnParams &p, cudaStream_t stream)
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(units * nsplit));
-    cfg.blockDim = dim3(kFewThreads);
+    cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kTotal;
     cfg.stream = stream;
     cfg.attrs = attr;

@@ -53,6 +53,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity)
         : "memory");
     return ok != 0;
 }
+// One poll that does not suspend the thread.
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // Bounded wait: polls for `limit` cycles of SM clock (default: about two seconds), then reports failure.
 constexpr long long kDefaultWaitCycles = 4000000000LL;
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, long long limit = kDefaultWaitCycles)

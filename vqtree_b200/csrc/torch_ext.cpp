@@ -9,12 +9,15 @@
 // Reference interfaces behind the operators: ops/mini_vq.py:4-18 (assign_codes), ops/attn_vq.py:352-384,
 // 411-417 (build_aggregates), ops/triton_fused_vq_attn.py:190-251 (prefill), README.md:8 and
 // ops/attn_vq.py:128-165 (decode, cache_advance).
+#include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
 #include <optional>
+#include <tuple>
 #include <utility>
+#include <vector>
 
 #include "vqattn.h"
 
@@ -191,7 +194,8 @@ void cache_advance(const at::Tensor &codes, const at::Tensor &v_new, int64_t K, 
           "vqattn::cache_advance");
 }
 
-// ---- the paged cache.  The *_status forms return the C status (what vqtree_b200/api.py turns into its own exception); the others raise.
+// ---- the paged cache.  The plain forms write into their arguments and raise; the *_status forms return the C status instead (what
+// vqtree_b200/api.py turns into its own exception), and the *_new forms allocate the outputs too (three times as fast here as from Python).
 
 VqTensorDesc any_desc(const at::Tensor &t)         // host tensors too: the C function answers VQ_EDEVICE for them
 {
@@ -286,6 +290,49 @@ int64_t paged_attention_status(const at::Tensor &q1, const at::Tensor &q2, const
     return vqattn_paged_attention(&a, stream_of(q1));
 }
 
+std::tuple<at::Tensor, at::Tensor, int64_t> paged_append_new(const at::Tensor &k, const at::Tensor &v, at::Tensor k1, at::Tensor v_pages,
+                                                             const OptTensor &k3, const OptTensor &k1_scale, const OptTensor &v_scale,
+                                                             const OptTensor &k3_scale, const at::Tensor &table, const at::Tensor &cu_q,
+                                                             const at::Tensor &lens, const at::Tensor &q, bool two, const OptTensor &cos_tab,
+                                                             const OptTensor &sin_tab, int64_t const_pos, const OptTensor &status_word)
+{
+    const at::Tensor q1 = at::empty(q.sizes(), q.options()), q2 = two ? at::empty(q.sizes(), q.options()) : q1;
+    const int64_t status = paged_append_status(k, v, std::move(k1), std::move(v_pages), k3, k1_scale, v_scale, k3_scale, table, cu_q, lens, q, q1,
+                                               two ? OptTensor(q2) : OptTensor(), cos_tab, sin_tab, const_pos, status_word);
+    return {q1, two ? q2 : at::Tensor(at::empty({0}, q.options())), status};
+}
+
+std::tuple<std::vector<at::Tensor>, int64_t> paged_read_new(at::TensorList pools, const c10::List<OptTensor> &scales, const at::Tensor &table,
+                                                            const at::Tensor &start, const at::Tensor &lens, int64_t n, at::ScalarType dtype,
+                                                            const OptTensor &status_word)
+{
+    TORCH_CHECK(!pools.empty() && pools.size() <= 3 && pools.size() == scales.size(), "vqattn: one to three pools, a scale or none for each");
+    TORCH_CHECK(pools[0].dim() == 4 && table.dim() == 2, "vqattn: pools [NP,Hkv,P,D], table [S,MB]");
+    std::vector<at::Tensor> outs;
+    OptTensor pool[3], scale[3], out[3];
+    for (size_t i = 0; i < pools.size(); ++i) {
+        outs.push_back(at::empty({table.size(0), pools[0].size(1), n, pools[0].size(3)}, pools[0].options().dtype(dtype)));
+        pool[i] = pools[i];
+        scale[i] = scales.get(i);
+        out[i] = outs.back();
+    }
+    const int64_t status = paged_read_status(pools[0], scale[0], outs[0], pool[1], scale[1], out[1], pool[2], scale[2], out[2], table, start, lens,
+                                             status_word);
+    return {outs, status};
+}
+
+std::tuple<at::Tensor, int64_t> paged_attention_new(const at::Tensor &q1, const at::Tensor &q2, const at::Tensor &k1, const at::Tensor &v_pages,
+                                                    const OptTensor &k3, const OptTensor &k1_scale, const OptTensor &v_scale,
+                                                    const OptTensor &k3_scale, const at::Tensor &table, const at::Tensor &cu_q,
+                                                    const at::Tensor &lens, const OptTensor &codebook, const OptTensor &cnt, const OptTensor &vsum,
+                                                    const OptTensor &snap_table, int64_t window, int64_t max_q, double scale,
+                                                    const OptTensor &status_word)
+{
+    const at::Tensor out = at::empty(q1.sizes(), q1.options());
+    return {out, paged_attention_status(q1, q2, k1, v_pages, k3, k1_scale, v_scale, k3_scale, table, cu_q, lens, codebook, cnt, vsum, snap_table, window,
+                                        max_q, scale, out, status_word)};
+}
+
 // the raising forms
 template <auto F> struct Raising;
 template <typename... A, int64_t (*F)(A...)> struct Raising<F> {
@@ -327,6 +374,14 @@ TORCH_LIBRARY(vqattn, m)
     m.def("paged_attention_status(Tensor q1, Tensor q2, Tensor k1, Tensor v_pages, Tensor? k3, Tensor? k1_scale, Tensor? v_scale, Tensor? k3_scale, Tensor table, "
           "Tensor cu_q, Tensor lens, Tensor? codebook, Tensor? cnt, Tensor? vsum, Tensor? snap_table, int window, int max_q, float scale, "
           "Tensor(a!) out, Tensor(b!)? status_word) -> int");
+    m.def("paged_append_new(Tensor k, Tensor v, Tensor(a!) k1, Tensor(b!) v_pages, Tensor(c!)? k3, Tensor(d!)? k1_scale, Tensor(e!)? v_scale, "
+          "Tensor(f!)? k3_scale, Tensor table, Tensor cu_q, Tensor lens, Tensor q, bool two, Tensor? cos_tab, Tensor? sin_tab, int const_pos, "
+          "Tensor(g!)? status_word) -> (Tensor, Tensor, int)");
+    m.def("paged_read_new(Tensor[] pools, Tensor?[] scales, Tensor table, Tensor start, Tensor lens, int n, ScalarType dtype, "
+          "Tensor(a!)? status_word) -> (Tensor[], int)");
+    m.def("paged_attention_new(Tensor q1, Tensor q2, Tensor k1, Tensor v_pages, Tensor? k3, Tensor? k1_scale, Tensor? v_scale, Tensor? k3_scale, "
+          "Tensor table, Tensor cu_q, Tensor lens, Tensor? codebook, Tensor? cnt, Tensor? vsum, Tensor? snap_table, int window, int max_q, "
+          "float scale, Tensor(a!)? status_word) -> (Tensor, int)");
 }
 
 TORCH_LIBRARY_IMPL(vqattn, CUDA, m)
@@ -336,6 +391,9 @@ TORCH_LIBRARY_IMPL(vqattn, CUDA, m)
     m.impl("prefill", &prefill);
     m.impl("decode", &decode);
     m.impl("cache_advance", &cache_advance);
+    m.impl("paged_append_new", &paged_append_new);
+    m.impl("paged_read_new", &paged_read_new);
+    m.impl("paged_attention_new", &paged_attention_new);
     m.impl("paged_append", &Raising<&paged_append_status>::call);
     m.impl("paged_append_status", &paged_append_status);
     m.impl("paged_read", &Raising<&paged_read_status>::call);

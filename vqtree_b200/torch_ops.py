@@ -22,7 +22,7 @@ that kernels raise on an expired bounded wait or a bad code):
     paged_read(pool0, scale0?, out0!, pool1?, scale1?, out1!?, pool2?, scale2?, out2!?, table, start, lens, status_word?)
     paged_attention(q1, q2, k1, v_pages, k3?, k1_scale?, v_scale?, k3_scale?, table, cu_q, lens, codebook?, cnt?, vsum?, snap_table?,
                     window, max_q, scale, out!, status_word?)
-    paged_*_status(...): the same, returning the C status instead of raising
+    paged_*_status(...): the same, returning the C status instead of raising; paged_*_new(...): that, and the outputs allocated
     abi_version(), assign_workspace_bytes(...), aggregates_workspace_bytes(...), decode_workspace_bytes(...)
 """
 from __future__ import annotations
@@ -53,6 +53,11 @@ def load():
             torch.library.register_fake(f"vqattn::{name}")(_nothing)
         for name in _PAGED:
             torch.library.register_fake(f"vqattn::{name}_status")(_ok)
+        torch.library.register_fake("vqattn::paged_append_new")(lambda k, v, k1, vp, k3, a, b, c, t, cu, ln, q, two, *rest: (
+            q.new_empty(q.shape), q.new_empty(q.shape if two else (0,)), 0))
+        torch.library.register_fake("vqattn::paged_read_new")(lambda pools, scales, table, start, lens, n, dtype, word: (
+            [p.new_empty((table.shape[0], p.shape[1], n, p.shape[3]), dtype=dtype) for p in pools], 0))
+        torch.library.register_fake("vqattn::paged_attention_new")(lambda q1, *rest: (q1.new_empty(q1.shape), 0))
         _loaded = True
     return torch.ops.vqattn
 
@@ -66,12 +71,13 @@ def _ok(*args, **kwargs):
 
 
 def paged_calls():
-    """The status forms of the paged operators, loaded once: what ``api.paged_*`` calls (describing some fifteen tensors in C++ takes 1 us,
-    from Python 30)."""
+    """What ``api.paged_*`` calls, looked up once: paged_append_status, paged_attention_status and the three ``*_new`` forms (describing some
+    fifteen tensors in C++ takes 1 us, from Python 30)."""
     global _calls
     if _calls is None:
         ops = load()
-        _calls = tuple(getattr(ops, f"{name}_status").default for name in _PAGED)
+        _calls = tuple(getattr(ops, n).default for n in ("paged_append_status", "paged_attention_status", "paged_append_new", "paged_read_new",
+                                                         "paged_attention_new"))
     return _calls
 
 
