@@ -36,13 +36,20 @@ template <> struct Codes8<__half> {
 // A weight times a value row of codes with scale vs, in halves: weight * (vs * 2^k) and codes * 2^-k, with k such that the first factor lies in
 // [1, 2) - and inside what a half holds for every scale of half values (2^-31 .. 2^10).  Otherwise a small scale would put
 // the products among the subnormal halves, where the codes of a snapshot (weights without a scale) share the accumulator.
+// half_weight_shift: k for one scale, or for the largest of a tile.
+__device__ __forceinline__ int half_weight_shift(float vs)
+{
+    const int k = 127 - static_cast<int>((__float_as_uint(vs) >> 23) & 255u);
+    return min(24, max(-5, k));
+}
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 __device__ __forceinline__ float half_weight_factor(float vs, float &pow2)
 {
-    int k = 127 - static_cast<int>((__float_as_uint(vs) >> 23) & 255u);
-    k = min(24, max(-5, k));
-    pow2 = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-    return vs * __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+    const int k = half_weight_shift(vs);
+    pow2 = pow2f(-k);
+    return vs * pow2f(k);
 }
+
 template <> struct Codes8<__nv_bfloat16> {
     // 0x4300 | (x & 127) is the bf16 128 + (x & 127), 0x4300 | (x & 128) is 128 or 256: their difference is x
     static __device__ __forceinline__ uint32_t pair(uint32_t e)

@@ -7,10 +7,10 @@
 // tensor memory that P overwrites, one thread per row and buffer, a reference maximum handed from step to step, lazily raised.
 // Which rows a tile has is read on the device (one warp counts the tiles of 32 sequences at a time), so a captured call may be
 // replayed with other lengths.
-//   16-bit rows   a thread loads pages by TMA, 128 / P boxes a tile; three softmax warpgroups, a ring of three 32 KB slots.
-//   8-bit rows    a warpgroup fetches the codes, turns them into 16-bit floats (exact) and writes them in the swizzled layout the tensor
-//                 cores read; the scales of a step's keys multiply scores, those of its values weights, per column.  Two softmax
-//                 warpgroups, a ring of four.
+//   16-bit rows   a thread loads pages by TMA, 128 / P boxes a tile, into a ring of four 32 KB slots.
+//   8-bit rows    codes arrive by TMA in two staging tiles; three warps turn them into 16-bit floats (exact) and write them in the swizzled layout the
+//                 tensor cores read, into a ring of three slots.  The scales of a step's keys multiply scores, those of its values weights,
+//                 per column.  (Fetched by plain loads one tile ahead the loads' latency was paid per tile: 410 us where this takes @@.)
 // Rows behind a sequence's end hold anything: their scores are masked and their value rows are zeroed before the product.
 #include "codes8.cuh"
 #include "paged_attn.cuh"
@@ -22,19 +22,19 @@ constexpr int kChunkPages = 256;        // page table entries of a tile kept in 
 
 template <int D, bool Q8>
 struct ChunkCfg {
-    static constexpr int kBufs = Q8 ? 2 : 3;                  // S/P buffers = softmax warpgroups
+    static constexpr int kBufs = 3;                           // S/P buffers = softmax warpgroups
     static constexpr int kSoft = 4 * kBufs;                   // softmax warps
-    static constexpr int kLoad = Q8 ? 4 : 1;                  // loading warps
+    static constexpr int kLoad = Q8 ? 3 : 1;                  // loading warps: 16 warps of 128 registers with 8-bit rows
     static constexpr int kWarpMma = kSoft, kWarpLoad = kSoft + 1;
     static constexpr int kThreads = (kSoft + 1 + kLoad) * 32;
     static constexpr int NH = D / 64;
     static constexpr int kTile = NH * kHalfBytes;             // 128 x D
-    static constexpr int kSlots = Q8 ? 4 : 3;
-    static constexpr int kQ = 0, kRing = 2 * kTile;
-    static constexpr int kTotal = kRing + kSlots * kTile + 1024;   // + slack for 1024-byte alignment
+    static constexpr int kSlots = Q8 ? 3 : 4;
+    static constexpr int kRaw = kBlock * D;                   // 128 rows of codes
+    static constexpr int kQ = 0, kRing = 2 * kTile, kRaws = kRing + kSlots * kTile;
+    static constexpr int kTotal = kRaws + (Q8 ? 2 * kRaw : 0) + 1024;   // + slack for 1024-byte alignment
     static constexpr uint32_t kColS = 0, kColO = kBlock * kBufs, kCols = 512;
     static constexpr int kOq = D / 2;
-    static constexpr int kScal = Q8 ? 4 : 1;                  // steps whose scales are in flight
 };
 
 struct ChunkParams {
@@ -128,6 +128,25 @@ __device__ __forceinline__ void fmul2(float &d0, float &d1, float a0, float a1, 
         : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
 
+// Barrier ID of THREADS threads that tells whether the condition holds in all of them.
+template <int ID, int THREADS>
+__device__ __forceinline__ bool all_of_named(bool x)
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(static_cast<uint32_t>(x)), "n"(ID), "n"(THREADS) : "memory");
+    return r != 0;
+}
+
+// maximum of four values of every lane
+__device__ __forceinline__ float warp_max4(const float (&x)[4])
+{
+    float m = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    return m;
+}
+
 // 8-bit rows: scores of 64 columns in log2 units (ks: scale of each key times the softmax scale), excluded ones -inf
 __device__ __forceinline__ void q8_scores(uint32_t s_addr, int kind, int lo, int hi, const float *ks, uint32_t (&r)[64])
 {
@@ -186,11 +205,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
 {
     using C = ChunkCfg<D, Q8>;
     using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
-    constexpr int NH = C::NH, NS = C::kSlots, NB = C::kBufs;
+    constexpr int NH = C::NH, NS = C::kSlots, NB = C::kBufs, kSoftThreads = C::kSoft * 32;
     const PagedAttnParams &p = cp.a;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-ptx::smem_u32(smem_raw) & 1023u);   // stays an address of shared memory for the compiler
-    __shared__ __align__(8) uint64_t bar_q, kv_full[NS], kv_empty[NS], s_full[NB], p_full[NB], pv_done[NB], refbar[NB][4], endbar, sc_full[C::kScal];
+    __shared__ __align__(8) uint64_t bar_q, kv_full[NS], kv_empty[NS], s_full[NB], p_full[NB], pv_done[NB], refbar[NB][4], endbar, raw_full[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_err, s_some;
     __shared__ ChunkTile s_tile;
@@ -198,7 +217,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
     __shared__ __align__(16) float s_cw[C::kSoft][kBlock];   // [softmax warp][column]: counts of the codebook tile it works on
     __shared__ float s_ref[kBlock];
     __shared__ float s_lend[NB][kBlock], s_mend[NB][kBlock];
-    __shared__ __align__(16) float s_ks[C::kScal][Q8 ? kBlock : 4], s_vs[C::kScal][Q8 ? kBlock : 4], s_p2[C::kScal][Q8 && F16 ? kBlock : 4];
+    __shared__ __align__(16) float s_cv[Q8 ? C::kSoft : 1][Q8 ? kBlock : 4];   // 8-bit rows: factors of its weights (s_cw: of its scores)
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int hk = blockIdx.y;
@@ -213,7 +232,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
     if (tid == C::kWarpMma * 32) {
         mbar_init(&bar_q, 1);
         for (int i = 0; i < NS; ++i) {
-            mbar_init(&kv_full[i], C::kLoad);
+            mbar_init(&kv_full[i], 1);
             mbar_init(&kv_empty[i], 1);
         }
         for (int i = 0; i < NB; ++i) {
@@ -222,7 +241,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
             mbar_init(&pv_done[i], 1);
             for (int g = 0; g < 4; ++g) mbar_init(&refbar[i][g], 1);
         }
-        for (int i = 0; i < C::kScal; ++i) mbar_init(&sc_full[i], C::kLoad);
+        mbar_init(&raw_full[0], 1);
+        mbar_init(&raw_full[1], 1);
         mbar_init(&endbar, C::kSoft);
         fence_mbar_init();
         s_err = 0;
@@ -230,6 +250,25 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
     if (tid < kBlock) s_ref[tid] = -INFINITY;
     __syncthreads();
     if (!s_some) return;
+    const ChunkTile tile = s_tile;
+    const ChunkWork work(p, tile);
+    const int n = work.n_items;
+    const int n_q2 = p.rerope ? work.n_far + (work.n_bd == 2 ? 1 : 0) : work.n_far;   // items scored with q2 come first
+    const int log_p = p.seqs.log_p, col0 = max(work.kb0, 0) * kBlock >> log_p, page_size = 1 << log_p;
+    if (warp == C::kWarpMma && elect_one()) {
+        prefetch_tmap(&tm_q1); prefetch_tmap(&tm_q2); prefetch_tmap(&tm_cb); prefetch_tmap(&tm_vs);
+        mbar_expect_tx(&bar_q, (n_q2 > 0 ? 2 : 1) * NH * 128 * cp.TQ * p.G);
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+            tma_load_3d(smem + C::kQ + h * kHalfBytes, &tm_q1, &bar_q, 64 * h, hk * p.G, tile.t0);
+            if (n_q2 > 0) tma_load_3d(smem + C::kQ + C::kTile + h * kHalfBytes, &tm_q2, &bar_q, 64 * h, hk * p.G, tile.t0);
+        }
+    }
+    {
+        const int last = min(tile.n - 1, (tile.pos0 / kBlock + 1) * kBlock - 1) >> log_p;   // page of the last key that is read
+        if (tid < kSoftThreads)
+            for (int x = tid; x < min(last - col0 + 1, kChunkPages); x += kSoftThreads) s_page[x] = p.seqs.page(tile.s, col0 + x);
+    }
     if (warp == C::kWarpLoad) {
         __syncwarp();
         tmem_alloc(&s_tmem, C::kCols);
@@ -239,35 +278,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    const ChunkTile tile = s_tile;
-    const ChunkWork work(p, tile);
-    const int n = work.n_items;
-    const int n_q2 = p.rerope ? work.n_far + (work.n_bd == 2 ? 1 : 0) : work.n_far;   // items scored with q2 come first
-    const int log_p = p.seqs.log_p, col0 = max(work.kb0, 0) * kBlock >> log_p, page_size = 1 << log_p;
     auto page_of = [&](int key) {
         const int x = (key >> log_p) - col0;
         return x < kChunkPages ? s_page[x] : p.seqs.page(tile.s, x + col0);
     };
 
     if (warp >= C::kWarpLoad) {
-        // ================================================================== loads
+        // ================================================================== loads, in the order the tensor pipe consumes them: K0 K1 K2 V0 K3 V1 ...
         const int lw = warp - C::kWarpLoad;
-        const bool leader = lw == 0 && elect_one();
-        if (leader) {
-            prefetch_tmap(&tm_q1); prefetch_tmap(&tm_q2); prefetch_tmap(&tm_cb); prefetch_tmap(&tm_vs);
-            mbar_expect_tx(&bar_q, (n_q2 > 0 ? 2 : 1) * NH * 128 * cp.TQ * p.G);
-#pragma unroll
-            for (int h = 0; h < NH; ++h) {
-                tma_load_3d(smem + C::kQ + h * kHalfBytes, &tm_q1, &bar_q, 64 * h, hk * p.G, tile.t0);
-                if (n_q2 > 0) tma_load_3d(smem + C::kQ + C::kTile + h * kHalfBytes, &tm_q2, &bar_q, 64 * h, hk * p.G, tile.t0);
-            }
-        }
-        {
-            const int cols = ((tile.n - 1) >> log_p) - col0 + 1, last = ((tile.pos0 / kBlock + 1) * kBlock - 1) >> log_p;
-            for (int x = tid - C::kWarpLoad * 32; x < min(min(cols, last - col0 + 1), kChunkPages); x += C::kLoad * 32) s_page[x] = p.seqs.page(tile.s, col0 + x);
-            if (C::kLoad == 1) __syncwarp();
-            else asm volatile("bar.sync 1, %0;" ::"n"(C::kLoad * 32) : "memory");
-        }
         int slot = 0;
         uint32_t free_par = 1u;
         bool first_round = true, ok = true;
@@ -278,150 +296,170 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
                 first_round = false;
             }
         };
-        auto far_tile = [&](int it, bool is_v, int arrive_bytes) {
+        auto wait_slot = [&]() { return first_round || mbar_wait(&kv_empty[slot], free_par, p.wait_limit); };
+        auto far_tile = [&](int it, bool is_v) {
             uint8_t *dst = smem + C::kRing + slot * C::kTile;
-            mbar_expect_tx(&kv_full[slot], arrive_bytes);
+            mbar_expect_tx(&kv_full[slot], C::kTile);
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
                 if (is_v) tma_load_3d(dst + h * kHalfBytes, &tm_vs, &kv_full[slot], 64 * h, work.block(it) * kBlock, tile.snap * p.Hkv + hk);
                 else tma_load_3d(dst + h * kHalfBytes, &tm_cb, &kv_full[slot], 64 * h, work.block(it) * kBlock, hk);
             }
         };
-        if constexpr (!Q8) {
-            if (leader) {
-                auto load = [&](int it, bool is_v) {
-                    if (!ok) return;
-                    if (!first_round && !mbar_wait(&kv_empty[slot], free_par, p.wait_limit)) {
-                        ok = false;
-                        return;
-                    }
-                    const int kind = work.kind(it);
-                    if (kind == kFar) {
-                        far_tile(it, is_v, C::kTile);
-                    } else {
-                        const CUtensorMap *tm = is_v ? &tm_v : (kind == kBdA ? &tm_k3 : &tm_k1);
-                        uint8_t *dst = smem + C::kRing + slot * C::kTile;
-                        const int key0 = work.block(it) * kBlock, end = min(tile.n, key0 + kBlock);
-                        int bytes = 0;                        // pages behind the end, or missing ones (reported), are not loaded
-                        for (int key = key0; key < end; key += page_size)
-                            if (page_of(key) >= 0) bytes += page_size * D * 2;
-                        mbar_expect_tx(&kv_full[slot], bytes);
-                        for (int key = key0; key < end; key += page_size) {
-                            const int page = page_of(key);
-                            if (page < 0) continue;
-#pragma unroll
-                            for (int h = 0; h < NH; ++h)
-                                tma_load_4d(dst + h * kHalfBytes + (key - key0) * 128, tm, &kv_full[slot], 64 * h, 0, hk, page);
-                        }
-                    }
-                    advance();
-                };
-                for (int j = 0; j < NB && j < n; ++j) load(j, false);
-                for (int j = 0; j < n; ++j) {
-                    load(j, true);
-                    if (j + NB < n) load(j + NB, false);
-                }
-                if (!ok) s_err = 1;
+        // Lane x has page x of an item's block; -1 for missing ones (reported) and those behind the end, which are not loaded.
+        auto page_of_lane = [&](int it) {
+            const int key = work.block(it) * kBlock + lane * page_size;
+            return lane * page_size < kBlock && key < tile.n ? page_of(key) : -1;
+        };
+        // their boxes, by one elected thread: put(page, number of the page in the block)
+        auto each_page = [&](int mine, auto put) {
+            for (unsigned left = __ballot_sync(~0u, mine >= 0); left; left &= left - 1) {
+                const int x = __ffs(left) - 1, pg = __shfl_sync(~0u, mine, x);
+                if (elect_one()) put(pg, x);
+                __syncwarp();
             }
-        } else {
-            // Codes of the next tile are fetched into registers while this one is converted.  CH lanes share a row, 16 codes each.
-            constexpr int CH = D / 16, RPI = 32 / CH, NL = 32 / RPI;       // rows per instruction, loads per thread and tile
-            const int ch = lane % CH, rsub = lane / CH;
-            const int total = 2 * n;
-            uint4 codes[NL];
-            float scale_k = 0.f, scale_v = 0.f;
-            // load number -> item, kind of tile (order K0 K1 V0 K2 V1 ... as the tensor pipe consumes them)
-            auto item_of = [&](int x, bool &is_v) {
-                if (x < NB || n <= NB) {
-                    if (x < min(NB, n)) {
-                        is_v = false;
-                        return x;
-                    }
-                    is_v = true;
-                    return x - n;
-                }
-                const int y = x - NB;                                      // V0 K(NB) V1 K(NB+1) ... until the keys run out
-                if (y < 2 * (n - NB)) {
-                    is_v = (y & 1) == 0;
-                    return is_v ? y / 2 : NB + y / 2;
-                }
-                is_v = true;
-                return y - (n - NB);
-            };
-            auto fetch = [&](int x) {
-                bool is_v;
-                const int it = item_of(x, is_v), kind = work.kind(it);
-                if (kind == kFar) return;
-                const int key0 = work.block(it) * kBlock + 32 * lw;
-                const PagedPool &pool = is_v ? p.v : (kind == kBdA ? p.k3 : p.k1);
-                const int8_t *base = static_cast<const int8_t *>(pool.ptr);
-#pragma unroll
-                for (int i = 0; i < NL; ++i) {
-                    const int key = key0 + RPI * i + rsub;
-                    codes[i] = make_uint4(0, 0, 0, 0);
-                    if (key < tile.n) {
-                        const int page = page_of(key);
-                        if (page >= 0) codes[i] = *reinterpret_cast<const uint4 *>(base + pool.row(page, hk, key & (page_size - 1)) + 16 * ch);
-                    }
-                }
-                if (!is_v) {
-                    const int key = key0 + lane, page = key < tile.n ? page_of(key) : -1, r = key & (page_size - 1);
-                    scale_k = page >= 0 ? __ldg(pool.scale + pool.scale_at(page, hk, r)) : 0.f;
-                    scale_v = page >= 0 ? __ldg(p.v.scale + p.v.scale_at(page, hk, r)) : 0.f;
-                }
-            };
-            fetch(0);
-            for (int x = 0; x < total; ++x) {
-                bool is_v;
-                const int it = item_of(x, is_v), kind = work.kind(it);
-                if (!first_round && !mbar_wait(&kv_empty[slot], free_par, p.wait_limit)) ok = false;
-                if (!__all_sync(~0u, ok)) {
+        };
+        if constexpr (!Q8) {
+            auto load = [&](int it, bool is_v) {
+                if (!ok) return;
+                const int kind = work.kind(it), mine = kind == kFar ? -1 : page_of_lane(it);   // known before the slot is free
+                const int bytes = __popc(__ballot_sync(~0u, mine >= 0)) * page_size * D * 2;
+                if (!__all_sync(~0u, wait_slot())) {
                     ok = false;
-                    break;
+                    return;
                 }
                 if (kind == kFar) {
-                    if (leader) far_tile(it, is_v, C::kTile);
-                    else if (lw != 0 && lane == 0) mbar_arrive(&kv_full[slot]);
-                    if (!is_v && lane == 0) mbar_arrive(&sc_full[it % C::kScal]);   // keeps the phases of sc_full in step with the items
-                    if (x + 1 < total) fetch(x + 1);
-                } else {
-                    if (!is_v) {
-                        const int b = it % C::kScal, col = 32 * lw + lane;
-                        s_ks[b][col] = scale_k * p.scale_log2;
-                        if constexpr (F16) s_vs[b][col] = half_weight_factor(scale_v, s_p2[b][col]);
-                        else s_vs[b][col] = scale_v;
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&sc_full[b]);
-                    }
-                    uint8_t *dst = smem + C::kRing + slot * C::kTile + (ch >> 2) * kHalfBytes;
-                    const int flip = D == 128 ? ch >> 2 : 0;                  // the two halves of a row take turns: no bank is asked for twice
-#pragma unroll
-                    for (int i = 0; i < NL; ++i) {
-                        const int row = 32 * lw + RPI * i + rsub;
-                        uint4 a, b;
-                        if (F16 && is_v) {
-                            if constexpr (F16) {
-                                const __half2 p2 = __float2half2_rn(s_p2[it % C::kScal][row]);
-                                Codes8<T>::expand_scaled(codes[i].x, p2, a.x, a.y);
-                                Codes8<T>::expand_scaled(codes[i].y, p2, a.z, a.w);
-                                Codes8<T>::expand_scaled(codes[i].z, p2, b.x, b.y);
-                                Codes8<T>::expand_scaled(codes[i].w, p2, b.z, b.w);
-                            }
-                        } else {
-                            Codes8<T>::expand(codes[i].x, a.x, a.y);
-                            Codes8<T>::expand(codes[i].y, a.z, a.w);
-                            Codes8<T>::expand(codes[i].z, b.x, b.y);
-                            Codes8<T>::expand(codes[i].w, b.z, b.w);
-                        }
-                        uint8_t *line = dst + row * 128;
-                        const int c0 = (2 * (ch & 3)) ^ (row & 7);            // 128-byte swizzle: 16-byte piece j of row r lies at j ^ (r % 8)
-                        *reinterpret_cast<uint4 *>(line + 16 * (c0 ^ flip)) = flip ? b : a;
-                        *reinterpret_cast<uint4 *>(line + 16 * (c0 ^ flip ^ 1)) = flip ? a : b;
-                    }
-                    if (x + 1 < total) fetch(x + 1);
-                    fence_proxy_async_smem();
+                    if (elect_one()) far_tile(it, is_v);
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&kv_full[slot]);
+                } else {
+                    const CUtensorMap *tm = is_v ? &tm_v : (kind == kBdA ? &tm_k3 : &tm_k1);
+                    uint8_t *dst = smem + C::kRing + slot * C::kTile;
+                    if (elect_one()) mbar_expect_tx(&kv_full[slot], bytes);
+                    __syncwarp();
+                    each_page(mine, [&](int pg, int x) {
+#pragma unroll
+                        for (int h = 0; h < NH; ++h)
+                            tma_load_4d(dst + h * kHalfBytes + x * page_size * 128, tm, &kv_full[slot], 64 * h, 0, hk, pg);
+                    });
+                }
+                advance();
+            };
+            for (int j = 0; j < NB && j < n; ++j) load(j, false);
+            for (int j = 0; j < n; ++j) {
+                load(j, true);
+                if (j + NB < n) load(j + NB, false);
+            }
+            if (!ok) s_err = 1;
+        } else {
+            // CH lanes share a row, 8 codes each: what eight of them write together lies in different banks.  A warp takes every third block of
+            // eight rows.
+            constexpr int CH = D / 8, RPI = 32 / CH, NI = 8 / RPI;
+            const int ch = lane % CH, rsub = lane / CH;
+            uint32_t from[NI], to[NI];                                     // offsets inside a block of eight rows, staged and swizzled
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int r = RPI * i + rsub;
+                from[i] = r * D + 8 * ch;
+                to[i] = (ch >> 3) * kHalfBytes + r * 128 + (((ch & 7) ^ r) << 4);   // 16-byte piece j of row r lies at j ^ (r % 8)
+            }
+            // load number -> item and kind of tile
+            auto item_of = [&](int x, bool &is_v) {
+                const int lead = min(NB, n);
+                is_v = false;
+                if (x < lead) return x;
+                const int y = x - lead;                                    // V0 K(NB) V1 K(NB+1) ... until the keys run out
+                if (y < 2 * (n - lead)) {
+                    is_v = (y & 1) == 0;
+                    return is_v ? y / 2 : lead + y / 2;
+                }
+                is_v = true;
+                return y - (n - lead);
+            };
+            // the next local load that has not been asked for yet, into staging tile `next_raw % 2` (the first loading warp)
+            int ask = 0, next_raw = 0;
+            auto stage = [&]() {
+                bool is_v = false;
+                int it = 0;
+                for (; ask < 2 * n; ++ask) {
+                    it = item_of(ask, is_v);
+                    if (work.kind(it) != kFar) break;
+                }
+                if (ask == 2 * n) return;
+                const int mine = page_of_lane(it), bytes = __popc(__ballot_sync(~0u, mine >= 0)) * page_size * D;
+                const CUtensorMap *tm = is_v ? &tm_v : (work.kind(it) == kBdA ? &tm_k3 : &tm_k1);
+                uint64_t *bar = &raw_full[next_raw & 1];
+                uint8_t *dst = smem + C::kRaws + (next_raw & 1) * C::kRaw;
+                if (elect_one()) mbar_expect_tx(bar, bytes);
+                __syncwarp();
+                each_page(mine, [&](int pg, int x) { tma_load_4d(dst + x * page_size * D, tm, bar, 0, 0, hk, pg); });
+                ++ask;
+                ++next_raw;
+            };
+            if (lw == 0) {
+                stage();
+                stage();
+            }
+            // Half values: their codes are multiplied by a power of two that goes with the tile's largest scale (the softmax warps put its inverse
+            // into the weights).  The scales are asked for one tile ahead, four rows per lane.
+            float vsc[4];
+            auto value_scales = [&](int x) {
+                if constexpr (F16) {
+                    bool is_v;
+                    if (x >= 2 * n) return;
+                    const int it = item_of(x, is_v);
+                    if (!is_v || work.kind(it) == kFar) return;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = work.block(it) * kBlock + 32 * i + lane, pg = key < tile.n ? page_of(key) : -1;
+                        vsc[i] = pg >= 0 ? __ldg(p.v.scale + p.v.scale_at(pg, hk, key & (page_size - 1))) : 0.f;
+                    }
+                }
+            };
+            int raw = 0;
+            value_scales(0);
+            for (int x = 0; x < 2 * n; ++x) {
+                bool is_v;
+                const int it = item_of(x, is_v);
+                const bool far = work.kind(it) == kFar;
+                ok = wait_slot() && (far || mbar_wait(&raw_full[raw & 1], (raw >> 1) & 1, p.wait_limit));
+                ok = all_of_named<2, C::kLoad * 32>(ok);                   // the loading warps leave together or not at all
+                if (!ok) break;
+                if (far) {
+                    if (lw == 0 && elect_one()) far_tile(it, is_v);
+                    __syncwarp();
+                    value_scales(x + 1);
+                } else {
+                    const uint8_t *src = smem + C::kRaws + (raw & 1) * C::kRaw;
+                    uint8_t *dst = smem + C::kRing + slot * C::kTile;
+                    __half2 p2;
+                    if constexpr (F16) p2 = __float2half2_rn(is_v ? pow2f(-half_weight_shift(warp_max4(vsc))) : 1.f);
+#pragma unroll 1
+                    for (int blk = lw; blk < kBlock / 8; blk += C::kLoad) {
+                        uint2 codes[NI];
+#pragma unroll
+                        for (int i = 0; i < NI; ++i) codes[i] = *reinterpret_cast<const uint2 *>(src + blk * (8 * D) + from[i]);
+#pragma unroll
+                        for (int i = 0; i < NI; ++i) {
+                            uint4 w;
+                            if constexpr (F16) {
+                                Codes8<T>::expand_scaled(codes[i].x, p2, w.x, w.y);
+                                Codes8<T>::expand_scaled(codes[i].y, p2, w.z, w.w);
+                            } else {
+                                Codes8<T>::expand(codes[i].x, w.x, w.y);
+                                Codes8<T>::expand(codes[i].y, w.z, w.w);
+                            }
+                            *reinterpret_cast<uint4 *>(dst + blk * 1024 + to[i]) = w;
+                        }
+                    }
+                    value_scales(x + 1);
+                    fence_proxy_async_smem();
+                    asm volatile("bar.sync 1, %0;" ::"n"(C::kLoad * 32) : "memory");   // staging tile read, slot written
+                    if (lw == 0) {
+                        if (elect_one()) mbar_arrive(&kv_full[slot]);
+                        __syncwarp();
+                        stage();
+                    }
+                    ++raw;
                 }
                 advance();
             }
@@ -510,37 +548,54 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
         bool ok = true;
         constexpr int NCW = kBlock / 32;
         const float *cnt_base = p.cnt + (static_cast<int64_t>(max(tile.snap, 0)) * p.Hkv + hk) * p.MK + lane;
-        float *cw = &s_cw[warp][0];
-        float cnt_reg[NCW];
+        float *cw = &s_cw[warp][0], *cv = &s_cv[Q8 ? warp : 0][0];
+        // Lane l fetches what goes with columns l, 32 + l, ... of one of the warp's steps ahead: counts of codes; scales of 8-bit keys and values.
+        float reg_w[NCW], reg_v[Q8 ? NCW : 1];
+        auto ahead = [&](int it) {
+            if (it < work.n_far) {
 #pragma unroll
-        for (int i = 0; i < NCW; ++i) cnt_reg[i] = g < work.n_far ? __ldg(cnt_base + g * kBlock + 32 * i) : 0.f;
+                for (int i = 0; i < NCW; ++i) reg_w[i] = __ldg(cnt_base + it * kBlock + 32 * i);
+            } else if constexpr (Q8) {
+                if (it >= n) return;
+                const bool old = work.kind(it) == kBdA;
+                const float *ks = old ? p.k3.scale : p.k1.scale;
+                const int64_t c_page = old ? p.k3.c_page : p.k1.c_page, c_head = old ? p.k3.c_head : p.k1.c_head, c_row = old ? p.k3.c_row : p.k1.c_row;
+#pragma unroll
+                for (int i = 0; i < NCW; ++i) {
+                    const int key = work.block(it) * kBlock + 32 * i + lane, pg = key < tile.n ? page_of(key) : -1, r = key & (page_size - 1);
+                    reg_w[i] = pg >= 0 ? __ldg(ks + pg * c_page + hk * c_head + r * c_row) : 0.f;
+                    reg_v[i] = pg >= 0 ? __ldg(p.v.scale + p.v.scale_at(pg, hk, r)) : 0.f;
+                }
+            }
+        };
+        ahead(g);
 #pragma unroll 1
         for (int it = g; it < n; it += NB) {
             const int par = (it / NB) & 1;
             const int kind = work.kind(it);
             const bool q8 = Q8 && kind != kFar;
-            const int sb = it % C::kScal;
             bool has_empty = false;
-            if (kind == kFar) {
+            if (kind == kFar || q8) {
                 __syncwarp();
                 bool full = true;
+                float mul = 1.f;                              // half weights: see half_weight_shift
+                if constexpr (Q8 && F16)
+                    if (kind != kFar) mul = pow2f(half_weight_shift(warp_max4(reg_v)));
 #pragma unroll
                 for (int i = 0; i < NCW; ++i) {
-                    cw[32 * i + lane] = cnt_reg[i];
-                    full = full && cnt_reg[i] > 0.f;
+                    if (kind == kFar) {
+                        cw[32 * i + lane] = reg_w[i];
+                        full = full && reg_w[i] > 0.f;
+                    } else if constexpr (Q8) {
+                        cw[32 * i + lane] = reg_w[i] * p.scale_log2;
+                        cv[32 * i + lane] = F16 ? reg_v[i] * mul : reg_v[i];
+                    }
                 }
-                has_empty = __any_sync(kAll, !full);
+                has_empty = kind == kFar && __any_sync(kAll, !full);
                 __syncwarp();
-                if (it + NB < work.n_far) {
-#pragma unroll
-                    for (int i = 0; i < NCW; ++i) cnt_reg[i] = __ldg(cnt_base + (it + NB) * kBlock + 32 * i);
-                }
+                ahead(it + NB);
             }
             const int lo = kind == kBdB ? rpos : 0, hi = kind == kDiag ? rpos + 1 : kind == kBdA ? rpos : kBlock;
-            if (q8 && !__all_sync(kAll, mbar_wait(&sc_full[sb], (it / C::kScal) & 1, p.wait_limit))) {
-                ok = false;
-                break;
-            }
             if (!__all_sync(kAll, mbar_wait(&s_full[g], par, p.wait_limit))) {
                 ok = false;
                 break;
@@ -551,7 +606,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
 #pragma unroll
             for (int c = 0; c < kBlock; c += 64) {
                 if (Q8 && q8) {
-                    q8_scores(sa + c, kind, lo - c, hi - c, &s_ks[sb][c], r);
+                    q8_scores(sa + c, kind, lo - c, hi - c, cw + c, r);
                     mx = fmaxf(mx, t4_max(r));
                 } else {
                     t4_scores(sa + c, kind, has_empty, lo - c, hi - c, cw + c, r);
@@ -596,8 +651,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
 #pragma unroll
             for (int c = 0; c < kBlock; c += 64) {
                 if (Q8 && q8) {
-                    q8_scores(sa + c, kind, lo - c, hi - c, &s_ks[sb][c], r);
-                    ls = q8_exp<F16>(r, sa + c / 2, kind != kFull, &s_vs[sb][c], -m_safe, ls);
+                    q8_scores(sa + c, kind, lo - c, hi - c, cw + c, r);
+                    ls = q8_exp<F16>(r, sa + c / 2, kind != kFull, cv + c, -m_safe, ls);
                 } else {
                     t4_scores(sa + c, kind, has_empty, lo - c, hi - c, cw + c, r);
                     ls = kind == kFar ? t4_exp<true, F16>(r, sa + c / 2, cw + c, p.scale_log2, -m_safe, ls)
@@ -707,18 +762,20 @@ static bool map_tokens(CUtensorMap *out, const void *ptr, int64_t T, const Paged
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// pool [NP, Hkv, P, D] in boxes of 64 columns x one page
+// pool [NP, Hkv, P, D] in boxes of one page: 64 columns of 16 bits, swizzled, or whole rows of 8 bits as they are
+template <bool Q8>
 static bool map_pool(CUtensorMap *out, const PagedPool &pool, const PagedAttnParams &p, bool f16)
 {
     EncodeTiledFn fn = encode_fn();
     if (fn == nullptr) return false;
-    const int P = 1 << p.seqs.log_p;
+    const int P = 1 << p.seqs.log_p, e = Q8 ? 1 : 2;
     const cuuint64_t dim[4] = {static_cast<cuuint64_t>(p.D), static_cast<cuuint64_t>(P), static_cast<cuuint64_t>(p.Hkv), static_cast<cuuint64_t>(p.seqs.NP)};
-    const cuuint64_t str[3] = {static_cast<cuuint64_t>(pool.s_row * 2), static_cast<cuuint64_t>(p.Hkv > 1 ? pool.s_head * 2 : pool.s_row * 2),
-                               static_cast<cuuint64_t>(p.seqs.NP > 1 ? pool.s_page * 2 : pool.s_row * 2)};
-    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(P), 1, 1}, es[4] = {1, 1, 1, 1};
-    return fn(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(pool.ptr), dim, str, box, es,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t str[3] = {static_cast<cuuint64_t>(pool.s_row * e), static_cast<cuuint64_t>((p.Hkv > 1 ? pool.s_head : pool.s_row) * e),
+                               static_cast<cuuint64_t>((p.seqs.NP > 1 ? pool.s_page : pool.s_row) * e)};
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(Q8 ? p.D : 64), static_cast<cuuint32_t>(P), 1, 1}, es[4] = {1, 1, 1, 1};
+    return fn(out, Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+              const_cast<void *>(pool.ptr), dim, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, Q8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int D, bool F16, bool Q8>
@@ -730,11 +787,7 @@ static int launch_chunk(const PagedAttnParams &a, cudaStream_t stream)
     cp.TQ = kBlock / a.G;
     TcMaps m;
     if (!map_tokens(&m.q1, a.q1, a.seqs.T, a, a.q1_t, a.q1_h, cp.TQ, F16) || !map_tokens(&m.q2, a.q2, a.seqs.T, a, a.q2_t, a.q2_h, cp.TQ, F16)) return VQ_ELAUNCH;
-    if (Q8) {
-        m.k1 = m.k3 = m.v = m.q1;   // not used: codes are fetched by plain loads
-    } else if (!map_pool(&m.k1, a.k1, a, F16) || !map_pool(&m.k3, a.k3, a, F16) || !map_pool(&m.v, a.v, a, F16)) {
-        return VQ_ELAUNCH;
-    }
+    if (!map_pool<Q8>(&m.k1, a.k1, a, F16) || !map_pool<Q8>(&m.k3, a.k3, a, F16) || !map_pool<Q8>(&m.v, a.v, a, F16)) return VQ_ELAUNCH;
     if (a.cb != nullptr) {
         const uint64_t MK = a.MK, cd[3] = {D, MK, static_cast<uint64_t>(a.Hkv)}, cs[3] = {1, D, MK * D}, vd[3] = {D, MK, static_cast<uint64_t>(a.NS) * a.Hkv};
         if (!make_map(&m.cb, a.cb, 3, cd, cs, kBlock, F16) || !make_map(&m.vs, a.vsum, 3, vd, cs, kBlock, F16)) return VQ_ELAUNCH;
