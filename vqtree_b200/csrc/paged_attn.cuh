@@ -40,8 +40,69 @@ struct PagedAttnParams {
     }
 };
 
+// Tokens [pos0, pos0 + ntok) of sequence s (of length n), rows t0 .. of the packed tensors: all in one 128-block of positions, so that they share a
+// boundary and its snapshot.
+struct ChunkTile {
+    int s, t0, ntok, pos0, n, snap;
+};
+
+// Tile number -> sequence and tokens, by one warp.  False: there are fewer tiles.
+__device__ __forceinline__ bool chunk_find(const PagedAttnParams &p, int TQ, int tile, ChunkTile &out)
+{
+    const int lane = threadIdx.x & 31, per = (kBlock + TQ - 1) / TQ;
+    int before = 0;
+    for (int base = 0; base < p.seqs.S; base += 32) {
+        int t0 = 0, q = 0, n = 0, cnt = 0;
+        if (base + lane < p.seqs.S && p.seqs.seq(base + lane, t0, q, n, p.max_q) && q > 0) {
+            const int i0 = n - q, nb = (n - 1) / kBlock - i0 / kBlock + 1;
+            cnt = nb == 1 ? (q + TQ - 1) / TQ
+                          : (kBlock - i0 % kBlock + TQ - 1) / TQ + (nb - 2) * per + ((n - 1) % kBlock + TQ) / TQ;
+        }
+        int sum = cnt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(~0u, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned mine = __ballot_sync(~0u, before + sum > tile);
+        if (mine) {
+            const int l = __ffs(mine) - 1;
+            int x = tile - before - (__shfl_sync(~0u, sum, l) - __shfl_sync(~0u, cnt, l));   // tile of the sequence
+            t0 = __shfl_sync(~0u, t0, l);
+            q = __shfl_sync(~0u, q, l);
+            n = __shfl_sync(~0u, n, l);
+            int i0 = n - q;
+            const int head = (min(kBlock - i0 % kBlock, q) + TQ - 1) / TQ;                   // tiles of its first block
+            int blk = i0 / kBlock;
+            if (x >= head) {
+                x -= head;
+                blk += 1 + x / per;
+                x %= per;
+            }
+            const int lo = max(i0, blk * kBlock) + x * TQ, hi = min(min(n, (blk + 1) * kBlock), lo + TQ);
+            out.s = base + l;
+            out.t0 = t0 + lo - i0;
+            out.ntok = hi - lo;
+            out.pos0 = lo;
+            out.n = n;
+            out.snap = p.snapshot(out.s, p.boundary(lo));
+            return true;
+        }
+        before += __shfl_sync(~0u, sum, 31);
+    }
+    return false;
+}
+
+// An upper bound of the number of tiles, known without the lengths: every block that a sequence touches rounds its tokens up.
+inline int64_t chunk_tiles(const PagedSeqs &q, int TQ)
+{
+    const int64_t tiles = q.T / TQ + q.T / kBlock + 2 * static_cast<int64_t>(q.S);
+    return tiles < q.T ? tiles : q.T;
+}
+
 constexpr int kFewRows = 32;     // query rows (tokens times query heads of a kv head) of the few-token kernel
 int launch_paged_few(const PagedAttnParams &p, int dtype, bool q8, cudaStream_t stream);
+int launch_paged_f32(const PagedAttnParams &p, bool q8, cudaStream_t stream);
 int launch_paged_chunk(const PagedAttnParams &p, int dtype, bool q8, cudaStream_t stream);
 
 }  // namespace vq

@@ -10,7 +10,8 @@
 //   16-bit rows   a thread loads pages by TMA, 128 / P boxes a tile, into a ring of four 32 KB slots.
 //   8-bit rows    codes arrive by TMA in two staging tiles; three warps turn them into 16-bit floats (exact) and write them in the swizzled layout the
 //                 tensor cores read, into a ring of three slots.  The scales of a step's keys multiply scores, those of its values weights,
-//                 per column.  (Fetched by plain loads one tile ahead the loads' latency was paid per tile: 410 us where this takes @@.)
+//                 per column.  (Codes fetched by plain loads, one tile ahead, paid their latency per tile: six second turns of 70 to 483 tokens,
+//                 32 query heads over 8, MK1024, W1024: 410 us, now 283.)
 // Rows behind a sequence's end hold anything: their scores are masked and their value rows are zeroed before the product.
 #include "codes8.cuh"
 #include "paged_attn.cuh"
@@ -42,10 +43,6 @@ struct ChunkParams {
     int TQ;                      // tokens per tile
 };
 
-struct ChunkTile {
-    int s, t0, ntok, pos0, n, snap;
-};
-
 // The tile's items, in order: codebook tiles, boundary block (ReRoPE: two masked passes), blocks between, causal block.
 struct ChunkWork {
     int kb0, n_far, n_bd, first_full, n_full, n_items, rerope;
@@ -74,53 +71,6 @@ struct ChunkWork {
         return it < n_bd ? kb0 : first_full + it - n_bd;
     }
 };
-
-// Tile number -> sequence and tokens, by one warp.  False: there are fewer tiles.
-__device__ __forceinline__ bool chunk_find(const PagedAttnParams &p, int TQ, int tile, ChunkTile &out)
-{
-    const int lane = threadIdx.x & 31, per = (kBlock + TQ - 1) / TQ;
-    int before = 0;
-    for (int base = 0; base < p.seqs.S; base += 32) {
-        int t0 = 0, q = 0, n = 0, cnt = 0;
-        if (base + lane < p.seqs.S && p.seqs.seq(base + lane, t0, q, n, p.max_q) && q > 0) {
-            const int i0 = n - q, nb = (n - 1) / kBlock - i0 / kBlock + 1;
-            cnt = nb == 1 ? (q + TQ - 1) / TQ
-                          : (kBlock - i0 % kBlock + TQ - 1) / TQ + (nb - 2) * per + ((n - 1) % kBlock + TQ) / TQ;
-        }
-        int sum = cnt;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(~0u, sum, o);
-            if (lane >= o) sum += x;
-        }
-        const unsigned mine = __ballot_sync(~0u, before + sum > tile);
-        if (mine) {
-            const int l = __ffs(mine) - 1;
-            int x = tile - before - (__shfl_sync(~0u, sum, l) - __shfl_sync(~0u, cnt, l));   // tile of the sequence
-            t0 = __shfl_sync(~0u, t0, l);
-            q = __shfl_sync(~0u, q, l);
-            n = __shfl_sync(~0u, n, l);
-            int i0 = n - q;
-            const int head = (min(kBlock - i0 % kBlock, q) + TQ - 1) / TQ;                   // tiles of its first block
-            int blk = i0 / kBlock;
-            if (x >= head) {
-                x -= head;
-                blk += 1 + x / per;
-                x %= per;
-            }
-            const int lo = max(i0, blk * kBlock) + x * TQ, hi = min(min(n, (blk + 1) * kBlock), lo + TQ);
-            out.s = base + l;
-            out.t0 = t0 + lo - i0;
-            out.ntok = hi - lo;
-            out.pos0 = lo;
-            out.n = n;
-            out.snap = p.snapshot(out.s, p.boundary(lo));
-            return true;
-        }
-        before += __shfl_sync(~0u, sum, 31);
-    }
-    return false;
-}
 
 __device__ __forceinline__ void fmul2(float &d0, float &d1, float a0, float a1, float b0, float b1)
 {
@@ -796,9 +746,7 @@ static int launch_chunk(const PagedAttnParams &a, cudaStream_t stream)
     }
     auto kern = paged_chunk_kernel<D, F16, Q8>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kTotal) != cudaSuccess) return VQ_ELAUNCH;
-    // tiles: every block of positions that a sequence touches rounds its tokens up to whole tiles
-    int64_t tiles = a.seqs.T / cp.TQ + a.seqs.T / kBlock + 2 * static_cast<int64_t>(a.seqs.S);
-    if (tiles > a.seqs.T) tiles = a.seqs.T;
+    const int64_t tiles = chunk_tiles(a.seqs, cp.TQ);
     kern<<<dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.Hkv)), C::kThreads, C::kTotal, stream>>>(m.q1, m.q2, m.k1, m.k3, m.v, m.cb, m.vs, cp);
     return launch_status();
 }
