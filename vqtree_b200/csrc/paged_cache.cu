@@ -5,9 +5,11 @@
 // (every lane of a token reads the same words).  8-bit rows: scale = max|x| * (1/127), code = rint(x * (1/scale)); the maximum is an
 // exchange inside the group, x is the fp32 rotation (quantising a rotation already rounded to 16 bits would round twice), and every
 // operation is rounded on its own, so codes and scales are reproducible bit for bit.  Division-free per element: one reciprocal a row.
-// Read: a thread per 16 bytes of output.  Both are bound by memory traffic, and by their launch when there are few rows.
+// Read: a thread per 16 bytes of stored rows.  Both are bound by memory traffic, and by their launch when there are few rows.
 #include "paged_common.cuh"
 #include "rope_common.cuh"
+
+#include <type_traits>
 
 namespace vq {
 
@@ -16,6 +18,16 @@ __device__ __forceinline__ float max_nan(float a, float b)
     float d;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
+}
+
+// rint(x * inv) of four values, as bytes.  Adding 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low bits (|x * inv| is at
+// most 127 and a few units): two additions of the fp32 pipe instead of a conversion of the slower one.
+__device__ __forceinline__ uint32_t four_codes(float x0, float x1, float x2, float x3, float inv)
+{
+    constexpr float kMagic = 12582912.f;
+    const uint32_t b0 = __float_as_uint(__fadd_rn(__fmul_rn(x0, inv), kMagic)), b1 = __float_as_uint(__fadd_rn(__fmul_rn(x1, inv), kMagic));
+    const uint32_t b2 = __float_as_uint(__fadd_rn(__fmul_rn(x2, inv), kMagic)), b3 = __float_as_uint(__fadd_rn(__fmul_rn(x3, inv), kMagic));
+    return __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
 }
 
 // One row, N elements of the first half in a and N of the second in b, written to a pool in its own type or as 8-bit codes with a scale.
@@ -40,12 +52,12 @@ struct RowStore {
             uint32_t lo[N / 4], hi[N / 4];
 #pragma unroll
             for (int w = 0; w < N / 4; ++w) {
-                lo[w] = hi[w] = 0;
+                lo[w] = four_codes(a[4 * w], a[4 * w + 1], a[4 * w + 2], a[4 * w + 3], inv);
+                hi[w] = four_codes(b[4 * w], b[4 * w + 1], b[4 * w + 2], b[4 * w + 3], inv);
+            }
+            if (!finite) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    lo[w] |= (static_cast<uint32_t>(finite ? __float2int_rn(__fmul_rn(a[4 * w + i], inv)) : 0) & 255u) << (8 * i);
-                    hi[w] |= (static_cast<uint32_t>(finite ? __float2int_rn(__fmul_rn(b[4 * w + i], inv)) : 0) & 255u) << (8 * i);
-                }
+                for (int w = 0; w < N / 4; ++w) lo[w] = hi[w] = 0;
             }
             if constexpr (N == 8) {
                 *reinterpret_cast<uint2 *>(dst) = make_uint2(lo[0], lo[1]);
@@ -72,11 +84,13 @@ struct AppendParams {
     int64_t k_t, k_h, v_t, v_h, q_t, q_h, q1_t, q1_h, q2_t, q2_h;   // strides in elements
     const float *cos_tab, *sin_tab;
     int64_t n_pos, const_pos;
-    uint32_t items;              // T * (2 Hkv + Hq)
+    uint32_t items;              // groups of heads of all tokens
 };
 
-template <typename T, typename KV, int D>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
+// A group of lanes takes U heads of one kind - keys, values or queries - of a token: they share the look-ups and the table's row, which is twice a
+// 16-bit row.
+template <typename T, typename KV, int D, int U>
+__global__ void __launch_bounds__(256, sizeof(KV) == 1 ? 3 : 2) paged_append_kernel(const AppendParams p)
 {
     using St = RowStore<T, KV, D>;
     constexpr int N = St::N, LPR = St::LPR;
@@ -84,61 +98,88 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
     const uint32_t item = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
     if (item >= p.items) return;                                     // whole groups leave together
     const unsigned g_mask = (LPR == 32 ? 0xffffffffu : (1u << LPR) - 1u) << (threadIdx.x % 32 / LPR * LPR);
-    const uint32_t rows = 2 * p.Hkv + p.Hq, t = item / rows, r = item - t * rows;
+    const uint32_t kg = (p.Hkv + U - 1) / U, per = 2 * kg + (p.Hq + U - 1) / U, t = item / per, r = item - t * per;
+    const bool is_q = r >= 2 * kg, is_v = !is_q && r >= kg;
+    const int h0 = static_cast<int>(is_q ? r - 2 * kg : is_v ? r - kg : r) * U, heads = min(U, (is_q ? p.Hq : p.Hkv) - h0);
+    const int64_t sh = is_q ? p.q_h : is_v ? p.v_h : p.k_h;
+    const T *src = (is_q ? static_cast<const T *>(p.q) + t * p.q_t : is_v ? static_cast<const T *>(p.vin) + t * p.v_t
+                                                                        : static_cast<const T *>(p.k) + t * p.k_t) + h0 * sh + l * N;
+    float x1[U][N], x2[U][N], o1[N], o2[N];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const T *row = src + (u < heads ? u : 0) * sh;
+        RopeVec<T>::load(row, x1[u]);
+        RopeVec<T>::load(row + D / 2, x2[u]);
+    }
     const int s = p.seqs.find(t);
     if (s >= p.seqs.S) return;                                       // behind the last sequence
     int t0, q, n;
     if (!p.seqs.seq(s, t0, q, n) || t < static_cast<uint32_t>(t0)) return;
-    const int pos = n - q + (static_cast<int>(t) - t0);
-    const bool is_q = r >= 2u * p.Hkv, is_v = !is_q && r >= static_cast<uint32_t>(p.Hkv);
-    const int h = static_cast<int>(is_q ? r - 2 * p.Hkv : is_v ? r - p.Hkv : r);
-    const T *src = is_q ? static_cast<const T *>(p.q) + t * p.q_t + h * p.q_h
-                 : is_v ? static_cast<const T *>(p.vin) + t * p.v_t + h * p.v_h : static_cast<const T *>(p.k) + t * p.k_t + h * p.k_h;
-    float x1[N], x2[N], o1[N], o2[N];
-    RopeVec<T>::load(src + l * N, x1);
-    RopeVec<T>::load(src + D / 2 + l * N, x2);
+    const int pos = n - q + (static_cast<int>(t) - t0), pr = pos & ((1 << p.seqs.log_p) - 1);
     int page = 0;
-    const int pr = pos & ((1 << p.seqs.log_p) - 1);
     if (!is_q) {
         page = p.seqs.page(s, pos >> p.seqs.log_p);
         if (page < 0) return;
     }
     if (is_v) {
-        St::put(p.v, page, h, pr, l, g_mask, x1, x2);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (u < heads) St::put(p.v, page, h0 + u, pr, l, g_mask, x1[u], x2[u]);
         return;
     }
-    if (p.cos_tab != nullptr) {
+    const bool turn = p.cos_tab != nullptr;
+    float cv[N], sv[N];
+    if (turn) {
         int64_t at = pos;
         if (at >= p.n_pos) {
             at = p.n_pos - 1;
             p.seqs.raise(VQ_WORD_BAD_POSITION);
         }
-        at = at * (D / 2) + l * N;
-        rope_rotate<N>(x1, x2, p.cos_tab + at, p.sin_tab + at, o1, o2);
-    } else {
+        rope_table<N>(p.cos_tab + at * (D / 2) + l * N, cv);
+        rope_table<N>(p.sin_tab + at * (D / 2) + l * N, sv);
+    }
+    auto rotate = [&](int u) {
+        if (turn) {
+            rope_apply<N>(x1[u], x2[u], cv, sv, o1, o2);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            o1[i] = x1[i];
-            o2[i] = x2[i];
+            o1[i] = x1[u][i];
+            o2[i] = x2[u][i];
         }
-    }
+    };
     if (!is_q) {
-        St::put(p.k1, page, h, pr, l, g_mask, o1, o2);
-        if (p.raw) St::put(p.k3, page, h, pr, l, g_mask, x1, x2);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= heads) continue;
+            rotate(u);
+            St::put(p.k1, page, h0 + u, pr, l, g_mask, o1, o2);
+            if (p.raw) St::put(p.k3, page, h0 + u, pr, l, g_mask, x1[u], x2[u]);
+        }
         return;
     }
-    T *d1 = static_cast<T *>(p.q1) + t * p.q1_t + h * p.q1_h + l * N;
-    RopeVec<T>::store(d1, o1);
-    RopeVec<T>::store(d1 + D / 2, o2);
+    auto queries = [&](void *out, int64_t st, int64_t shd) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= heads) continue;
+            rotate(u);
+            T *dst = static_cast<T *>(out) + t * st + (h0 + u) * shd + l * N;
+            RopeVec<T>::store(dst, o1);
+            RopeVec<T>::store(dst + D / 2, o2);
+        }
+    };
+    queries(p.q1, p.q1_t, p.q1_h);
     if (p.q2 == nullptr) return;
-    if (p.cos_tab != nullptr) {
-        const int64_t at = p.const_pos * (D / 2) + l * N;
-        rope_rotate<N>(x1, x2, p.cos_tab + at, p.sin_tab + at, o1, o2);
+    if (turn) {
+        rope_table<N>(p.cos_tab + p.const_pos * (D / 2) + l * N, cv);
+        rope_table<N>(p.sin_tab + p.const_pos * (D / 2) + l * N, sv);
     }
-    T *d2 = static_cast<T *>(p.q2) + t * p.q2_t + h * p.q2_h + l * N;
-    RopeVec<T>::store(d2, o1);
-    RopeVec<T>::store(d2 + D / 2, o2);
+    queries(p.q2, p.q2_t, p.q2_h);
 }
+
+// byte j of w, which is code + 128, as the code's fp32 value: 2^23 + w[j] - (2^23 + 128)
+__device__ __forceinline__ float code_f32(uint32_t w, int j) { return __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | j)) - 8388736.f; }
 
 struct ReadParams {
     PagedPool pool[3];
@@ -146,85 +187,138 @@ struct ReadParams {
     const int32_t *table, *start, *lens;
     int64_t t_row;
     int MB, NP, log_p, S, Hkv, n;
-    uint64_t items;              // threads' worth of output of one pool
+    uint64_t items;              // 16-byte pieces of one pool's rows
     int32_t *status;
 };
 
-// A thread writes N elements (16 bytes) of an output row.
-template <typename KV, typename O, int D>
-__global__ void __launch_bounds__(256) paged_read_kernel(const ReadParams p)
+// A thread takes 16 bytes of U rows, whose loads are under way together.  Eight CTAs of an SM: the way to a row is a chain of loads (length, table,
+// row), which only more threads can hide.
+template <typename KV, typename O, int D, int U>
+__global__ void __launch_bounds__(256, 8) paged_read_kernel(const ReadParams p)
 {
-    constexpr int N = 16 / sizeof(O), LPR = D / N;
-    const uint64_t i = blockIdx.x * uint64_t(256) + threadIdx.x;
-    if (i >= p.items) return;
-    const int which = blockIdx.y, l = static_cast<int>(i % LPR);
-    uint64_t row = i / LPR;
+    constexpr int N = 16 / sizeof(KV), LPR = D / N, STEP = 256 / LPR;
+    const int which = blockIdx.y, l = threadIdx.x % LPR;
+    const uint64_t row0 = blockIdx.x * static_cast<uint64_t>(U * STEP) + threadIdx.x / LPR, rows = p.items / LPR;
+    if (row0 >= rows) return;
     uint32_t s, h, r;
-    if (p.items <= 0xffffffffu) {                                    // the usual case: divisions in 32 bits
-        const uint32_t w = static_cast<uint32_t>(row), sh = w / p.n;
+    if (rows <= 0xffffffffu) {                                       // the usual case: divisions in 32 bits
+        const uint32_t w = static_cast<uint32_t>(row0), sh = w / p.n;
         r = w - sh * p.n;
         s = sh / p.Hkv;
         h = sh - s * p.Hkv;
     } else {
-        const uint64_t sh = row / p.n;
-        r = static_cast<uint32_t>(row - sh * p.n);
+        const uint64_t sh = row0 / p.n;
+        r = static_cast<uint32_t>(row0 - sh * p.n);
         s = static_cast<uint32_t>(sh / p.Hkv);
         h = static_cast<uint32_t>(sh - static_cast<uint64_t>(s) * p.Hkv);
     }
-    const int64_t pos = static_cast<int64_t>(__ldg(p.start + s)) + r;
-    float x[N];
+    const PagedPool &pool = p.pool[which];
+    uint4 in[U];
+    float scale[U];
+    bool there[U];
+    const KV *head = static_cast<const KV *>(pool.ptr) + h * pool.s_head + l * N;
+    const float *head_scale = pool.scale + h * pool.c_head;
+    int start = __ldg(p.start + s), len = __ldg(p.lens + s);
+    const int32_t *table = p.table + s * p.t_row;
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = 0.f;
-    O *dst = static_cast<O *>(p.out[which]) + row * D + l * N;
-    if (pos >= 0 && pos < __ldg(p.lens + s)) {
-        const int64_t col = pos >> p.log_p;
-        const int page = col < p.MB ? __ldg(p.table + s * p.t_row + col) : -1;
-        if (page < 0 || page >= p.NP) {
-            if (p.status) atomicExch(p.status, VQ_WORD_BAD_PAGE);
-        } else {
-            const PagedPool &pool = p.pool[which];
-            const int pr = static_cast<int>(pos) & ((1 << p.log_p) - 1);
-            const KV *src = static_cast<const KV *>(pool.ptr) + pool.row(page, h, pr) + l * N;
-            if constexpr (sizeof(KV) == 1) {
-                const float scale = __ldg(pool.scale + pool.scale_at(page, h, pr));
-                uint32_t w[N / 4];
-                if constexpr (N == 8) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(src);
-                    w[0] = v.x; w[1] = v.y;
+    for (int u = 0; u < U; ++u) {
+        there[u] = false;
+        in[u] = make_uint4(0, 0, 0, 0);
+        scale[u] = 0.f;
+        if (row0 + u * STEP < rows) {
+            const int64_t pos = static_cast<int64_t>(start) + r;
+            if (pos >= 0 && pos < len) {
+                const int col = static_cast<int>(pos) >> p.log_p, pr = static_cast<int>(pos) & ((1 << p.log_p) - 1);
+                const int page = col < p.MB ? __ldg(table + col) : -1;
+                if (page < 0 || page >= p.NP) {
+                    if (p.status) atomicExch(p.status, VQ_WORD_BAD_PAGE);
                 } else {
-                    w[0] = *reinterpret_cast<const uint32_t *>(src);
+                    there[u] = true;
+                    in[u] = *reinterpret_cast<const uint4 *>(head + page * pool.s_page + pr * pool.s_row);
+                    if constexpr (sizeof(KV) == 1) scale[u] = __ldg(head_scale + page * pool.c_page + pr * pool.c_row);
                 }
-#pragma unroll
-                for (int j = 0; j < N; ++j) x[j] = dequant(static_cast<int8_t>(w[j / 4] >> (8 * (j % 4))), scale);
-            } else {
-                *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
-                return;
             }
         }
+        if (u + 1 == U || row0 + (u + 1) * STEP >= rows) continue;
+        r += STEP;
+        if (r < static_cast<uint32_t>(p.n)) continue;
+        do {
+            r -= p.n;
+            if (++h == static_cast<uint32_t>(p.Hkv)) {
+                h = 0;
+                ++s;
+            }
+        } while (r >= static_cast<uint32_t>(p.n));
+        head = static_cast<const KV *>(pool.ptr) + h * pool.s_head + l * N;
+        head_scale = pool.scale + h * pool.c_head;
+        start = __ldg(p.start + s);
+        len = __ldg(p.lens + s);
+        table = p.table + s * p.t_row;
     }
-    RopeVec<O>::store(dst, x);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (row0 + u * STEP >= rows) return;
+        O *dst = static_cast<O *>(p.out[which]) + (row0 + u * STEP) * D + l * N;
+        if constexpr (sizeof(KV) == 1) {
+            constexpr int V = RopeVec<O>::kN;
+            const uint32_t w[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
+#pragma unroll
+            for (int i = 0; i < N; i += V) {
+                float x[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[j] = there[u] ? __fmul_rn(code_f32(w[(i + j) / 4] ^ 0x80808080u, (i + j) % 4), scale[u]) : 0.f;
+                RopeVec<O>::store(dst + i, x);
+            }
+        } else {
+            *reinterpret_cast<uint4 *>(dst) = in[u];
+        }
+    }
+}
+
+// Rows per thread: several where there are many CTAs anyway, one where there are few.  Measured with several / with one, us: appending 2048 tokens
+// of 32 kv heads, 16 bits 29.8 / 32.5; second turns of 12 sequences, 8 bits, with reading them back 120 / 132; reading 16 windows of 2303 rows,
+// 32 heads, 8 bits to half (915 MB) 162 / 215.
+constexpr int kManyCtas = 148 * 8;
+
+template <typename T, typename KV, int D>
+static int launch_append(AppendParams &p, cudaStream_t stream)
+{
+    constexpr int U = 4;
+    constexpr uint32_t per = 256u / RowStore<T, KV, D>::LPR;
+    const int64_t T_ = p.seqs.T;
+    const bool many = T_ * (2 * p.Hkv + p.Hq) / per >= static_cast<int64_t>(U) * kManyCtas;
+    const int u = many ? U : 1;
+    p.items = static_cast<uint32_t>(T_ * (2 * ((p.Hkv + u - 1) / u) + (p.Hq + u - 1) / u));
+    const uint32_t grid = (p.items + per - 1) / per;
+    if (many) paged_append_kernel<T, KV, D, U><<<grid, 256, 0, stream>>>(p);
+    else paged_append_kernel<T, KV, D, 1><<<grid, 256, 0, stream>>>(p);
+    return launch_status();
 }
 
 template <typename T, typename KV>
-static int launch_append(const AppendParams &p, int D, cudaStream_t stream)
+static int launch_append(AppendParams &p, int D, cudaStream_t stream)
 {
-    const int lpr = D / 2 / RopeVec<T>::kN;
-    const uint32_t per = 256u / lpr, grid = (p.items + per - 1) / per;
-    if (D == 64) paged_append_kernel<T, KV, 64><<<grid, 256, 0, stream>>>(p);
-    else paged_append_kernel<T, KV, 128><<<grid, 256, 0, stream>>>(p);
+    return D == 64 ? launch_append<T, KV, 64>(p, stream) : launch_append<T, KV, 128>(p, stream);
+}
+
+template <typename KV, typename O, int D>
+static int launch_read(ReadParams &p, int pools, cudaStream_t stream)
+{
+    constexpr int U = 2;
+    p.items = static_cast<uint64_t>(p.S) * p.Hkv * p.n * (D * sizeof(KV) / 16);
+    const uint64_t blocks = (p.items + 255) / 256;
+    if (blocks > 0x7fffffffu) return VQ_EUNSUPPORTED;
+    if (blocks * pools >= U * kManyCtas)
+        paged_read_kernel<KV, O, D, U><<<dim3(static_cast<unsigned>((blocks + U - 1) / U), static_cast<unsigned>(pools)), 256, 0, stream>>>(p);
+    else
+        paged_read_kernel<KV, O, D, 1><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(pools)), 256, 0, stream>>>(p);
     return launch_status();
 }
 
 template <typename KV, typename O>
 static int launch_read(ReadParams &p, int D, int pools, cudaStream_t stream)
 {
-    p.items = static_cast<uint64_t>(p.S) * p.Hkv * p.n * (D * sizeof(O) / 16);
-    const uint64_t blocks = (p.items + 255) / 256;
-    if (blocks > 0x7fffffffu) return VQ_EUNSUPPORTED;
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(pools));
-    if (D == 64) paged_read_kernel<KV, O, 64><<<grid, 256, 0, stream>>>(p);
-    else paged_read_kernel<KV, O, 128><<<grid, 256, 0, stream>>>(p);
-    return launch_status();
+    return D == 64 ? launch_read<KV, O, 64>(p, pools, stream) : launch_read<KV, O, 128>(p, pools, stream);
 }
 
 }  // namespace vq
@@ -267,7 +361,6 @@ extern "C" int vqattn_paged_append(const VqPagedAppendArgs *a, void *stream)
     p.q_t = a->q.stride[0]; p.q_h = a->q.stride[1]; p.q1_t = a->q1.stride[0]; p.q1_h = a->q1.stride[1];
     p.q2_t = a->q2.stride[0]; p.q2_h = a->q2.stride[1];
     p.cos_tab = a->cos_tab; p.sin_tab = a->sin_tab; p.n_pos = a->n_pos; p.const_pos = a->const_pos;
-    p.items = static_cast<uint32_t>(T * rows);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (kv.dtype == VQ_I8) {
         if (dt == VQ_F32) return launch_append<float, int8_t>(p, kv.D, s);
