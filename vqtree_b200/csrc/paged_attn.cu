@@ -52,7 +52,15 @@ extern "C" int vqattn_paged_attention(const VqPagedAttentionArgs *a, void *strea
     p.wait_limit = wait_limit_cycles();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv.dtype == VQ_I8;
-    if (is_16bit(dt) && static_cast<int64_t>(p.max_q) * G <= kFewRows) return launch_paged_few(p, dt, q8, s);
-    if (is_16bit(dt)) return launch_paged_chunk(p, dt, q8, s);
+    if (is_16bit(dt)) {
+        // The line between the forms, in us, few / chunk, 8 kv heads, MK1024, W1024.  16 rows: 8 sequences 18 / 34, 32 sequences 46 / 75; 32 rows: 8
+        // sequences 31 / 35 (8 bits 39 / 59; D = 64 23 / 33), 32 sequences 94 / 77 (8 bits 125 / 127; D = 64 68 / 72): more than 16 rows of
+        // 16-bit caches with D = 128 go to the chunk form once the pairs of sequences and heads fill the chip.
+        int dev = 0, sms = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return VQ_EDEVICE;
+        const int64_t rows = static_cast<int64_t>(p.max_q) * G;
+        const bool few = rows <= 16 || (rows <= kFewRows && (q8 || kv.D == 64 || static_cast<int64_t>(p.seqs.S) * p.Hkv <= sms));
+        return few ? launch_paged_few(p, dt, q8, s) : launch_paged_chunk(p, dt, q8, s);
+    }
     return launch_paged_f32(p, q8, s);
 }

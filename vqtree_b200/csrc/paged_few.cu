@@ -53,11 +53,13 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x)
 }
 template <typename T, bool Q8, int D, int NT>
 struct FewCfg {
-    // Warps that compute (one more issues the loads), stages of their FIFOs, CTAs of an SM: what registers and shared memory allow.  Measured,
-    // us: 64 sequences of 8 kv heads, 16 bits, 3 warps x 2 stages x 4 CTAs / 4 x 3 x 2: 136 / 152 (all 512 units run at once); 16 sequences
-    // of 32 heads, 8 bits, 5 x 2 x 2 / 4 x 3 x 2 / 3 x 2 x 3: 77 / 87 / 104.
-    static constexpr int kWarps = Q8 ? 5 : NT == 1 ? 3 : 4, kThreads = (kWarps + 1) * 32;
-    static constexpr int kStages = NT == 1 ? 2 : 3;
+    // Warps that compute (one more issues the loads), stages of their FIFOs, CTAs of an SM: what registers and shared memory allow.  Measured, us.
+    // Up to 8 rows: 64 sequences of 8 kv heads, 16 bits, 3 warps x 2 stages x 4 CTAs / 4 x 3 x 2: 136 / 152 (all 512 units run at once); 16
+    // sequences of 32 heads, 8 bits, 5 x 2 x 2 / 4 x 3 x 2 / 3 x 2 x 3: 77 / 87 / 104.  16 rows, 32 sequences of 8 heads, D = 128, 3 x 3 x 2 /
+    // 4 x 3 x 2 (8 bits: 5 x 3 x 2): 46 / 50, 8 bits 64 / 90 (which spills); D = 64: 42 / 38, 45 / 34.  32 rows, 7 x 2 x 1 / 4 x 3 x 1: 94 / 123,
+    // 8 bits 125 / 144, D = 64 68 / 74.
+    static constexpr int kWarps = NT == 1 ? (Q8 ? 5 : 3) : NT == 2 ? (D == 128 ? 3 : Q8 ? 5 : 4) : 7, kThreads = (kWarps + 1) * 32;
+    static constexpr int kStages = NT == 2 ? 3 : 2;
     static constexpr int kCtas = NT == 1 ? (Q8 ? 2 : 4) : NT == 2 ? 2 : 1;
     static constexpr int kCols = 8 * NT;                         // query rows, padded
     static constexpr int VC = D / 64;                            // boxes of 64 columns of a 16-bit row
@@ -102,7 +104,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
     int unit = blockIdx.x / nsplit;
     const int hk = unit % p.Hkv;
     unit /= p.Hkv;
-    const int grp = unit % groups, s = unit / groups;
+    const int s = unit % p.seqs.S, grp = unit / p.seqs.S;           // second blocks, hardly ever there, come last: the others get an SM each
     int t0, q, n;
     grid_dependency_launch();
     grid_dependency_wait();
