@@ -363,7 +363,7 @@ typedef struct VqPagedKv {
  * NULL), v [T,Hkv,D] -> v, rounded to the pools' type or quantised to i8 (from the fp32 rotation, not from a rounded one).
  * q [T,Hq,D] (ptr NULL: none) -> q1 [T,Hq,D] rotated to the tokens' positions, and q2 [T,Hq,D] (ptr NULL: none) rotated to const_pos.
  * cos_tab / sin_tab [n_pos, D/2] f32 as for vqattn_rope; NULL: keys (and queries) are stored as they are.
- * The pools' type is k's, or i8.  A position outside the tables raises VQ_WORD_BAD_POSITION and uses the nearest row.
+ * The pools' type is k's, or i8; k3 may not be k1's memory.  A position outside the tables raises VQ_WORD_BAD_POSITION and uses the nearest row.
  */
 typedef struct VqPagedAppendArgs {
     VqPagedKv kv;
@@ -393,7 +393,7 @@ int vqattn_paged_read(const VqPagedReadArgs *args, void *stream);
  * Attention of the new tokens over a paged cache that already holds them: row t of sequence s at position
  * i = lens[s] - (cu_q[s+1] - cu_q[s]) + (t - cu_q[s]) gets what row i of vqattn_prefill over the whole sequence is defined to be, with
  * boundary = max(0, ((i - window) / 128) * 128):
- *   keys [max(0,i-window), i] scored q1.k1, keys [boundary, max(0,i-window)) scored q2.k3 (k3.ptr NULL: q2.k1), older keys through counts
+ *   keys [max(0,i-window), i] scored q1.k1, keys [boundary, max(0,i-window)) scored q2.k3 (k3.ptr NULL: q1.k1 as well), older keys by counts
  *   and value sums per code of the snapshot of that boundary: snapshot snap_table[s][(boundary / 128) % MS] of cnt and vsum.
  *   A decode therefore needs one column (the running aggregates), a chunk of c tokens (c - 1) / 128 + 2 of them at most.
  *   q1, q2, out [T,Hq,D] f32 | bf16 | f16 (q2 may alias q1);  pools of that type or i8;

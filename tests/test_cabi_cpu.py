@@ -115,6 +115,8 @@ def test_paged_entry_points_refuse_bad_arguments_without_a_device():
 
     z = torch.zeros
     assert append() == -4                                           # host tensors
+    pool = z(4, 2, 16, 64)
+    assert append(k1=pool, k3=pool) == -7 and append(k1=pool, v_pool=pool) == -7 and append(k3=None) == -4
     assert append(k=None) == -7 and append(k1=None) == -7 and append(v_pool=None) == -7
     assert append(k=z(7, 2, 64, dtype=torch.int32)) == -2 and append(k=z(7, 2, 64, dtype=torch.bfloat16)) == -2
     assert append(v=z(7, 3, 64)) == -1 and append(v=z(6, 2, 64)) == -1 and append(k=z(7, 2)) == -1

@@ -335,6 +335,7 @@ extern "C" int vqattn_paged_append(const VqPagedAppendArgs *a, void *stream)
     PagedArgs kv;
     if ((st = check_paged_kv(a->kv, T, a->status_word, kv)) != VQ_OK) return st;
     if (kv.dtype != VQ_I8 && kv.dtype != dt) return VQ_EINVAL_DTYPE;
+    if (a->kv.k3.ptr == a->kv.k1.ptr || a->kv.v.ptr == a->kv.k1.ptr || a->kv.v.ptr == a->kv.k3.ptr) return VQ_EINVAL_ARG;   // three writers of one row
     if ((st = check_tokens(a->k, T, kv.Hkv, kv.D, dt)) != VQ_OK) return st;
     if ((st = check_tokens(a->v, T, kv.Hkv, kv.D, dt)) != VQ_OK) return st;
     const bool has_q = a->q.ptr != nullptr;
