@@ -402,6 +402,11 @@ int vqattn_paged_read(const VqPagedReadArgs *args, void *stream);
  *   max_q: an upper bound of the new tokens of any sequence; a sequence with more is left out (VQ_WORD_BAD_LENGTH).
  * Codes with cnt == 0 are excluded and their vsum rows must be finite.  Values of a sequence are expected to be finite; what lies behind its
  * end in its last page may be anything.
+ *
+ * workspace: NULL, or vqattn_paged_attention_workspace_bytes(...) bytes of device memory, 256-byte aligned, contents arbitrary before and after.
+ * With i8 pools and chunks that are long for their windows every key is needed by many query tiles; its codes are then turned into 16-bit
+ * floats once, in the workspace, instead of once per tile.  Same results.  The size is 0 where none would be used; one that is too small is not
+ * used either.
  */
 typedef struct VqPagedAttentionArgs {
     VqPagedKv kv;
@@ -410,8 +415,12 @@ typedef struct VqPagedAttentionArgs {
     int64_t window, max_q;
     float scale;           /* <= 0: 1/sqrt(D) */
     int32_t *status_word;
+    void *workspace;
+    size_t workspace_bytes;
 } VqPagedAttentionArgs;
 
+size_t vqattn_paged_attention_workspace_bytes(int64_t S, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t max_q,
+                                              int32_t pool_dtype, int32_t act_dtype);
 int vqattn_paged_attention(const VqPagedAttentionArgs *args, void *stream);
 
 #ifdef __cplusplus

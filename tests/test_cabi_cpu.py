@@ -172,3 +172,13 @@ def test_paged_entry_points_refuse_bad_arguments_without_a_device():
     assert attend(cnt=z(4, 2, 128)) == -1 and attend(cnt=None) == -7 and attend(snap_table=i32(2, 2)) == -1 and attend(snap_table=z(3, 2)) == -2
     assert attend(vsum=z(5, 2, 64, 128).transpose(2, 3)) == -3
     assert attend(q1=z(7, 258, 64), q2=z(7, 258, 64), out=z(7, 258, 64)) == -8   # more than 128 query heads per kv head
+
+
+def test_paged_attention_workspace_size():
+    ws = _native().lib.vqattn_paged_attention_workspace_bytes
+    # six sequences, 2228 new tokens of 4 query heads per kv head: three pools of 6 * (8 + 3) + 17 blocks of 128 rows
+    assert ws(6, 2228, 32, 8, 128, 1024, 597, 7, 1) == 3 * (6 * 11 + 17) * 8 * 128 * 128 * 2
+    assert ws(6, 2228, 32, 8, 128, 1024, 597, 1, 1) == 0            # rows of 16 bits
+    assert ws(6, 2228, 32, 8, 128, 1024, 597, 7, 0) == 0            # full precision
+    assert ws(64, 2228, 32, 8, 128, 1024, 597, 7, 1) == 0           # few tiles per sequence
+    assert ws(1, 4, 32, 8, 128, 1024, 4, 7, 1) == 0 and ws(0, 0, 0, 0, 0, 0, 0, 7, 1) == 0 and ws(-1, 9, 4, 4, 128, 128, 9, 7, 1) == 0

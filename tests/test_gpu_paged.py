@@ -168,6 +168,24 @@ def test_attention(api, qs, lens, Hkv, G, D, P, W, MK, dtype, q8, rerope):
     check_attention(out, c)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rerope", [True, False])
+@pytest.mark.parametrize("qs,lens,Hkv,G,D,P,W", [((300,), (1000,), 2, 4, 128, 64, 256), ((0, 700, 0, 600, 3), (7, 700, 0, 900, 500), 1, 8, 64, 16, 128),
+                                                 ((257, 300), (257, 600), 2, 4, 128, 128, 512)])
+def test_attention_8_bit_rows_converted_first_or_on_the_way(api, dtype, rerope, qs, lens, Hkv, G, D, P, W):
+    """Long chunks over 8-bit pages: through the workspace and without one, the same bits."""
+    c = Case(sum(lens), qs, lens, Hkv, G, D, P, W, 128, dtype, True, rerope)
+    need = api.paged_attention_workspace_bytes(len(qs), c.T, Hkv * G, D, Hkv, W, max(qs), torch.int8, dtype)
+    assert need > 0
+    room = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")          # bytes that are no numbers, and a guard behind them
+    a = c.attend(api, workspace=room[:need])
+    assert (room[need:] == 255).all()
+    b = c.attend(api, workspace=room[:16])                                            # too small: not used
+    api.check_status()
+    check_attention(a, c)
+    assert torch.equal(a, b) and torch.equal(a, c.attend(api))
+
+
 @pytest.mark.parametrize("dtype,q8", [(BF16, False), (F16, True), (F32, False)])
 @pytest.mark.parametrize("qs,lens", [((1, 1), (300, 800)), ((3, 2), (259, 700)), ((140, 9), (600, 777))])
 def test_attention_without_codebook_and_with_spare_snapshot_columns(api, dtype, q8, qs, lens):

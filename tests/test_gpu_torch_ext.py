@@ -107,11 +107,11 @@ def test_paged_operators_through_the_dispatcher_equal_the_api(ops, api):
         q1, q2, out = c.q1.cuda(), c.q2.cuda(), torch.empty_like(want)
         meta = (c.table.cuda(), c.cu_q.cuda(), c.seq_lens.cuda())
         args = (q1, q2, *p, *meta, far["codebook"], far["cnt"], far["vsum"], far["snap_table"], c.W)
-        ops.paged_attention(*args, max(qs), 0.0, out, None)
+        ops.paged_attention(*args, max(qs), 0.0, out, None, None)
         assert torch.equal(out, want)
         with pytest.raises(RuntimeError, match="status -7"):
-            ops.paged_attention(*args, 0, 0.0, out, None)
-        assert ops.paged_attention_status(*args, 0, 0.0, out, None) == -7
+            ops.paged_attention(*args, 0, 0.0, out, None, None)
+        assert ops.paged_attention_status(*args, 0, 0.0, out, None, None) == -7
         back = torch.empty(2, 2, 40, 64, dtype=torch.bfloat16, device="cuda")
         start = (meta[2] - 40).contiguous()
         ops.paged_read(p.v, p.v_scale, back, None, None, None, None, None, None, meta[0], start, meta[2], None)

@@ -541,17 +541,25 @@ def paged_read(pools, block_table: torch.Tensor, starts: torch.Tensor, seq_lens:
     return outs
 
 
+def paged_attention_workspace_bytes(S: int, T: int, Hq: int, D: int, Hkv: int, window: int, max_q: int, pool_dtype: torch.dtype,
+                                    dtype: torch.dtype) -> int:
+    """Bytes of workspace ``paged_attention`` makes use of (0: none): int8 pages whose keys are needed by many query tiles."""
+    return int(lib.vqattn_paged_attention_workspace_bytes(S, T, Hq, Hkv, D, int(window), int(max_q), native._DTYPES[pool_dtype], native._DTYPES[dtype]))
+
+
 def paged_attention(q1: torch.Tensor, q2: torch.Tensor, pages: PagedKV, block_table: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor,
                     window: int, max_q: int, codebook: Optional[torch.Tensor] = None, cnt: Optional[torch.Tensor] = None,
                     vsum: Optional[torch.Tensor] = None, snap_table: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the new tokens of S sequences over their pages (which hold them already): every row is what the same row of
     ``vq_attention_prefill`` over the whole sequence is defined to be.
 
     q1, q2 [T,Hq,D] (q2 may be q1) packed by cu_q; block_table, cu_q, seq_lens as in ``paged_append``; max_q: an upper bound of the new
     tokens of one sequence.  codebook [Hkv,MK,D], cnt [NS,Hkv,MK] f32, vsum [NS,Hkv,MK,D], snap_table int32 [S,MS]: keys before the
     boundary b of a query count through snapshot ``snap_table[s, b // 128 % MS]`` (None: the local part only).  Returns [T,Hq,D]; rows
-    from cu_q[S] on are left as they are."""
+    from cu_q[S] on are left as they are.
+    workspace: uint8, paged_attention_workspace_bytes(...) of them (None: allocated for the call where one is of use - long chunks over int8
+    pages)."""
     if codebook is None:
         cnt = vsum = snap_table = None
     elif cnt is None or vsum is None or snap_table is None:
@@ -560,12 +568,17 @@ def paged_attention(q1: torch.Tensor, q2: torch.Tensor, pages: PagedKV, block_ta
         return q1.new_empty(q1.shape) if out is None else out
     calls, word = _paged_calls(q1)
     k1, vp, k3, k1_scale, v_scale, k3_scale = pages
-    if out is None:
+    if out is None and workspace is None:
         out, status = calls[4](q1, q2, k1, vp, k3, k1_scale, v_scale, k3_scale, block_table, cu_q, seq_lens, codebook, cnt, vsum, snap_table, window,
                                max_q, scale or 0.0, word)
     else:
+        if out is None:
+            out = q1.new_empty(q1.shape)
+        if workspace is None and k1.dtype == torch.int8:
+            need = paged_attention_workspace_bytes(block_table.shape[0], *q1.shape, k1.shape[1], window, max_q, k1.dtype, q1.dtype)
+            workspace = torch.empty(need, dtype=torch.uint8, device=q1.device) if need else None
         status = calls[1](q1, q2, k1, vp, k3, k1_scale, v_scale, k3_scale, block_table, cu_q, seq_lens, codebook, cnt, vsum, snap_table, window, max_q,
-                          scale or 0.0, out, word)
+                          scale or 0.0, out, workspace, word)
     if status != 0:
         _paged_failed(status, "vqattn_paged_attention", q1, q2, *pages, block_table, cu_q, seq_lens, codebook, cnt, vsum, snap_table, out)
     return out

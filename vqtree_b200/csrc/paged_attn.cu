@@ -2,6 +2,33 @@
 // paged_chunk.cu; fp32: paged_f32.cu.
 #include "paged_attn.cuh"
 
+namespace vq {
+
+// The line between the forms, in us, few / chunk, 8 kv heads, MK1024, W1024.  16 rows: 8 sequences 18 / 34, 32 sequences 46 / 75; 32 rows: 8
+// sequences 31 / 35 (8 bits 39 / 59; D = 64 23 / 33), 32 sequences 94 / 77 (8 bits 125 / 127; D = 64 68 / 72): more than 16 rows of
+// 16-bit caches with D = 128 go to the chunk form once the pairs of sequences and heads fill the chip.
+static bool few_form(int64_t max_q, int64_t G, int64_t D, bool q8, int64_t units, int sms)
+{
+    const int64_t rows = max_q * G;
+    return rows <= 16 || (rows <= kFewRows && (q8 || D == 64 || units <= sms));
+}
+
+// three pools of blocks as 16-bit floats
+static size_t workspace_bytes(int64_t blocks, int64_t Hkv, int64_t D) { return static_cast<size_t>(3 * blocks * Hkv * kBlock * D * 2); }
+
+}  // namespace vq
+
+extern "C" size_t vqattn_paged_attention_workspace_bytes(int64_t S, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t max_q,
+                                                         int32_t pool_dtype, int32_t act_dtype)
+{
+    using namespace vq;
+    if (pool_dtype != VQ_I8 || !is_16bit(act_dtype) || S <= 0 || T <= 0 || Hkv <= 0 || Hq < Hkv || (D != 64 && D != 128) || window <= 0 || max_q <= 0) return 0;
+    if (S > (1 << 20) || T > 0x7fffffff || window > 0x40000000 || Hkv > 65535) return 0;
+    const int64_t G = Hq / Hkv, q = max_q < T ? max_q : T;
+    if (few_form(q, G, D, true, S * Hkv, 0) || !convert_first(S, T, G)) return 0;
+    return workspace_bytes(paged_blocks(S, T, window), Hkv, D);
+}
+
 extern "C" int vqattn_paged_attention(const VqPagedAttentionArgs *a, void *stream)
 {
     using namespace vq;
@@ -53,13 +80,15 @@ extern "C" int vqattn_paged_attention(const VqPagedAttentionArgs *a, void *strea
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv.dtype == VQ_I8;
     if (is_16bit(dt)) {
-        // The line between the forms, in us, few / chunk, 8 kv heads, MK1024, W1024.  16 rows: 8 sequences 18 / 34, 32 sequences 46 / 75; 32 rows: 8
-        // sequences 31 / 35 (8 bits 39 / 59; D = 64 23 / 33), 32 sequences 94 / 77 (8 bits 125 / 127; D = 64 68 / 72): more than 16 rows of
-        // 16-bit caches with D = 128 go to the chunk form once the pairs of sequences and heads fill the chip.
         int dev = 0, sms = 0;
         if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return VQ_EDEVICE;
-        const int64_t rows = static_cast<int64_t>(p.max_q) * G;
-        const bool few = rows <= 16 || (rows <= kFewRows && (q8 || kv.D == 64 || static_cast<int64_t>(p.seqs.S) * p.Hkv <= sms));
+        const bool few = few_form(p.max_q, G, kv.D, q8, static_cast<int64_t>(p.seqs.S) * p.Hkv, sms);
+        if (!few && q8 && convert_first(p.seqs.S, T, G)) {
+            p.ws_blocks = paged_blocks(p.seqs.S, T, p.W);
+            const size_t need = workspace_bytes(p.ws_blocks, kv.Hkv, kv.D);
+            if (p.ws_blocks * kv.Hkv <= 0x7fffffff && a->workspace != nullptr && a->workspace_bytes >= need && reinterpret_cast<uintptr_t>(a->workspace) % 256 == 0)
+                p.ws = a->workspace;
+        }
         return few ? launch_paged_few(p, dt, q8, s) : launch_paged_chunk(p, dt, q8, s);
     }
     return launch_paged_f32(p, q8, s);

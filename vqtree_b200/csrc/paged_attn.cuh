@@ -22,8 +22,12 @@ struct PagedAttnParams {
     int max_q;
     float scale_log2;            // softmax scale * log2(e)
     long long wait_limit;
+    void *ws;                    // 8-bit rows: their blocks as 16-bit floats, [pool][ws_blocks][Hkv][128][D]; NULL: none
+    int64_t ws_blocks;
 
     __device__ __forceinline__ int boundary(int i) const { return i > W ? (i - W) / kBlock * kBlock : 0; }
+    // first key block that the query at position i sees one by one
+    __device__ __forceinline__ int first_block(int i) const { return max(0, i / kBlock - W / kBlock); }
     // snapshot of boundary b of sequence s; -1: none is wanted, or the table names none (reported)
     __device__ __forceinline__ int snapshot(int s, int b) const { return checked_snapshot(b, snapshot_entry(s, b)); }
     // the same in two parts: what the table says, and the check
@@ -44,25 +48,35 @@ struct PagedAttnParams {
 // boundary and its snapshot.
 struct ChunkTile {
     int s, t0, ntok, pos0, n, snap;
+    int ws0;                     // workspace block of the sequence's key block 0 (may be negative: early blocks are not there)
 };
 
 // Tile number -> sequence and tokens, by one warp.  False: there are fewer tiles.
 __device__ __forceinline__ bool chunk_find(const PagedAttnParams &p, int TQ, int tile, ChunkTile &out)
 {
     const int lane = threadIdx.x & 31, per = (kBlock + TQ - 1) / TQ;
-    int before = 0;
+    int before = 0, ws_before = 0;
     for (int base = 0; base < p.seqs.S; base += 32) {
-        int t0 = 0, q = 0, n = 0, cnt = 0;
+        int t0 = 0, q = 0, n = 0, cnt = 0, blocks = 0;
         if (base + lane < p.seqs.S && p.seqs.seq(base + lane, t0, q, n, p.max_q) && q > 0) {
             const int i0 = n - q, nb = (n - 1) / kBlock - i0 / kBlock + 1;
             cnt = nb == 1 ? (q + TQ - 1) / TQ
                           : (kBlock - i0 % kBlock + TQ - 1) / TQ + (nb - 2) * per + ((n - 1) % kBlock + TQ) / TQ;
+            blocks = (n - 1) / kBlock - p.first_block(i0) + 1;
         }
         int sum = cnt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(~0u, sum, o);
             if (lane >= o) sum += x;
+        }
+        int ws_sum = blocks;
+        if (p.ws != nullptr) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(~0u, ws_sum, o);
+                if (lane >= o) ws_sum += x;
+            }
         }
         const unsigned mine = __ballot_sync(~0u, before + sum > tile);
         if (mine) {
@@ -86,9 +100,11 @@ __device__ __forceinline__ bool chunk_find(const PagedAttnParams &p, int TQ, int
             out.pos0 = lo;
             out.n = n;
             out.snap = p.snapshot(out.s, p.boundary(lo));
+            out.ws0 = ws_before + __shfl_sync(~0u, ws_sum, l) - __shfl_sync(~0u, blocks, l) - p.first_block(i0);
             return true;
         }
         before += __shfl_sync(~0u, sum, 31);
+        ws_before += __shfl_sync(~0u, ws_sum, 31);
     }
     return false;
 }
@@ -99,6 +115,11 @@ inline int64_t chunk_tiles(const PagedSeqs &q, int TQ)
     const int64_t tiles = q.T / TQ + q.T / kBlock + 2 * static_cast<int64_t>(q.S);
     return tiles < q.T ? tiles : q.T;
 }
+
+// Blocks of 128 keys that the new tokens of a call can see, at most.
+inline int64_t paged_blocks(int64_t S, int64_t T, int64_t window) { return S * (window / kBlock + 3) + T / kBlock; }
+// 8-bit rows: converting a block once per call pays where its keys meet many query tiles: eight per sequence on average.
+inline bool convert_first(int64_t S, int64_t T, int64_t G) { return T * G >= 8 * kBlock * S; }
 
 constexpr int kFewRows = 32;     // query rows (tokens times query heads of a kv head) of the few-token kernel
 int launch_paged_few(const PagedAttnParams &p, int dtype, bool q8, cudaStream_t stream);

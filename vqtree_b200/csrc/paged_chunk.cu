@@ -17,23 +17,26 @@
 #include "paged_attn.cuh"
 #include "tc_softmax.cuh"
 
+#include <type_traits>
+
 namespace vq {
 
 constexpr int kChunkPages = 256;        // page table entries of a tile kept in shared memory; the rest is read where it is needed
 
-template <int D, bool Q8>
+// CONV: 8-bit rows converted on their way into the ring
+template <int D, bool CONV>
 struct ChunkCfg {
     static constexpr int kBufs = 3;                           // S/P buffers = softmax warpgroups
     static constexpr int kSoft = 4 * kBufs;                   // softmax warps
-    static constexpr int kLoad = Q8 ? 3 : 1;                  // loading warps: 16 warps of 128 registers with 8-bit rows
+    static constexpr int kLoad = CONV ? 3 : 1;                  // loading warps: 16 warps of 128 registers with 8-bit rows
     static constexpr int kWarpMma = kSoft, kWarpLoad = kSoft + 1;
     static constexpr int kThreads = (kSoft + 1 + kLoad) * 32;
     static constexpr int NH = D / 64;
     static constexpr int kTile = NH * kHalfBytes;             // 128 x D
-    static constexpr int kSlots = Q8 ? 3 : 4;
+    static constexpr int kSlots = CONV ? 3 : 4;
     static constexpr int kRaw = kBlock * D;                   // 128 rows of codes
     static constexpr int kQ = 0, kRing = 2 * kTile, kRaws = kRing + kSlots * kTile;
-    static constexpr int kTotal = kRaws + (Q8 ? 2 * kRaw : 0) + 1024;   // + slack for 1024-byte alignment
+    static constexpr int kTotal = kRaws + (CONV ? 2 * kRaw : 0) + 1024;   // + slack for 1024-byte alignment
     static constexpr uint32_t kColS = 0, kColO = kBlock * kBufs, kCols = 512;
     static constexpr int kOq = D / 2;
 };
@@ -147,13 +150,17 @@ __device__ __forceinline__ float q8_exp(const uint32_t (&r)[64], uint32_t p_addr
     return sum;
 }
 
-template <int D, bool F16, bool Q8>
-__global__ void __launch_bounds__(ChunkCfg<D, Q8>::kThreads, 1)
+// SRC: where local rows come from
+enum ChunkSrc : int { kPages16 = 0, kPages8 = 1, kWorkspace = 2 };
+
+template <int D, bool F16, int SRC>
+__global__ void __launch_bounds__(ChunkCfg<D, SRC == kPages8>::kThreads, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_constant__ CUtensorMap tm_q2, const __grid_constant__ CUtensorMap tm_k1,
                    const __grid_constant__ CUtensorMap tm_k3, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_cb,
                    const __grid_constant__ CUtensorMap tm_vs, const ChunkParams cp)
 {
-    using C = ChunkCfg<D, Q8>;
+    constexpr bool Q8 = SRC != kPages16, CONV = SRC == kPages8;
+    using C = ChunkCfg<D, CONV>;
     using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
     constexpr int NH = C::NH, NS = C::kSlots, NB = C::kBufs, kSoftThreads = C::kSoft * 32;
     const PagedAttnParams &p = cp.a;
@@ -269,10 +276,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
                 __syncwarp();
             }
         };
-        if constexpr (!Q8) {
+        if constexpr (!CONV) {
             auto load = [&](int it, bool is_v) {
                 if (!ok) return;
-                const int kind = work.kind(it), mine = kind == kFar ? -1 : page_of_lane(it);   // known before the slot is free
+                const int kind = work.kind(it), mine = kind == kFar || SRC == kWorkspace ? -1 : page_of_lane(it);   // known before the slot is free
                 const int bytes = __popc(__ballot_sync(~0u, mine >= 0)) * page_size * D * 2;
                 if (!__all_sync(~0u, wait_slot())) {
                     ok = false;
@@ -284,6 +291,17 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
                 } else {
                     const CUtensorMap *tm = is_v ? &tm_v : (kind == kBdA ? &tm_k3 : &tm_k1);
                     uint8_t *dst = smem + C::kRing + slot * C::kTile;
+                    if (SRC == kWorkspace) {
+                        if (elect_one()) {
+                            const int z = (tile.ws0 + work.block(it)) * p.Hkv + hk;
+                            mbar_expect_tx(&kv_full[slot], C::kTile);
+#pragma unroll
+                            for (int h = 0; h < NH; ++h) tma_load_3d(dst + h * kHalfBytes, tm, &kv_full[slot], 64 * h, 0, z);
+                        }
+                        __syncwarp();
+                        advance();
+                        return;
+                    }
                     if (elect_one()) mbar_expect_tx(&kv_full[slot], bytes);
                     __syncwarp();
                     each_page(mine, [&](int pg, int x) {
@@ -610,7 +628,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
                 }
             }
             l_part += ls;
-            if (!Q8 && it == n - 1) {
+            if (SRC == kPages16 && it == n - 1) {
                 // The value rows behind the sequence's end: the weights there are zero, what the page holds need not be a number.
                 const int valid = tile.n - tile.pos0 / kBlock * kBlock;
                 if (valid < kBlock) {
@@ -728,34 +746,140 @@ static bool map_pool(CUtensorMap *out, const PagedPool &pool, const PagedAttnPar
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, bool F16, bool Q8>
+// Blocks of 128 keys of a call's sequences, from the first that a new token sees on: codes -> 16-bit floats (exact; half values times the power of two
+// that goes with their block's largest scale), rows behind the end -> zeros.  A CTA per block, kv head and pool; bound by memory traffic.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) convert_blocks_kernel(const PagedAttnParams p)
+{
+    __shared__ int s_seq, s_blk, s_n, s_last;
+    __shared__ float s_max[4];
+    const int tid = threadIdx.x, lane = tid & 31, hk = blockIdx.y, pool_id = blockIdx.z;      // 0: k1, 1: v, 2: k3
+    if (tid < 32) {
+        int before = 0, seq = -1, blk = 0, len = 0, last = 0;
+        for (int base = 0; base < p.seqs.S; base += 32) {
+            int t0 = 0, q = 0, n = 0, blocks = 0, first = 0;
+            if (base + lane < p.seqs.S && p.seqs.seq(base + lane, t0, q, n, p.max_q) && q > 0) {
+                first = p.first_block(n - q);
+                blocks = (n - 1) / kBlock - first + 1;
+            }
+            int sum = blocks;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(~0u, sum, o);
+                if (lane >= o) sum += x;
+            }
+            const unsigned mine = __ballot_sync(~0u, before + sum > static_cast<int>(blockIdx.x));
+            if (mine) {
+                const int l = __ffs(mine) - 1;
+                seq = base + l;
+                blk = __shfl_sync(~0u, first, l) + static_cast<int>(blockIdx.x) - (before + __shfl_sync(~0u, sum, l) - __shfl_sync(~0u, blocks, l));
+                len = __shfl_sync(~0u, n, l);
+                last = (len - 1) / kBlock;
+                break;
+            }
+            before += __shfl_sync(~0u, sum, 31);
+        }
+        if (lane == 0) {
+            s_seq = seq;
+            s_blk = blk;
+            s_n = len;
+            s_last = last;
+        }
+    }
+    __syncthreads();
+    const int seq = s_seq, blk = s_blk, n = s_n;
+    if (seq < 0 || (pool_id == 2 && blk > s_last - p.W / kBlock)) return;      // raw keys: those before somebody's exact window
+    const PagedPool &pool = pool_id == 0 ? p.k1 : pool_id == 1 ? p.v : p.k3;
+    const int page_mask = (1 << p.seqs.log_p) - 1;
+    float mul = 1.f;
+    if constexpr (!IsBf16<T>::value) {
+        if (pool_id == 1) {
+            if (tid < kBlock) {
+                const int key = blk * kBlock + tid, page = key < n ? p.seqs.page(seq, key >> p.seqs.log_p) : -1;
+                float x = page >= 0 ? __ldg(pool.scale + pool.scale_at(page, hk, key & page_mask)) : 0.f;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
+                if (lane == 0) s_max[tid >> 5] = x;
+            }
+            __syncthreads();
+            mul = pow2f(-half_weight_shift(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]))));
+        }
+    }
+    T *dst = static_cast<T *>(p.ws) + ((pool_id * p.ws_blocks + blockIdx.x) * p.Hkv + hk) * (kBlock * D);
+    constexpr int CH = D / 16;
+#pragma unroll
+    for (int x = tid; x < kBlock * CH; x += 256) {
+        const int row = x / CH, c = x % CH * 16, key = blk * kBlock + row;
+        uint4 codes = make_uint4(0, 0, 0, 0), a, b;
+        const int page = key < n ? p.seqs.page(seq, key >> p.seqs.log_p) : -1;
+        if (page >= 0) codes = *reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(pool.ptr) + pool.row(page, hk, key & page_mask) + c);
+        if constexpr (IsBf16<T>::value) {
+            Codes8<T>::expand(codes.x, a.x, a.y);
+            Codes8<T>::expand(codes.y, a.z, a.w);
+            Codes8<T>::expand(codes.z, b.x, b.y);
+            Codes8<T>::expand(codes.w, b.z, b.w);
+        } else {
+            const __half2 m2 = __float2half2_rn(mul);
+            Codes8<T>::expand_scaled(codes.x, m2, a.x, a.y);
+            Codes8<T>::expand_scaled(codes.y, m2, a.z, a.w);
+            Codes8<T>::expand_scaled(codes.z, m2, b.x, b.y);
+            Codes8<T>::expand_scaled(codes.w, m2, b.z, b.w);
+        }
+        *reinterpret_cast<uint4 *>(dst + row * D + c) = a;
+        *reinterpret_cast<uint4 *>(dst + row * D + c + 8) = b;
+    }
+}
+
+template <int D, bool F16, int SRC>
 static int launch_chunk(const PagedAttnParams &a, cudaStream_t stream)
 {
-    using C = ChunkCfg<D, Q8>;
+    using C = ChunkCfg<D, SRC == kPages8>;
+    using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
     ChunkParams cp;
     cp.a = a;
+    if (SRC != kWorkspace) cp.a.ws = nullptr;
     cp.TQ = kBlock / a.G;
     TcMaps m;
     if (!map_tokens(&m.q1, a.q1, a.seqs.T, a, a.q1_t, a.q1_h, cp.TQ, F16) || !map_tokens(&m.q2, a.q2, a.seqs.T, a, a.q2_t, a.q2_h, cp.TQ, F16)) return VQ_ELAUNCH;
-    if (!map_pool<Q8>(&m.k1, a.k1, a, F16) || !map_pool<Q8>(&m.k3, a.k3, a, F16) || !map_pool<Q8>(&m.v, a.v, a, F16)) return VQ_ELAUNCH;
+    if (SRC == kWorkspace) {
+        const uint64_t wd[3] = {D, kBlock, static_cast<uint64_t>(a.ws_blocks) * a.Hkv}, wst[3] = {1, D, kBlock * D};
+        const int64_t per = a.ws_blocks * a.Hkv * (kBlock * D);
+        T *ws = static_cast<T *>(a.ws);
+        if (!make_map(&m.k1, ws, 3, wd, wst, kBlock, F16) || !make_map(&m.v, ws + per, 3, wd, wst, kBlock, F16) ||
+            !make_map(&m.k3, a.rerope ? ws + 2 * per : ws, 3, wd, wst, kBlock, F16))
+            return VQ_ELAUNCH;
+        const dim3 grid(static_cast<unsigned>(a.ws_blocks), static_cast<unsigned>(a.Hkv), a.rerope ? 3u : 2u);
+        convert_blocks_kernel<T, D><<<grid, 256, 0, stream>>>(cp.a);
+        const int st = launch_status();
+        if (st != VQ_OK) return st;
+    } else if (!map_pool<SRC != kPages16>(&m.k1, a.k1, a, F16) || !map_pool<SRC != kPages16>(&m.k3, a.k3, a, F16) ||
+               !map_pool<SRC != kPages16>(&m.v, a.v, a, F16)) {
+        return VQ_ELAUNCH;
+    }
     if (a.cb != nullptr) {
         const uint64_t MK = a.MK, cd[3] = {D, MK, static_cast<uint64_t>(a.Hkv)}, cs[3] = {1, D, MK * D}, vd[3] = {D, MK, static_cast<uint64_t>(a.NS) * a.Hkv};
         if (!make_map(&m.cb, a.cb, 3, cd, cs, kBlock, F16) || !make_map(&m.vs, a.vsum, 3, vd, cs, kBlock, F16)) return VQ_ELAUNCH;
     } else {
         m.cb = m.vs = m.q1;         // never read: no tile has codes
     }
-    auto kern = paged_chunk_kernel<D, F16, Q8>;
+    auto kern = paged_chunk_kernel<D, F16, SRC>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kTotal) != cudaSuccess) return VQ_ELAUNCH;
     const int64_t tiles = chunk_tiles(a.seqs, cp.TQ);
     kern<<<dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.Hkv)), C::kThreads, C::kTotal, stream>>>(m.q1, m.q2, m.k1, m.k3, m.v, m.cb, m.vs, cp);
     return launch_status();
 }
 
+template <int D, bool F16>
+static int launch_chunk_src(const PagedAttnParams &p, bool q8, cudaStream_t stream)
+{
+    if (!q8) return launch_chunk<D, F16, kPages16>(p, stream);
+    return p.ws != nullptr ? launch_chunk<D, F16, kWorkspace>(p, stream) : launch_chunk<D, F16, kPages8>(p, stream);
+}
+
 template <bool F16>
 static int launch_chunk_type(const PagedAttnParams &p, bool q8, cudaStream_t stream)
 {
-    if (p.D == 64) return q8 ? launch_chunk<64, F16, true>(p, stream) : launch_chunk<64, F16, false>(p, stream);
-    return q8 ? launch_chunk<128, F16, true>(p, stream) : launch_chunk<128, F16, false>(p, stream);
+    return p.D == 64 ? launch_chunk_src<64, F16>(p, q8, stream) : launch_chunk_src<128, F16>(p, q8, stream);
 }
 
 int launch_paged_chunk(const PagedAttnParams &p, int dtype, bool q8, cudaStream_t stream)

@@ -275,7 +275,7 @@ int64_t paged_attention_status(const at::Tensor &q1, const at::Tensor &q2, const
                                const OptTensor &k1_scale, const OptTensor &v_scale, const OptTensor &k3_scale, const at::Tensor &table,
                                const at::Tensor &cu_q, const at::Tensor &lens, const OptTensor &codebook, const OptTensor &cnt,
                                const OptTensor &vsum, const OptTensor &snap_table, int64_t window, int64_t max_q, double scale, at::Tensor out,
-                               const OptTensor &status_word)
+                               const OptTensor &workspace, const OptTensor &status_word)
 {
     if (!q1.is_cuda()) return VQ_EDEVICE;
     const c10::cuda::CUDAGuard guard(q1.device());
@@ -287,7 +287,19 @@ int64_t paged_attention_status(const at::Tensor &q1, const at::Tensor &q2, const
     a.max_q = max_q;
     a.scale = static_cast<float>(scale);
     a.status_word = word_of(status_word);
+    const Workspace ws(workspace);
+    a.workspace = ws.ptr;
+    a.workspace_bytes = ws.bytes;
     return vqattn_paged_attention(&a, stream_of(q1));
+}
+
+// a workspace for the call, undefined where it would use none
+OptTensor paged_workspace(const at::Tensor &q1, const at::Tensor &k1, const at::Tensor &table, int64_t window, int64_t max_q)
+{
+    if (k1.scalar_type() != at::kChar || q1.dim() != 3 || k1.dim() != 4 || table.dim() != 2 || !q1.is_cuda()) return {};
+    const size_t n = vqattn_paged_attention_workspace_bytes(table.size(0), q1.size(0), q1.size(1), k1.size(1), q1.size(2), window, max_q, VQ_I8,
+                                                            dtype_of(q1));
+    return n ? OptTensor(at::empty({static_cast<int64_t>(n)}, q1.options().dtype(at::kByte))) : OptTensor();
 }
 
 std::tuple<at::Tensor, at::Tensor, int64_t> paged_append_new(const at::Tensor &k, const at::Tensor &v, at::Tensor k1, at::Tensor v_pages,
@@ -330,7 +342,7 @@ std::tuple<at::Tensor, int64_t> paged_attention_new(const at::Tensor &q1, const 
 {
     const at::Tensor out = at::empty(q1.sizes(), q1.options());
     return {out, paged_attention_status(q1, q2, k1, v_pages, k3, k1_scale, v_scale, k3_scale, table, cu_q, lens, codebook, cnt, vsum, snap_table, window,
-                                        max_q, scale, out, status_word)};
+                                        max_q, scale, out, paged_workspace(q1, k1, table, window, max_q), status_word)};
 }
 
 // the raising forms
@@ -338,6 +350,13 @@ template <auto F> struct Raising;
 template <typename... A, int64_t (*F)(A...)> struct Raising<F> {
     static void call(A... args) { check(static_cast<int>(F(std::forward<A>(args)...)), "vqattn::paged"); }
 };
+
+int64_t paged_attention_workspace_bytes(int64_t S, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window, int64_t max_q,
+                                        at::ScalarType pool, at::ScalarType act)
+{
+    auto code = [](at::ScalarType t) { return t == at::kChar ? VQ_I8 : t == at::kBFloat16 ? VQ_BF16 : t == at::kHalf ? VQ_F16 : VQ_F32; };
+    return static_cast<int64_t>(vqattn_paged_attention_workspace_bytes(S, T, Hq, Hkv, D, window, max_q, code(pool), code(act)));
+}
 
 int64_t abi_version() { return vqattn_version(); }
 
@@ -349,6 +368,8 @@ TORCH_LIBRARY(vqattn, m)
     m.def("assign_workspace_bytes(int B, int Hkv, int L, int M, int K, int D) -> int", &assign_workspace_bytes);
     m.def("aggregates_workspace_bytes(int B, int Hkv, int NB, int M, int K) -> int", &aggregates_workspace_bytes);
     m.def("decode_workspace_bytes(int B, int Hq, int Hkv, int D) -> int", &decode_workspace_bytes);
+    m.def("paged_attention_workspace_bytes(int S, int T, int Hq, int Hkv, int D, int window, int max_q, ScalarType pool, ScalarType act) -> int",
+          &paged_attention_workspace_bytes);
     m.def("assign_codes(Tensor k, Tensor codebooks, Tensor? bias, Tensor(a!) codes, Tensor(b!)? workspace, Tensor(c!)? status_word) -> ()");
     m.def("build_aggregates(Tensor codes, Tensor v, int K, Tensor(a!) cnt, Tensor(b!) vsum, Tensor(c!)? state_cnt, Tensor(d!)? state_vsum, "
           "int state_blocks, Tensor(e!)? workspace, Tensor(f!)? status_word) -> ()");
@@ -370,10 +391,10 @@ TORCH_LIBRARY(vqattn, m)
           "Tensor(c!)? out2, Tensor table, Tensor start, Tensor lens, Tensor(d!)? status_word) -> int");
     m.def("paged_attention(Tensor q1, Tensor q2, Tensor k1, Tensor v_pages, Tensor? k3, Tensor? k1_scale, Tensor? v_scale, Tensor? k3_scale, Tensor table, "
           "Tensor cu_q, Tensor lens, Tensor? codebook, Tensor? cnt, Tensor? vsum, Tensor? snap_table, int window, int max_q, float scale, "
-          "Tensor(a!) out, Tensor(b!)? status_word) -> ()");
+          "Tensor(a!) out, Tensor(b!)? workspace, Tensor(c!)? status_word) -> ()");
     m.def("paged_attention_status(Tensor q1, Tensor q2, Tensor k1, Tensor v_pages, Tensor? k3, Tensor? k1_scale, Tensor? v_scale, Tensor? k3_scale, Tensor table, "
           "Tensor cu_q, Tensor lens, Tensor? codebook, Tensor? cnt, Tensor? vsum, Tensor? snap_table, int window, int max_q, float scale, "
-          "Tensor(a!) out, Tensor(b!)? status_word) -> int");
+          "Tensor(a!) out, Tensor(b!)? workspace, Tensor(c!)? status_word) -> int");
     m.def("paged_append_new(Tensor k, Tensor v, Tensor(a!) k1, Tensor(b!) v_pages, Tensor(c!)? k3, Tensor(d!)? k1_scale, Tensor(e!)? v_scale, "
           "Tensor(f!)? k3_scale, Tensor table, Tensor cu_q, Tensor lens, Tensor q, bool two, Tensor? cos_tab, Tensor? sin_tab, int const_pos, "
           "Tensor(g!)? status_word) -> (Tensor, Tensor, int)");

@@ -38,7 +38,7 @@ EXPORTS = (
     "vqattn_assign_workspace_bytes", "vqattn_assign_codes_ws", "vqattn_rope",
     "vqattn_status_from_word", "vqattn_set_wait_limit_cycles", "vqattn_wait_selftest", "vqattn_rope_qk",
     "vqattn_decode_append", "vqattn_decode_step", "vqattn_store_window",
-    "vqattn_paged_append", "vqattn_paged_read", "vqattn_paged_attention",
+    "vqattn_paged_append", "vqattn_paged_read", "vqattn_paged_attention", "vqattn_paged_attention_workspace_bytes",
 )
 
 
@@ -98,7 +98,8 @@ class VqPagedReadArgs(ctypes.Structure):
 
 class VqPagedAttentionArgs(ctypes.Structure):
     _fields_ = [("kv", VqPagedKv)] + [(n, VqTensorDesc) for n in ("q1", "q2", "out", "codebook", "cnt", "vsum", "snap_table")] + [
-        ("window", ctypes.c_int64), ("max_q", ctypes.c_int64), ("scale", ctypes.c_float), ("status_word", ctypes.c_void_p)]
+        ("window", ctypes.c_int64), ("max_q", ctypes.c_int64), ("scale", ctypes.c_float), ("status_word", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 def _load() -> ctypes.CDLL:
@@ -148,6 +149,8 @@ def _load() -> ctypes.CDLL:
     lib.vqattn_paged_append.argtypes = [P(VqPagedAppendArgs), ctypes.c_void_p]
     lib.vqattn_paged_read.argtypes = [P(VqPagedReadArgs), ctypes.c_void_p]
     lib.vqattn_paged_attention.argtypes = [P(VqPagedAttentionArgs), ctypes.c_void_p]
+    lib.vqattn_paged_attention_workspace_bytes.argtypes = [ctypes.c_int64] * 7 + [ctypes.c_int32] * 2
+    lib.vqattn_paged_attention_workspace_bytes.restype = ctypes.c_size_t
     lib.vqattn_status_from_word.argtypes = [ctypes.c_int32]
     lib.vqattn_set_wait_limit_cycles.argtypes = [ctypes.c_int64]
     lib.vqattn_set_wait_limit_cycles.restype = ctypes.c_int64
@@ -156,7 +159,8 @@ def _load() -> ctypes.CDLL:
                                 P(VqTensorDesc), P(VqTensorDesc), ctypes.c_void_p, ctypes.c_void_p]
     for name in EXPORTS:
         if name not in ("vqattn_status_string", "vqattn_decode_workspace_bytes", "vqattn_decode_static_capacity",
-                        "vqattn_assign_workspace_bytes", "vqattn_aggregates_workspace_bytes", "vqattn_set_wait_limit_cycles"):
+                        "vqattn_assign_workspace_bytes", "vqattn_aggregates_workspace_bytes", "vqattn_set_wait_limit_cycles",
+                        "vqattn_paged_attention_workspace_bytes"):
             getattr(lib, name).restype = ctypes.c_int
     return lib
 

@@ -21,9 +21,10 @@ that kernels raise on an expired bounded wait or a bad code):
                  const_pos, status_word?)
     paged_read(pool0, scale0?, out0!, pool1?, scale1?, out1!?, pool2?, scale2?, out2!?, table, start, lens, status_word?)
     paged_attention(q1, q2, k1, v_pages, k3?, k1_scale?, v_scale?, k3_scale?, table, cu_q, lens, codebook?, cnt?, vsum?, snap_table?,
-                    window, max_q, scale, out!, status_word?)
+                    window, max_q, scale, out!, workspace!?, status_word?)
     paged_*_status(...): the same, returning the C status instead of raising; paged_*_new(...): that, and the outputs allocated
-    abi_version(), assign_workspace_bytes(...), aggregates_workspace_bytes(...), decode_workspace_bytes(...)
+    abi_version(), assign_workspace_bytes(...), aggregates_workspace_bytes(...), decode_workspace_bytes(...),
+    paged_attention_workspace_bytes(S, T, Hq, Hkv, D, window, max_q, pool dtype, activations' dtype)
 """
 from __future__ import annotations
 
