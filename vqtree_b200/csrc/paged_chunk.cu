@@ -100,25 +100,37 @@ __device__ __forceinline__ float warp_max4(const float (&x)[4])
     return m;
 }
 
-// 8-bit rows: scores of 64 columns in log2 units (ks: scale of each key times the softmax scale), excluded ones -inf
-__device__ __forceinline__ void q8_scores(uint32_t s_addr, int kind, int lo, int hi, const float *ks, uint32_t (&r)[64])
+// 8-bit rows.  ks: scale of each of 64 keys times the softmax scale, vs: factor of each value row.
+__device__ __forceinline__ void load_scores(uint32_t s_addr, uint32_t (&r)[64])
 {
     tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
     tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
     tc_wait_ld();
+}
+// the largest score, in log2 units; [lo, hi): the columns that count
+template <bool MASKED>
+__device__ __forceinline__ float q8_max(const uint32_t (&r)[64], int lo, int hi, const float *ks)
+{
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int c = 0; c < 64; c += 4) {
         const float4 k = *reinterpret_cast<const float4 *>(ks + c);
-        float x0, x1, x2, x3;
-        fmul2(x0, x1, __uint_as_float(r[c]), __uint_as_float(r[c + 1]), k.x, k.y);
-        fmul2(x2, x3, __uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]), k.z, k.w);
-        r[c] = __float_as_uint(x0); r[c + 1] = __float_as_uint(x1); r[c + 2] = __float_as_uint(x2); r[c + 3] = __float_as_uint(x3);
+        float x[4];
+        fmul2(x[0], x[1], __uint_as_float(r[c]), __uint_as_float(r[c + 1]), k.x, k.y);
+        fmul2(x[2], x[3], __uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]), k.z, k.w);
+        if (MASKED) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < lo || c + i >= hi) x[i] = -INFINITY;
+        }
+        mx[(c >> 2) & 3] = fmax3(mx[(c >> 2) & 3], x[0], x[1]);
+        mx[((c >> 2) + 1) & 3] = fmax3(mx[((c >> 2) + 1) & 3], x[2], x[3]);
     }
-    if (kind != kFull) t4_mask_range(r, lo, hi);
+    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
-// weights times value scales (vs), packed; returns sum plus the weights
-template <bool F16>
-__device__ __forceinline__ float q8_exp(const uint32_t (&r)[64], uint32_t p_addr, bool masked, const float *vs, float neg_m, float sum)
+// weights times value factors, packed 16-bit floats; returns sum plus the weights.  What does not count weighs nothing, whatever its value is.
+template <bool F16, bool MASKED>
+__device__ __forceinline__ float q8_exp(const uint32_t (&r)[64], uint32_t p_addr, int lo, int hi, const float *ks, const float *vs, float neg_m, float sum)
 {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -127,20 +139,20 @@ __device__ __forceinline__ float q8_exp(const uint32_t (&r)[64], uint32_t p_addr
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int c = 32 * half + 4 * j;
-            const float4 v4 = *reinterpret_cast<const float4 *>(vs + c);
-            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+            const float4 k4 = *reinterpret_cast<const float4 *>(ks + c), v4 = *reinterpret_cast<const float4 *>(vs + c);
+            const float k[4] = {k4.x, k4.y, k4.z, k4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float r0 = __uint_as_float(r[c + 2 * i]), r1 = __uint_as_float(r[c + 2 * i + 1]);
                 float t0, t1, w0, w1;
-                fadd2(t0, t1, r0, r1, neg_m, neg_m);
-                const float p0 = ex2(t0), p1 = ex2(t1);
+                ffma2(t0, t1, __uint_as_float(r[c + 2 * i]), __uint_as_float(r[c + 2 * i + 1]), k[2 * i], k[2 * i + 1], neg_m, neg_m);
+                float p0 = ex2(t0), p1 = ex2(t1);
+                const bool out0 = MASKED && (c + 2 * i < lo || c + 2 * i >= hi), out1 = MASKED && (c + 2 * i + 1 < lo || c + 2 * i + 1 >= hi);
+                if (out0) p0 = 0.f;
+                if (out1) p1 = 0.f;
                 fadd2(ls[2 * i], ls[2 * i + 1], ls[2 * i], ls[2 * i + 1], p0, p1);
                 fmul2(w0, w1, p0, p1, v[2 * i], v[2 * i + 1]);
-                if (masked) {                                 // a value that is not finite must not reach rows that do not see it
-                    if (r0 == -INFINITY) w0 = 0.f;
-                    if (r1 == -INFINITY) w1 = 0.f;
-                }
+                if (out0) w0 = 0.f;
+                if (out1) w1 = 0.f;
                 pk[2 * j + i] = pack16<F16>(w0, w1);
             }
         }
@@ -574,8 +586,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
 #pragma unroll
             for (int c = 0; c < kBlock; c += 64) {
                 if (Q8 && q8) {
-                    q8_scores(sa + c, kind, lo - c, hi - c, cw + c, r);
-                    mx = fmaxf(mx, t4_max(r));
+                    load_scores(sa + c, r);
+                    mx = fmaxf(mx, kind == kFull ? q8_max<false>(r, 0, 64, cw + c) : q8_max<true>(r, lo - c, hi - c, cw + c));
                 } else {
                     t4_scores(sa + c, kind, has_empty, lo - c, hi - c, cw + c, r);
                     mx = fmaxf(mx, t4_max(r));
@@ -619,8 +631,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
 #pragma unroll
             for (int c = 0; c < kBlock; c += 64) {
                 if (Q8 && q8) {
-                    q8_scores(sa + c, kind, lo - c, hi - c, cw + c, r);
-                    ls = q8_exp<F16>(r, sa + c / 2, kind != kFull, cv + c, -m_safe, ls);
+                    load_scores(sa + c, r);
+                    ls = kind == kFull ? q8_exp<F16, false>(r, sa + c / 2, 0, 64, cw + c, cv + c, -m_safe, ls)
+                                       : q8_exp<F16, true>(r, sa + c / 2, lo - c, hi - c, cw + c, cv + c, -m_safe, ls);
                 } else {
                     t4_scores(sa + c, kind, has_empty, lo - c, hi - c, cw + c, r);
                     ls = kind == kFar ? t4_exp<true, F16>(r, sa + c / 2, cw + c, p.scale_log2, -m_safe, ls)
