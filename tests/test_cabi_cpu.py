@@ -176,8 +176,8 @@ def test_paged_entry_points_refuse_bad_arguments_without_a_device():
 
 def test_paged_attention_workspace_size():
     ws = _native().lib.vqattn_paged_attention_workspace_bytes
-    # six sequences, 2228 new tokens of 4 query heads per kv head: three pools of 6 * (8 + 3) + 17 blocks of 128 rows
-    assert ws(6, 2228, 32, 8, 128, 1024, 597, 7, 1) == 3 * (6 * 11 + 17) * 8 * 128 * 128 * 2
+    # six sequences, 2228 new tokens of 4 query heads per kv head: three pools of 6 * (8 + 3) + 17 blocks of 128 rows and factors
+    assert ws(6, 2228, 32, 8, 128, 1024, 597, 7, 1) == 3 * (6 * 11 + 17) * 8 * 128 * (128 * 2 + 4)
     assert ws(6, 2228, 32, 8, 128, 1024, 597, 1, 1) == 0            # rows of 16 bits
     assert ws(6, 2228, 32, 8, 128, 1024, 597, 7, 0) == 0            # full precision
     assert ws(64, 2228, 32, 8, 128, 1024, 597, 7, 1) == 0           # few tiles per sequence

@@ -13,8 +13,8 @@ static bool few_form(int64_t max_q, int64_t G, int64_t D, bool q8, int64_t units
     return rows <= 16 || (rows <= kFewRows && (q8 || D == 64 || units <= sms));
 }
 
-// three pools of blocks as 16-bit floats
-static size_t workspace_bytes(int64_t blocks, int64_t Hkv, int64_t D) { return static_cast<size_t>(3 * blocks * Hkv * kBlock * D * 2); }
+// three pools of blocks as 16-bit floats, a factor per row
+static size_t workspace_bytes(int64_t blocks, int64_t Hkv, int64_t D) { return static_cast<size_t>(3 * blocks * Hkv * kBlock * (D * 2 + 4)); }
 
 }  // namespace vq
 

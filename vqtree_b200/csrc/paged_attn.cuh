@@ -22,10 +22,12 @@ struct PagedAttnParams {
     int max_q;
     float scale_log2;            // softmax scale * log2(e)
     long long wait_limit;
-    void *ws;                    // 8-bit rows: their blocks as 16-bit floats, [pool][ws_blocks][Hkv][128][D]; NULL: none
+    // 8-bit rows: their blocks as 16-bit floats, [k1, v, k3][ws_blocks][Hkv][128][D], and behind them a factor per row; NULL: none
+    void *ws;
     int64_t ws_blocks;
 
     __device__ __forceinline__ int boundary(int i) const { return i > W ? (i - W) / kBlock * kBlock : 0; }
+    __device__ __forceinline__ float *ws_scales(int64_t row_bytes) const { return reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + row_bytes); }
     // first key block that the query at position i sees one by one
     __device__ __forceinline__ int first_block(int i) const { return max(0, i / kBlock - W / kBlock); }
     // snapshot of boundary b of sequence s; -1: none is wanted, or the table names none (reported)

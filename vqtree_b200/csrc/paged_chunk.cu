@@ -535,6 +535,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
             if (it < work.n_far) {
 #pragma unroll
                 for (int i = 0; i < NCW; ++i) reg_w[i] = __ldg(cnt_base + it * kBlock + 32 * i);
+            } else if constexpr (SRC == kWorkspace) {
+                if (it >= n) return;
+                const float *f = p.ws_scales(3 * p.ws_blocks * p.Hkv * (kBlock * D * 2)) + (static_cast<int64_t>(tile.ws0 + work.block(it)) * p.Hkv + hk) * kBlock + lane;
+                const int64_t pool = p.ws_blocks * p.Hkv * kBlock, from = work.kind(it) == kBdA ? 2 * pool : 0;
+#pragma unroll
+                for (int i = 0; i < NCW; ++i) {
+                    reg_w[i] = __ldg(f + from + 32 * i);
+                    reg_v[i] = __ldg(f + pool + 32 * i);
+                }
             } else if constexpr (Q8) {
                 if (it >= n) return;
                 const bool old = work.kind(it) == kBdA;
@@ -559,7 +568,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
                 __syncwarp();
                 bool full = true;
                 float mul = 1.f;                              // half weights: see half_weight_shift
-                if constexpr (Q8 && F16)
+                if constexpr (CONV && F16)
                     if (kind != kFar) mul = pow2f(half_weight_shift(warp_max4(reg_v)));
 #pragma unroll
                 for (int i = 0; i < NCW; ++i) {
@@ -567,8 +576,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
                         cw[32 * i + lane] = reg_w[i];
                         full = full && reg_w[i] > 0.f;
                     } else if constexpr (Q8) {
-                        cw[32 * i + lane] = reg_w[i] * p.scale_log2;
-                        cv[32 * i + lane] = F16 ? reg_v[i] * mul : reg_v[i];
+                        cw[32 * i + lane] = CONV ? reg_w[i] * p.scale_log2 : reg_w[i];
+                        cv[32 * i + lane] = CONV && F16 ? reg_v[i] * mul : reg_v[i];
                     }
                 }
                 has_empty = kind == kFar && __any_sync(kAll, !full);
@@ -818,7 +827,13 @@ __global__ void __launch_bounds__(256) convert_blocks_kernel(const PagedAttnPara
             mul = pow2f(-half_weight_shift(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]))));
         }
     }
-    T *dst = static_cast<T *>(p.ws) + ((pool_id * p.ws_blocks + blockIdx.x) * p.Hkv + hk) * (kBlock * D);
+    const int64_t at = (pool_id * p.ws_blocks + blockIdx.x) * p.Hkv + hk;
+    if (tid < kBlock) {                                      // what multiplies the scores of a key, or the weights of a value
+        const int key = blk * kBlock + tid, page = key < n ? p.seqs.page(seq, key >> p.seqs.log_p) : -1;
+        const float x = page >= 0 ? __ldg(pool.scale + pool.scale_at(page, hk, key & page_mask)) : 0.f;
+        p.ws_scales(3 * p.ws_blocks * p.Hkv * (kBlock * D * 2))[at * kBlock + tid] = pool_id == 1 ? x * (1.f / mul) : x * p.scale_log2;
+    }
+    T *dst = static_cast<T *>(p.ws) + at * (kBlock * D);
     constexpr int CH = D / 16;
 #pragma unroll
     for (int x = tid; x < kBlock * CH; x += 256) {
