@@ -180,5 +180,6 @@ def test_paged_attention_workspace_size():
     assert ws(6, 2228, 32, 8, 128, 1024, 597, 7, 1) == 3 * (6 * 11 + 17) * 8 * 128 * (128 * 2 + 4)
     assert ws(6, 2228, 32, 8, 128, 1024, 597, 1, 1) == 0            # rows of 16 bits
     assert ws(6, 2228, 32, 8, 128, 1024, 597, 7, 0) == 0            # full precision
-    assert ws(64, 2228, 32, 8, 128, 1024, 597, 7, 1) == 0           # few tiles per sequence
+    assert ws(17, 2228, 32, 8, 128, 1024, 597, 7, 1) > 0
+    assert ws(18, 2228, 32, 8, 128, 1024, 597, 7, 1) == 0           # fewer than four tiles per sequence
     assert ws(1, 4, 32, 8, 128, 1024, 4, 7, 1) == 0 and ws(0, 0, 0, 0, 0, 0, 0, 7, 1) == 0 and ws(-1, 9, 4, 4, 128, 128, 9, 7, 1) == 0

@@ -120,8 +120,11 @@ inline int64_t chunk_tiles(const PagedSeqs &q, int TQ)
 
 // Blocks of 128 keys that the new tokens of a call can see, at most.
 inline int64_t paged_blocks(int64_t S, int64_t T, int64_t window) { return S * (window / kBlock + 3) + T / kBlock; }
-// 8-bit rows: converting a block once per call pays where its keys meet many query tiles: eight per sequence on average.
-inline bool convert_first(int64_t S, int64_t T, int64_t G) { return T * G >= 8 * kBlock * S; }
+// 8-bit rows: converting a block once per call pays where its keys meet several query tiles.  Measured, us, first / on the way, 32 query heads over 8,
+// D = 128, MK1024, window 2048 (512), new tokens per sequence: 2 tiles each, 8 sequences 131 / 160 (80 / 83); 4 tiles, 8 sequences 176 / 238 (109 /
+// 122), 24 sequences 414 / 561 (255 / 291); 16 tiles, 2 sequences 118 / 166 (77 / 88).  The line is at four: below it the workspace grows
+// faster than what it saves.
+inline bool convert_first(int64_t S, int64_t T, int64_t G) { return T * G >= 4 * kBlock * S; }
 
 constexpr int kFewRows = 32;     // query rows (tokens times query heads of a kv head) of the few-token kernel
 int launch_paged_few(const PagedAttnParams &p, int dtype, bool q8, cudaStream_t stream);
