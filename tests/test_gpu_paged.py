@@ -240,6 +240,23 @@ def test_attention_values_of_any_size(api, dtype, size, q8, qs, lens):
     assert ((got - ref).abs() <= tol).all(), float(((got - ref).abs() / tol).max())
 
 
+@pytest.mark.parametrize("D,heads", [(64, 32), (128, 2)])
+def test_attention_fp32_sums_over_long_windows_keep_their_bits(api, D, heads):
+    """Queries of zeros weigh every key by exactly 1, so the result is the value itself.  Column d's values are 1 + 0.4 * 2^-(d % 16): added one
+    by one to a sum near 2^12 each loses 0.4 of the sum's last bits, the same way every time, up to 2^-13 of the result.  Sums of 32 that are
+    then added up round 32 + 4128 / 32 times, plus the division: 2^-24 each at the most."""
+    n, q, W, P, S = 4128, 32, 4096, 64, 8
+    col = (1 + 0.4 * 2.0 ** -(torch.arange(D) % 16).float()).cuda()
+    pool = col.expand(-(-n // P), heads, P, D).contiguous()
+    table = torch.arange(-(-n // P), dtype=torch.int32, device="cuda").repeat(S, 1)
+    cu_q = torch.arange(0, (S + 1) * q, q, dtype=torch.int32, device="cuda")
+    lens = torch.full((S,), n, dtype=torch.int32, device="cuda")
+    zero = torch.zeros(S * q, heads, D, device="cuda")
+    got = api.paged_attention(zero, zero, api.PagedKV(pool, pool), table, cu_q, lens, W, q)
+    err = ((got - col).abs() / col).max().item()
+    assert err <= (32 + n / 32 + 3) * 2.0 ** -24, err
+
+
 def test_attention_reports_bad_tables_and_lengths_and_stays_in_bounds(api):
     """Pages, snapshots and lengths that do not fit raise the status word; the other sequences are right."""
     for qs, lens in (((1, 1, 1), (300, 400, 500)), ((150, 140, 130), (300, 400, 500))):
