@@ -288,6 +288,24 @@ def test_attention_reports_bad_tables_and_lengths_and_stays_in_bounds(api):
                     assert ((got - ref).abs() <= tol)[part].all(), what
 
 
+def test_attention_more_blocks_than_the_workspace_holds(api):
+    """cu_q that decreases in between names rows more than once: the sequences' blocks may then be more than a call of that many rows can have."""
+    S, q, n, W, P, G, D = 15, 1024, 1300, 128, 64, 8, 64
+    g = torch.Generator(device="cuda").manual_seed(5)
+    pages = api.PagedKV(*(torch.randint(-127, 128, (21, 1, P, D), generator=g, device="cuda", dtype=torch.int8) for _ in range(3)),
+                        *(torch.full((21, 1, P), 0.01, device="cuda") for _ in range(3)))
+    table = torch.arange(21, dtype=torch.int32, device="cuda").repeat(S, 1)
+    lens = torch.full((S,), n, dtype=torch.int32, device="cuda")
+    cu_q = torch.tensor([0, q] * 8, dtype=torch.int32, device="cuda")
+    q1 = torch.randn(q, G, D, generator=g, device="cuda", dtype=BF16)
+    assert api.paged_attention_workspace_bytes(S, q, G, D, 1, W, q, torch.int8, BF16) > 0
+    got = api.paged_attention(q1, q1, pages, table, cu_q, lens, W, q)
+    with pytest.raises(native.VqError):
+        api.check_status()
+    assert torch.equal(got, api.paged_attention(q1, q1, pages, table[:1], cu_q[:2], lens[:1], W, q))
+    api.check_status()
+
+
 def test_append_reports_bad_tables_and_lengths_and_writes_nothing_for_them(api):
     D, P = 64, 16
     k = torch.randn(6, 1, D, device="cuda")

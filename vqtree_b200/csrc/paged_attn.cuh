@@ -102,7 +102,12 @@ __device__ __forceinline__ bool chunk_find(const PagedAttnParams &p, int TQ, int
             out.pos0 = lo;
             out.n = n;
             out.snap = p.snapshot(out.s, p.boundary(lo));
-            out.ws0 = ws_before + __shfl_sync(~0u, ws_sum, l) - __shfl_sync(~0u, blocks, l) - p.first_block(i0);
+            const int ws_end = ws_before + __shfl_sync(~0u, ws_sum, l);
+            out.ws0 = ws_end - __shfl_sync(~0u, blocks, l) - p.first_block(i0);
+            if (p.ws != nullptr && ws_end > p.ws_blocks) {       // only where sequences share rows (cu_q decreases in between): their blocks may be
+                p.seqs.raise(VQ_WORD_BAD_LENGTH);                // more than the workspace was sized for
+                return false;
+            }
             return true;
         }
         before += __shfl_sync(~0u, sum, 31);

@@ -351,7 +351,7 @@ extern "C" int vqattn_paged_append(const VqPagedAppendArgs *a, void *stream)
         if (reinterpret_cast<uintptr_t>(a->cos_tab) % 16 || reinterpret_cast<uintptr_t>(a->sin_tab) % 16) return VQ_EINVAL_STRIDE;
     }
     const int64_t rows = 2 * kv.Hkv + Hq;
-    if (T * rows > 0xffffffffLL) return VQ_EUNSUPPORTED;
+    if (T * rows > 0x7fffffffLL) return VQ_EUNSUPPORTED;
     const VqTensorDesc *all[] = {&a->k, &a->v, has_q ? &a->q : nullptr, has_q ? &a->q1 : nullptr, has_q ? &a->q2 : nullptr};
     if ((st = check_device(all, 5)) != VQ_OK || (st = check_paged_devices(a->kv)) != VQ_OK) return st;
     AppendParams p{};
