@@ -288,6 +288,22 @@ def test_attention_reports_bad_tables_and_lengths_and_stays_in_bounds(api):
                     assert ((got - ref).abs() <= tol)[part].all(), what
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("qs,lens", [((1, 5), (300, 800)), ((70, 150), (300, 800)), ((700, 3), (900, 301))])
+@pytest.mark.parametrize("which", [0, 2])
+def test_attention_8_bit_rows_that_are_not_finite_reach_only_their_readers(api, dtype, qs, lens, which):
+    """The key or value of the last sequence's last token but one was not finite: its scale is NaN.  Earlier tokens do not see it."""
+    c = Case(11, qs, lens, 2, 2, 64, 32, 128, 128, dtype, True, True)
+    at = lens[-1] - 2
+    c.scales[which][c.table[-1, at // c.P], :, at % c.P] = float("nan")
+    got = c.attend(api).double().cpu()
+    ref, mag = c.expected()
+    seen = min(2, qs[-1])
+    clean = slice(0, c.T - seen)
+    assert ((got - ref).abs() <= c.tolerance(ref, mag))[clean].all()
+    assert got[c.T - seen:].isnan().all()
+
+
 def test_attention_more_blocks_than_the_workspace_holds(api):
     """cu_q that decreases in between names rows more than once: the sequences' blocks may then be more than a call of that many rows can have."""
     S, q, n, W, P, G, D = 15, 1024, 1300, 128, 64, 8, 64

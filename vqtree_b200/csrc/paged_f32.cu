@@ -96,7 +96,11 @@ __global__ void __launch_bounds__(kF32Threads, 3) paged_f32_kernel(const PagedAt
         const KV *k = static_cast<const KV *>(kp.ptr) + kp.row(page, hk, pr) + 4 * lp;
         const KV *v = static_cast<const KV *>(p.v.ptr) + p.v.row(page, hk, pr) + 4 * lp;
         if constexpr (Q8) {
-            const float ks = __ldg(kp.scale + kp.scale_at(page, hk, pr)), vs = __ldg(p.v.scale + p.v.scale_at(page, hk, pr));
+            float ks = __ldg(kp.scale + kp.scale_at(page, hk, pr)), vs = __ldg(p.v.scale + p.v.scale_at(page, hk, pr));
+            if (!(fabsf(vs) < INFINITY)) {                   // a value row that is not finite: its score says so to the tokens that see it
+                ks = __int_as_float(0x7fffffff);
+                vs = 0.f;
+            }
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const char4 a = *reinterpret_cast<const char4 *>(k + 16 * j), b = *reinterpret_cast<const char4 *>(v + 16 * j);

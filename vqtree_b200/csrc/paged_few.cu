@@ -239,6 +239,10 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
             const float *ks = old ? p.k3.scale + p.k3.scale_at(page, hk, pr) : p.k1.scale + p.k1.scale_at(page, hk, pr);
             x = __ldg(ks);
             y = __ldg(p.v.scale + p.v.scale_at(page, hk, pr));
+            if (!(fabsf(y) < INFINITY)) {                            // a value row that is not finite: its score says so to the tokens that see it,
+                x = __int_as_float(0x7fffffff);                      // and the others do not multiply it by zero
+                y = 0.f;
+            }
             if (pg < 0) x = y = 0.f;
         }
     };
