@@ -2,9 +2,9 @@
 // dispatcher operators (torch.ops.vqattn.*), so that a PyTorch program can call them like any other
 // operator - under a device guard, on PyTorch's current stream, with TORCH_CHECK errors - without going
 // through Python's ctypes.  Nothing here computes: every operator describes its tensors as VqTensorDesc,
-// calls the C function the header declares and turns a negative status into an exception.  All operators
+// calls the C function the header declares and turns a negative status into an exception.  The operators
 // write into tensors the caller passes (out-variants): the library allocates nothing, and neither does
-// this file.
+// this file, but for the paged_*_new forms, which return new tensors.
 //
 // Reference interfaces behind the operators: ops/mini_vq.py:4-18 (assign_codes), ops/attn_vq.py:352-384,
 // 411-417 (build_aggregates), ops/triton_fused_vq_attn.py:190-251 (prefill), README.md:8 and
