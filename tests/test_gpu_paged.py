@@ -257,6 +257,49 @@ def test_attention_fp32_sums_over_long_windows_keep_their_bits(api, D, heads):
     assert err <= (32 + n / 32 + 3) * 2.0 ** -24, err
 
 
+@pytest.mark.parametrize("dtype,q8", [(F32, True), (BF16, False), (BF16, True), (F16, True)])
+@pytest.mark.parametrize("most", [3, 41])
+def test_attention_many_sequences(api, dtype, q8, most):
+    """More sequences than a warp looks up at a time, some without new tokens."""
+    qs = [7 * s % most for s in range(70)]
+    c = Case(13, qs, [max(1, q + 53 * s % 333) for s, q in enumerate(qs)], 1, 2, 64, 32, 128, 128, dtype, q8, True)
+    check_attention(c.attend(api), c)
+    api.check_status()
+
+
+@pytest.mark.parametrize("dtype,q8", [(F32, False), (BF16, False), (F16, True)])
+@pytest.mark.parametrize("G", [100, 128])
+def test_attention_widest_groups(api, dtype, q8, G):
+    c = Case(G, (3, 1), (270, 40), 1, G, 64, 64, 128, 128, dtype, q8, True)
+    check_attention(c.attend(api), c)
+    api.check_status()
+
+
+@pytest.mark.parametrize("dtype,q8,D", [(BF16, False, 128), (F16, True, 64)])
+def test_rows_behind_32_bits_of_a_pool(api, dtype, q8, D):
+    """The same sequences in the first pages of a small pool and in the last of one with more than 2^32 elements: the same bits."""
+    P, H, W, n, last = 128, 8, 128, 300, 2 ** 32 // (128 * 8 * D) + 4
+    kind = torch.int8 if q8 else dtype
+    g = torch.Generator(device="cuda").manual_seed(17)
+    k, v, q = (torch.randn(n, h, D, generator=g, device="cuda", dtype=dtype) for h in (H, H, 2 * H))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    room = lambda np: [torch.empty(np, H, P, D, dtype=kind, device="cuda") for _ in range(2)]
+    scale = lambda np: [torch.empty(np, H, P, device="cuda") for _ in range(2)] if q8 else [None, None]
+    got = []
+    for np, first in ((3, 0), (last, last - 3)):
+        (k1, vp), (ks, vs) = room(np), scale(np)
+        pages = api.PagedKV(k1, vp, None, ks, vs)
+        table = i32(first, first + 1, first + 2)[None]
+        q1, _ = api.paged_append(k, v, pages, table, i32(0, n), i32(n), q=q)
+        rows = api.paged_read([(k1, ks), (vp, vs)], table, i32(0), i32(n), n, dtype)
+        few = api.paged_attention(q1[-1:], q1[-1:], pages, table, i32(0, 1), i32(n), W, 1)
+        chunk = api.paged_attention(q1, q1, pages, table, i32(0, n), i32(n), W, n)
+        got.append(rows + [few, chunk])
+        api.check_status()
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and a.isfinite().all()
+
+
 def test_attention_reports_bad_tables_and_lengths_and_stays_in_bounds(api):
     """Pages, snapshots and lengths that do not fit raise the status word; the other sequences are right."""
     for qs, lens in (((1, 1, 1), (300, 400, 500)), ((150, 140, 130), (300, 400, 500))):
