@@ -136,6 +136,7 @@ def test_paged_entry_points_refuse_bad_arguments_without_a_device():
     assert append(k1=i8(), k3=i8(), v_pool=i8(), k1_scale=sc(), k3_scale=sc(), v_scale=z(4, 2, 8)) == -1
     assert append(k1=i8(), k3=i8(), v_pool=i8(), k1_scale=sc(), k3_scale=sc(), v_scale=sc()) == -4
     assert append(v_scale=sc()) == -7                               # scales of rows that have none
+    assert append(k1=z(1, 2, 16, 64).expand(4, 2, 16, 64)) == -3 and append(**dict(q, q1=z(1, 4, 64).expand(7, 4, 64))) == -3   # written to
 
     def read(pool, out, scale=None, table=i32(3, 5), start=i32(3), lens=i32(3)):
         a = native.VqPagedReadArgs()
@@ -165,6 +166,7 @@ def test_paged_entry_points_refuse_bad_arguments_without_a_device():
 
     assert lib.vqattn_paged_attention(None, None) == -7 and lib.vqattn_paged_append(None, None) == -7 and lib.vqattn_paged_read(None, None) == -7
     assert attend() == -4 and attend(codebook=None) == -4
+    assert attend(out=z(7, 1, 64).expand(7, 4, 64)) == -3
     assert attend(window=100) == -7 and attend(window=0) == -7 and attend(max_q=0) == -7
     assert attend(q1=z(7, 3, 64), q2=z(7, 3, 64), out=z(7, 3, 64)) == -1      # 3 query heads over 2
     assert attend(q2=z(7, 4, 64, dtype=torch.float16)) == -2 and attend(out=None) == -7 and attend(out=z(8, 4, 64)) == -1

@@ -345,6 +345,8 @@ extern "C" int vqattn_paged_append(const VqPagedAppendArgs *a, void *stream)
         if ((st = check_tokens(a->q1, T, Hq, kv.D, dt)) != VQ_OK) return st;
         if (a->q2.ptr != nullptr && (st = check_tokens(a->q2, T, Hq, kv.D, dt)) != VQ_OK) return st;
     }
+    for (const VqTensorDesc *t : {&a->kv.k1, &a->kv.k3, &a->kv.v, &a->kv.k1_scale, &a->kv.k3_scale, &a->kv.v_scale, &a->q1, &a->q2})
+        if (expanded(*t)) return VQ_EINVAL_STRIDE;
     if ((a->cos_tab == nullptr) != (a->sin_tab == nullptr)) return VQ_EINVAL_ARG;
     if (a->cos_tab != nullptr) {
         if (a->n_pos <= 0 || (has_q && a->q2.ptr != nullptr && (a->const_pos < 0 || a->const_pos >= a->n_pos))) return VQ_EINVAL_ARG;

@@ -78,6 +78,15 @@ inline bool rows_aligned(const VqTensorDesc &t)
     return reinterpret_cast<uintptr_t>(t.ptr) % 16 == 0;
 }
 
+// an expanded tensor: several elements in one place, which cannot be written to
+inline bool expanded(const VqTensorDesc &t)
+{
+    if (t.ptr == nullptr) return false;
+    for (int i = 0; i < t.ndim; ++i)
+        if (t.shape[i] > 1 && t.stride[i] == 0) return true;
+    return false;
+}
+
 // int32 vector of n entries, contiguous
 inline int check_i32(const VqTensorDesc &t, int64_t n)
 {
