@@ -107,9 +107,30 @@ class PagedVectorQuantizedCache:
             raise ValueError(f"the cache holds {self.dtype}")
         if key.shape != value.shape or tuple(key.shape) != (T, self.codebooks.shape[0], d) or d != self.codebooks.shape[3]:
             raise ValueError("key and value must be [T, kv heads, head dim] of the codebook")
+        if key.dtype != self.dtype or value.dtype != self.dtype:
+            raise ValueError(f"the cache holds {self.dtype}")
+        if hq % key.shape[1] != 0 or not 1 <= hq // key.shape[1] <= 128:
+            raise ValueError("query heads must be 1 to 128 times the kv heads")
         if T == 0:
             return query.new_empty(0, hq * d)
         seqs = [self._sequences[s] for s in sids]
+        before, saved = [(seq, seq.bd, len(seq.pages)) for seq in seqs], []
+        try:
+            lens, out = self._run(seqs, q_lens, query, key, value, scale, saved)
+        except BaseException:                               # out of memory, say: the sequences stay what they were before the call
+            self._undo(before, saved)
+            raise
+        for seq, n in zip(seqs, lens):                      # pages in front of the boundary have become counts and sums
+            seq.n = n
+            gone = seq.bd // self.page_size - seq.first
+            if gone > 0:
+                self._free_pages.extend(reversed(seq.pages[:gone]))
+                del seq.pages[:gone]
+                seq.first += gone
+        return out.reshape(T, hq * d)
+
+    def _run(self, seqs, q_lens, query, key, value, scale, saved):
+        """The call on checked arguments: what it changes, but for ``n`` and the pages that fall free, ``_undo`` takes back."""
         lens = self._reserve(seqs, q_lens)
         meta = [0]
         for x in q_lens:
@@ -121,17 +142,22 @@ class PagedVectorQuantizedCache:
         W = self.window_length
         q1, q2 = api.paged_append(key, value, self.pages, table, cu_q, seq_lens, q=query, const_pos=W + 1 if self.rerope else None,
                                   base=self.rope_base, n_pos=max(self.max_length, W + 2))
-        snaps = self._fold(seqs, q_lens, table, seq_lens)
+        snaps = self._fold(seqs, q_lens, table, seq_lens, saved)
         out = api.paged_attention(q1, q2 if self.rerope else q1, self.pages, table, cu_q, seq_lens, W, max(q_lens), codebook=self.codebook_act,
-                                  cnt=self.cnt, vsum=self.vsum, snap_table=snaps, scale=scale or 1.0 / math.sqrt(d))
-        for seq, n in zip(seqs, lens):                      # pages in front of the boundary have become counts and sums
-            seq.n = n
-            gone = seq.bd // self.page_size - seq.first
-            if gone > 0:
-                self._free_pages.extend(reversed(seq.pages[:gone]))
-                del seq.pages[:gone]
-                seq.first += gone
-        return out.reshape(T, hq * d)
+                                  cnt=self.cnt, vsum=self.vsum, snap_table=snaps, scale=scale or 1.0 / math.sqrt(query.shape[2]))
+        return lens, out
+
+    def _undo(self, before, saved) -> None:
+        """After a call that failed: pages it took go back, boundaries and aggregates are those of before."""
+        for seq, bd, pages in before:
+            self._free_pages.extend(reversed(seq.pages[pages:]))
+            del seq.pages[pages:]
+            seq.bd = bd
+        for slots, cnt, vsum32 in saved:
+            for i, s in enumerate(slots):
+                self.cnt[s].copy_(cnt[i])
+                self.vsum32[s].copy_(vsum32[i])
+                self.vsum[s].copy_(vsum32[i])
 
     def _upload(self, numbers) -> torch.Tensor:
         t = torch.tensor(numbers, dtype=torch.int32)
@@ -164,9 +190,10 @@ class PagedVectorQuantizedCache:
             self.block_table.view(-1).index_copy_(0, new[: len(where)].long(), new[len(where):])
         return lens
 
-    def _fold(self, seqs, q_lens, table, seq_lens) -> torch.Tensor:
+    def _fold(self, seqs, q_lens, table, seq_lens, saved) -> torch.Tensor:
         """Blocks that the new queries no longer see one by one go into counts and value sums; where the queries of one call have
-        several boundaries, the aggregates of the earlier ones are kept in spare rows.  Returns the snapshot table of the call."""
+        several boundaries, the aggregates of the earlier ones are kept in spare rows.  Returns the snapshot table of the call.
+        saved: takes (slots, counts, fp32 sums) of the sequences that change, as they were."""
         leaving = []                                        # (index of the sequence in the call, block)
         plan = []
         for x, (seq, q) in enumerate(zip(seqs, q_lens)):
@@ -179,10 +206,12 @@ class PagedVectorQuantizedCache:
         if leaving:
             kv = self.pages
             pair = [(kv.k3, kv.k3_scale) if self.rerope else (kv.k1, kv.k1_scale), (kv.v, kv.v_scale)]
-            idx = self._upload([x for x, _ in leaving] + [b for _, b in leaving])
-            which, starts = idx[: len(leaving)], idx[len(leaving):]
+            slots = sorted({seqs[x].slot for x, _ in leaving})
+            idx = self._upload([x for x, _ in leaving] + [b for _, b in leaving] + slots)
+            which, starts, rows = idx[: len(leaving)], idx[len(leaving): 2 * len(leaving)], idx[2 * len(leaving):]
             raw, val = api.paged_read(pair, table.index_select(0, which), starts, seq_lens.index_select(0, which), BLOCK_SIZE, self.dtype)
             codes = api.assign_codes(raw, self.codebooks)
+            saved.append((slots, self.cnt.index_select(0, rows), self.vsum32.index_select(0, rows)))
         K, spare, at = self.codebooks.shape[2], self.max_sequences, 0
         for x, (seq, (b0, b1)) in enumerate(zip(seqs, plan)):
             s = seq.slot
