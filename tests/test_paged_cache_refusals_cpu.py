@@ -5,7 +5,8 @@ import torch
 from tests import fake_paged
 from tests.paged_scenarios import whole_sequences
 from vqtree_b200 import api
-from vqtree_b200.paged_cache import PagedVectorQuantizedCache
+from vqtree_b200.attn_vq import VectorQuantizedReRoPECache
+from vqtree_b200.paged_cache import OutOfPages, PagedVectorQuantizedCache
 
 W, D, M, K = 128, 64, 1, 128
 
@@ -88,3 +89,29 @@ def test_query_heads_that_attention_would_refuse_are_refused_before_anything_cha
         with pytest.raises(ValueError):
             cache.attend([s], [20], torch.randn(20, 4, D), k.half(), k.half())
         assert cache.length(s) == 0 and cache.free_pages == 64
+
+
+def _dense(n, cb, batch=2, **kw):
+    """A dense cache as a prefill of n tokens leaves it: rows of ones, counts of zeros."""
+    bd = max(0, (n - W) // 128 * 128)
+    H, rows = cb.shape[0], torch.ones(batch, cb.shape[0], n - bd, D)
+    dense = VectorQuantizedReRoPECache(W, cb, **kw)
+    dense.update_prefill(torch.zeros(batch, H, M * K), torch.zeros(batch, H, M * K, D), rows, rows, 0, n, {"key_unrotated": rows})
+    return dense
+
+
+def test_adopt_that_is_refused_or_fails_keeps_no_slot_and_no_page(monkeypatch):
+    cb = torch.randn(1, M, K, D)
+    with fake_paged.installed():
+        cache = _cache(cb, max_length=256)
+        with pytest.raises(ValueError, match="max_length"):
+            cache.adopt(_dense(300, cb))
+        with pytest.raises(OutOfPages):
+            cache.adopt(_dense(200, cb, batch=4))
+        with monkeypatch.context() as m:
+            _fail_once(m, "paged_append", 1)
+            with pytest.raises(RuntimeError):
+                cache.adopt(_dense(200, cb))
+        assert cache.free_pages == 64
+        sids = cache.adopt(_dense(200, cb, batch=3))          # all three slots
+        assert [cache.length(s) for s in sids] == [200] * 3 and cache.free_pages == 64 - 3 * 13

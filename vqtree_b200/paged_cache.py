@@ -237,10 +237,23 @@ class PagedVectorQuantizedCache:
         assert dense.window_length == self.window_length and tuple(dense.codebooks.shape) == tuple(self.codebooks.shape)
         st = dense.states[layer_idx]
         live, B = st["n"] - st["bd"], st["win_k3"].shape[0]
+        if st["n"] > self.max_length:
+            raise ValueError(f"a sequence of {st['n']} tokens exceeds max_length")
         if B > len(self._free_slots) or B * (-(-st["n"] // self.page_size) - st["bd"] // self.page_size) > len(self._free_pages):
             raise OutOfPages("the dense cache's sequences do not fit")
-        sids = [self.add_sequence() for _ in range(B)]
-        seqs = [self._sequences[s] for s in sids]
+        sids = []
+        try:
+            for _ in range(B):
+                sids.append(self.add_sequence())
+            self._take_over(dense, st, [self._sequences[s] for s in sids], live)
+        except BaseException:
+            for s in sids:
+                self.remove_sequence(s)
+            raise
+        return sids
+
+    def _take_over(self, dense, st, seqs, live) -> None:
+        B = len(seqs)
         for b, seq in enumerate(seqs):
             seq.n = seq.bd = st["bd"]
             seq.first = st["bd"] // self.page_size
@@ -255,7 +268,6 @@ class PagedVectorQuantizedCache:
                              meta[B + 1: 2 * B + 1], base=self.rope_base, n_pos=max(self.max_length, self.window_length + 2))
         for seq in seqs:
             seq.n = st["n"]
-        return sids
 
     def to_dense(self, sid: int) -> VectorQuantizedReRoPECache:
         """One sequence as a dense cache of its own (layer 0), window rows read back from their pages; the sequence stays here too."""
