@@ -115,3 +115,19 @@ def test_adopt_that_is_refused_or_fails_keeps_no_slot_and_no_page(monkeypatch):
         assert cache.free_pages == 64
         sids = cache.adopt(_dense(200, cb, batch=3))          # all three slots
         assert [cache.length(s) for s in sids] == [200] * 3 and cache.free_pages == 64 - 3 * 13
+
+
+def test_adopt_refuses_another_codebook_and_another_rotary_base():
+    cb = torch.randn(1, M, K, D)
+    with fake_paged.installed():
+        cache = _cache(cb, rope_base=5e5)
+        with pytest.raises(ValueError, match="base"):
+            cache.adopt(_dense(200, cb, rope_base=1e4))
+        with pytest.raises(ValueError, match="codebook"):
+            cache.adopt(_dense(200, cb + 1, rope_base=5e5))
+        assert cache.free_pages == 64
+        # an equal codebook elsewhere, one of fewer bits that stands for the same numbers, a base left to the model's configuration
+        cache.adopt(_dense(150, cb.clone(), batch=1, rope_base=5e5))
+        cache.adopt(_dense(150, cb, batch=1))
+        half = _cache(cb.half().float())
+        half.adopt(_dense(150, cb.half(), batch=1))

@@ -232,9 +232,16 @@ class PagedVectorQuantizedCache:
 
     # ---- to and from the dense cache
     def adopt(self, dense: VectorQuantizedReRoPECache, layer_idx: int = 0) -> List[int]:
-        """The sequences of a dense cache's layer (a prompt that one call prefilled), continued here; returns their ids."""
+        """The sequences of a dense cache's layer (a prompt that one call prefilled), continued here; returns their ids.  Its counts belong
+        to its codebook's entries and its queries to its rotary base: both have to be this cache's (a base it left to the model's
+        configuration is not known here)."""
         assert self.rerope, "the dense cache holds ReRoPE keys"
         assert dense.window_length == self.window_length and tuple(dense.codebooks.shape) == tuple(self.codebooks.shape)
+        if dense.rope_base is not None and dense.rope_base != self.rope_base:
+            raise ValueError(f"the dense cache rotates with base {dense.rope_base}, this one with {self.rope_base}")
+        other = dense.codebooks.to(self.device, torch.float32)
+        if other.data_ptr() != self.codebooks.data_ptr() and not torch.equal(other, self.codebooks):
+            raise ValueError("the dense cache counts codes of another codebook")
         st = dense.states[layer_idx]
         live, B = st["n"] - st["bd"], st["win_k3"].shape[0]
         if st["n"] > self.max_length:
