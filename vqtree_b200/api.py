@@ -157,8 +157,19 @@ _ROPE_TABLES = {}
 _ROPE_REPLACED = []     # tables that a longer one replaced: a captured graph may still read them (together they are shorter than the longest)
 
 
+def _capturing(dev) -> bool:
+    """The current stream of ``dev`` is being captured: what is launched now runs at a replay."""
+    if dev.type != "cuda":
+        return False
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def rope_tables(n_pos: int, dim: int, device, base: float = 10000.0):
-    """fp32 cos / sin tables [n_pos, dim/2] (angle = pos * base^(-2i/dim), evaluated in float64), cached per device."""
+    """fp32 cos / sin tables [n_pos, dim/2] (angle = pos * base^(-2i/dim), evaluated in float64), cached per device.
+
+    The stream that fills a cached table is waited for once, so that every stream may read it.  Under capture a table that is not
+    there yet is filled by every replay of that graph, for its own use: one call before the capture saves that."""
     dev = torch.device(device)
     key = (_device_index(dev), dim, float(base))
     have = _ROPE_TABLES.get(key)
@@ -166,9 +177,14 @@ def rope_tables(n_pos: int, dim: int, device, base: float = 10000.0):
         n = max(n_pos, 2 * have[0].shape[0] if have is not None else 0)
         inv = 1.0 / (base ** (torch.arange(0, dim, 2, dtype=torch.float64, device=dev) / dim))
         ang = torch.outer(torch.arange(n, dtype=torch.float64, device=dev), inv)
+        new = (ang.cos().float().contiguous(), ang.sin().float().contiguous())
+        if _capturing(dev):
+            return new
+        if dev.type == "cuda" and not torch.compiler.is_compiling():
+            torch.cuda.current_stream(dev).synchronize()
         if have is not None:
             _ROPE_REPLACED.append(have)
-        have = _ROPE_TABLES[key] = (ang.cos().float().contiguous(), ang.sin().float().contiguous())
+        have = _ROPE_TABLES[key] = new
     return have
 
 
@@ -389,7 +405,8 @@ class DecodeStepCall:
 
     def _tables(self, n_pos):
         D = self.keep[0].shape[-1]
-        self.cos, self.sin = rope_tables(n_pos, D, self.dev, self.base)
+        tables = self.cos, self.sin = rope_tables(n_pos, D, self.dev, self.base)
+        self._one_graph = tables is not _ROPE_TABLES.get((self.dev_index, D, float(self.base)))    # a capture's own: not for the next call
         a = self.args
         a.cos_tab, a.sin_tab, a.n_pos = self.cos.data_ptr(), self.sin.data_ptr(), self.cos.shape[0]
 
@@ -414,7 +431,7 @@ class DecodeStepCall:
             self._in = sig
         else:
             a.q.ptr, a.k.ptr, a.v.ptr, a.decode.out.ptr = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-        if pos + 1 > a.n_pos:
+        if pos + 1 > a.n_pos or self._one_graph:
             self._tables(pos + 1)
         a.positions = positions.data_ptr() if positions is not None else None
         a.pos, a.row = int(pos), int(row)
