@@ -36,7 +36,7 @@ template <> struct Codes8<__half> {
 // A weight times a value row of codes with scale vs, in halves: weight * (vs * 2^k) and codes * 2^-k, with k such that the first factor lies in
 // [1, 2) - and inside what a half holds for every scale of half values (2^-31 .. 2^10).  Otherwise a small scale would put
 // the products among the subnormal halves, where the codes of a snapshot (weights without a scale) share the accumulator.
-// half_weight_shift: k for one scale, or for the largest of a tile.
+// k goes by the row's own scale: one for several rows would take the bits of the weights of the small ones.
 __device__ __forceinline__ int half_weight_shift(float vs)
 {
     const int k = 127 - static_cast<int>((__float_as_uint(vs) >> 23) & 255u);

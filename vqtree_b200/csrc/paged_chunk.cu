@@ -94,15 +94,6 @@ __device__ __forceinline__ bool all_of_named(bool x)
     return r != 0;
 }
 
-// maximum of four values of every lane
-__device__ __forceinline__ float warp_max4(const float (&x)[4])
-{
-    float m = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    return m;
-}
-
 // 8-bit rows.  ks: scale of each of 64 keys times the softmax scale, vs: factor of each value row.
 __device__ __forceinline__ void load_scores(uint32_t s_addr, uint32_t (&r)[64])
 {
@@ -382,8 +373,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
                 stage();
                 stage();
             }
-            // Half values: their codes are multiplied by a power of two that goes with the tile's largest scale (the softmax warps put its inverse
-            // into the weights).  The scales are asked for one tile ahead, four rows per lane.
+            // Half values: a row's codes are multiplied by a power of two that goes with its scale (the softmax warps put its inverse into the
+            // weights).  The scales are asked for one tile of values ahead.  A lane has those of four rows: of the NI that a lane converts in block x / RPI as
+            // its row x % RPI, for x = the lane's number (and 32 more, with heads of 64).
             float vsc[4];
             auto value_scales = [&](int x) {
                 if constexpr (F16) {
@@ -393,13 +385,19 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
                     if (!is_v || work.kind(it) == kFar) return;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int key = work.block(it) * kBlock + 32 * i + lane, pg = key < tile.n ? page_of(key) : -1;
+                        const int x4 = lane + 32 * (i / NI), key = work.block(it) * kBlock + x4 / RPI * 8 + RPI * (i % NI) + x4 % RPI;
+                        const int pg = key < tile.n ? page_of(key) : -1;
                         vsc[i] = pg >= 0 ? __ldg(p.v.scale + p.v.scale_at(pg, hk, key & (page_size - 1))) : 0.f;
                     }
                 }
             };
+            auto next_value_scales = [&](int x) {                          // behind values in load x
+                bool is_v;
+                item_of(x + 1, is_v);
+                value_scales(is_v ? x + 1 : x + 2);
+            };
             int raw = 0;
-            value_scales(0);
+            value_scales(min(NB, n));
             for (int x = 0; x < 2 * n; ++x) {
                 bool is_v;
                 const int it = item_of(x, is_v);
@@ -410,31 +408,50 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
                 if (far) {
                     if (lw == 0 && elect_one()) far_tile(it, is_v);
                     __syncwarp();
-                    value_scales(x + 1);
+                    if (is_v) next_value_scales(x);
                 } else {
                     const uint8_t *src = smem + C::kRaws + (raw & 1) * C::kRaw;
                     uint8_t *dst = smem + C::kRing + slot * C::kTile;
-                    __half2 p2;
-                    if constexpr (F16) p2 = __float2half2_rn(is_v ? pow2f(-half_weight_shift(warp_max4(vsc))) : 1.f);
-#pragma unroll 1
-                    for (int blk = lw; blk < kBlock / 8; blk += C::kLoad) {
-                        uint2 codes[NI];
+                    uint32_t p2s[2];                                       // of those rows, two halves a word
+                    if (F16 && is_v) {
 #pragma unroll
-                        for (int i = 0; i < NI; ++i) codes[i] = *reinterpret_cast<const uint2 *>(src + blk * (8 * D) + from[i]);
-#pragma unroll
-                        for (int i = 0; i < NI; ++i) {
-                            uint4 w;
-                            if constexpr (F16) {
-                                Codes8<T>::expand_scaled(codes[i].x, p2, w.x, w.y);
-                                Codes8<T>::expand_scaled(codes[i].y, p2, w.z, w.w);
-                            } else {
-                                Codes8<T>::expand(codes[i].x, w.x, w.y);
-                                Codes8<T>::expand(codes[i].y, w.z, w.w);
-                            }
-                            *reinterpret_cast<uint4 *>(dst + blk * 1024 + to[i]) = w;
-                        }
+                        for (int i = 0; i < 2; ++i)
+                            p2s[i] = ptx::pack_f16(pow2f(-half_weight_shift(vsc[2 * i])), pow2f(-half_weight_shift(vsc[2 * i + 1])));
+                        next_value_scales(x);
                     }
-                    value_scales(x + 1);
+                    auto convert = [&](auto scaled) {
+#pragma unroll 1
+                        for (int blk = lw; blk < kBlock / 8; blk += C::kLoad) {
+                            uint2 codes[NI];
+                            uint32_t p2_of[2] = {0, 0};
+                            if constexpr (scaled.value) {
+                                p2_of[0] = __shfl_sync(~0u, NI == 4 || blk < 8 ? p2s[0] : p2s[1], (blk * RPI + rsub) & 31);
+                                if (NI == 4) p2_of[1] = __shfl_sync(~0u, p2s[1], (blk * RPI + rsub) & 31);
+                            }
+#pragma unroll
+                            for (int i = 0; i < NI; ++i) codes[i] = *reinterpret_cast<const uint2 *>(src + blk * (8 * D) + from[i]);
+#pragma unroll
+                            for (int i = 0; i < NI; ++i) {
+                                uint4 w;
+                                if constexpr (scaled.value) {
+                                    const uint32_t h = __byte_perm(p2_of[i / 2], 0, i & 1 ? 0x3232 : 0x1010);
+                                    const __half2 p2 = *reinterpret_cast<const __half2 *>(&h);
+                                    Codes8<__half>::expand_scaled(codes[i].x, p2, w.x, w.y);
+                                    Codes8<__half>::expand_scaled(codes[i].y, p2, w.z, w.w);
+                                } else {
+                                    Codes8<T>::expand(codes[i].x, w.x, w.y);
+                                    Codes8<T>::expand(codes[i].y, w.z, w.w);
+                                }
+                                *reinterpret_cast<uint4 *>(dst + blk * 1024 + to[i]) = w;
+                            }
+                        }
+                    };
+                    if constexpr (F16) {
+                        if (is_v) convert(std::true_type());
+                        else convert(std::false_type());
+                    } else {
+                        convert(std::false_type());
+                    }
                     fence_proxy_async_smem();
                     asm volatile("bar.sync 1, %0;" ::"n"(C::kLoad * 32) : "memory");   // staging tile read, slot written
                     if (lw == 0) {
@@ -570,9 +587,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
             if (kind == kFar || q8) {
                 __syncwarp();
                 bool full = true;
-                float mul = 1.f;                              // half weights: see half_weight_shift
-                if constexpr (CONV && F16)
-                    if (kind != kFar) mul = pow2f(half_weight_shift(warp_max4(reg_v)));
 #pragma unroll
                 for (int i = 0; i < NCW; ++i) {
                     if (kind == kFar) {
@@ -580,7 +594,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q1, const __grid_const
                         full = full && reg_w[i] > 0.f;
                     } else if constexpr (Q8) {
                         cw[32 * i + lane] = CONV ? reg_w[i] * p.scale_log2 : reg_w[i];
-                        cv[32 * i + lane] = CONV && F16 ? reg_v[i] * mul : reg_v[i];
+                        float p2;
+                        cv[32 * i + lane] = CONV && F16 ? half_weight_factor(reg_v[i], p2) : reg_v[i];
                     }
                 }
                 has_empty = kind == kFar && __any_sync(kAll, !full);
@@ -772,12 +787,11 @@ static bool map_pool(CUtensorMap *out, const PagedPool &pool, const PagedAttnPar
 }
 
 // Blocks of 128 keys of a call's sequences, from the first that a new token sees on: codes -> 16-bit floats (exact; half values times the power of two
-// that goes with their block's largest scale), rows behind the end -> zeros.  A CTA per block, kv head and pool; bound by memory traffic.
+// that goes with their row's scale), rows behind the end -> zeros.  A CTA per block, kv head and pool; bound by memory traffic.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) convert_blocks_kernel(const PagedAttnParams p)
 {
     __shared__ int s_seq, s_blk, s_n, s_last;
-    __shared__ float s_max[4];
     const int tid = threadIdx.x, lane = tid & 31, hk = blockIdx.y, pool_id = blockIdx.z;      // 0: k1, 1: v, 2: k3
     if (tid < 32) {
         int before = 0, seq = -1, blk = 0, len = 0, last = 0;
@@ -816,25 +830,14 @@ __global__ void __launch_bounds__(256) convert_blocks_kernel(const PagedAttnPara
     if (seq < 0 || (pool_id == 2 && blk > s_last - p.W / kBlock)) return;      // raw keys: those before somebody's exact window
     const PagedPool &pool = pool_id == 0 ? p.k1 : pool_id == 1 ? p.v : p.k3;
     const int page_mask = (1 << p.seqs.log_p) - 1;
-    float mul = 1.f;
-    if constexpr (!IsBf16<T>::value) {
-        if (pool_id == 1) {
-            if (tid < kBlock) {
-                const int key = blk * kBlock + tid, page = key < n ? p.seqs.page(seq, key >> p.seqs.log_p) : -1;
-                float x = page >= 0 ? __ldg(pool.scale + pool.scale_at(page, hk, key & page_mask)) : 0.f;
-#pragma unroll
-                for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
-                if (lane == 0) s_max[tid >> 5] = x;
-            }
-            __syncthreads();
-            mul = pow2f(-half_weight_shift(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]))));
-        }
-    }
+    constexpr bool kHalf = !IsBf16<T>::value;
     const int64_t at = (pool_id * p.ws_blocks + blockIdx.x) * p.Hkv + hk;
     if (tid < kBlock) {                                      // what multiplies the scores of a key, or the weights of a value
         const int key = blk * kBlock + tid, page = key < n ? p.seqs.page(seq, key >> p.seqs.log_p) : -1;
         const float x = page >= 0 ? __ldg(pool.scale + pool.scale_at(page, hk, key & page_mask)) : 0.f;
-        p.ws_scales(3 * p.ws_blocks * p.Hkv * (kBlock * D * 2))[at * kBlock + tid] = pool_id == 1 ? x * (1.f / mul) : x * p.scale_log2;
+        float p2;
+        p.ws_scales(3 * p.ws_blocks * p.Hkv * (kBlock * D * 2))[at * kBlock + tid] =
+            pool_id != 1 ? x * p.scale_log2 : kHalf ? half_weight_factor(x, p2) : x;
     }
     T *dst = static_cast<T *>(p.ws) + at * (kBlock * D);
     constexpr int CH = D / 16;
@@ -850,7 +853,8 @@ __global__ void __launch_bounds__(256) convert_blocks_kernel(const PagedAttnPara
             Codes8<T>::expand(codes.z, b.x, b.y);
             Codes8<T>::expand(codes.w, b.z, b.w);
         } else {
-            const __half2 m2 = __float2half2_rn(mul);
+            const float scale = pool_id == 1 && page >= 0 ? __ldg(pool.scale + pool.scale_at(page, hk, key & page_mask)) : 0.f;
+            const __half2 m2 = __float2half2_rn(pool_id == 1 ? pow2f(-half_weight_shift(scale)) : 1.f);
             Codes8<T>::expand_scaled(codes.x, m2, a.x, a.y);
             Codes8<T>::expand_scaled(codes.y, m2, a.z, a.w);
             Codes8<T>::expand_scaled(codes.z, m2, b.x, b.y);
