@@ -72,6 +72,10 @@ struct FewCfg {
     static constexpr int kPages = 256;                           // page table entries kept in shared memory; the rest is read where it is needed
     static constexpr int kTotal = kWarps * kWarpBytes + kQ + kPages * 4 + 1024;   // + slack for 1024-byte alignment
     static_assert(kCols * D * 4 <= kStages * kStage, "a warp's sums fit into its FIFO");
+    // Log2 units that a row's reference lies below the score that set it.  Weights meet their values in 16 bits: a half loses bits below 2^-14, which
+    // half caches have anyway, but a bf16 does not.  So the halves of a bf16 cache with 8-bit rows use the upper end of their range: up to
+    // 2^(8 + 6) times a factor below 2, all bits down to 2^-20 of the largest weight.
+    static constexpr float kBelow = Q8 && IsBf16<T>::value ? 6.f : 0.f;
     static constexpr int MT = D / 16;
 };
 
@@ -342,9 +346,10 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constan
                         float v = mx[nt][x];
 #pragma unroll
                         for (int y = 4; y < 32; y <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, y));
-                        if (v > m[nt][x]) {
-                            const float a = m[nt][x] == -INFINITY ? 0.f : ptx::ex2(m[nt][x] - v);
-                            m[nt][x] = v;
+                        const float ref = v - C::kBelow;
+                        if (ref > m[nt][x]) {
+                            const float a = m[nt][x] == -INFINITY ? 0.f : ptx::ex2(m[nt][x] - ref);
+                            m[nt][x] = ref;
                             lim[nt][x] = v + kFewLazy;
                             l[nt][x] *= a;
 #pragma unroll
