@@ -347,7 +347,8 @@ int vqattn_store_window(const VqTensorDesc *k1, const VqTensorDesc *k3, const Vq
  *   cu_q       [S+1] i32     new tokens of sequence s: rows cu_q[s] .. cu_q[s+1]-1 of the packed tensors; rows from cu_q[S] on are
  *                            left as they are.  A sequence may have none.
  *   lens       [S] i32       tokens of sequence s, the new ones included (they are its last)
- * Row and outer strides of the pools are free (multiples of 16 bytes; strides of scales: any; of what is written to none is 0).  table, cu_q and lens are read on the
+ * Row and outer strides of the pools are free (multiples of 16 bytes; strides of scales: any; none is 0 of what is written, nor of
+ * the pools, queries and outputs of the attention).  table, cu_q and lens are read on the
  * device: a captured call replays with the values they then hold.  Lengths that do not fit (cu_q decreasing or beyond the packed rows, more
  * new tokens than tokens, more tokens than the table has columns for) leave that sequence out and raise VQ_WORD_BAD_LENGTH.  A page that is needed and lies outside the pool raises
  * VQ_WORD_BAD_PAGE: nothing is read or written for it, and output rows that would need it are unspecified (finite or not).

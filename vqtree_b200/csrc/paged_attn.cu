@@ -43,7 +43,9 @@ extern "C" int vqattn_paged_attention(const VqPagedAttentionArgs *a, void *strea
     if (kv.dtype != VQ_I8 && kv.dtype != dt) return VQ_EINVAL_DTYPE;
     for (const VqTensorDesc *t : {&a->q1, &a->q2, &a->out})
         if ((st = check_tokens(*t, T, Hq, kv.D, dt)) != VQ_OK) return st;
-    if (expanded(a->out)) return VQ_EINVAL_STRIDE;
+    // outputs cannot be written, and rows that tensor maps fetch are not described with a stride of 0: the same answer in every form
+    for (const VqTensorDesc *t : {&a->q1, &a->q2, &a->out, &a->kv.k1, &a->kv.k3, &a->kv.v})
+        if (expanded(*t)) return VQ_EINVAL_STRIDE;
     if (Hq % kv.Hkv != 0) return VQ_EINVAL_SHAPE;
     if (a->window <= 0 || a->window % kBlock != 0 || a->window > 0x40000000 || a->max_q <= 0) return VQ_EINVAL_ARG;
     const int64_t G = Hq / kv.Hkv;

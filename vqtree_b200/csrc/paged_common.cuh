@@ -78,7 +78,7 @@ inline bool rows_aligned(const VqTensorDesc &t)
     return reinterpret_cast<uintptr_t>(t.ptr) % 16 == 0;
 }
 
-// an expanded tensor: several elements in one place, which cannot be written to
+// an expanded tensor: several elements in one place
 inline bool expanded(const VqTensorDesc &t)
 {
     if (t.ptr == nullptr) return false;
