@@ -364,7 +364,8 @@ typedef struct VqPagedKv {
  * NULL), v [T,Hkv,D] -> v, rounded to the pools' type or quantised to i8 (from the fp32 rotation, not from a rounded one).
  * q [T,Hq,D] (ptr NULL: none) -> q1 [T,Hq,D] rotated to the tokens' positions, and q2 [T,Hq,D] (ptr NULL: none) rotated to const_pos.
  * cos_tab / sin_tab [n_pos, D/2] f32 as for vqattn_rope; NULL: keys (and queries) are stored as they are.
- * The pools' type is k's, or i8; k3 may not be k1's memory.  A position outside the tables raises VQ_WORD_BAD_POSITION and uses the nearest row.
+ * The pools' type is k's, or i8; no two of k1, k3 and v, of their scales, or of q1 and q2 start at the same
+ * address.  A position outside the tables raises VQ_WORD_BAD_POSITION and uses the nearest row.
  */
 typedef struct VqPagedAppendArgs {
     VqPagedKv kv;

@@ -46,3 +46,28 @@ def test_attention_refuses_expanded_rows_in_every_form(dtype, q8, T):
     assert _attend(dtype, q8, T, table=_i32(1, 5).expand(3, 5)) == -4
     if q8:
         assert _attend(dtype, q8, T, v_scale=z(1).expand(4, 2, 16)) == -4
+
+
+def _append(**kw):
+    native = _native()
+    i8, sc, q = (lambda: z(4, 2, 16, 64, dtype=torch.int8)), (lambda: z(4, 2, 16)), (lambda: z(7, 4, 64))
+    t = dict(k1=i8(), k3=i8(), v_pool=i8(), k1_scale=sc(), k3_scale=sc(), v_scale=sc(), table=_i32(3, 5), cu_q=_i32(4), lens=_i32(3), k=z(7, 2, 64),
+             v=z(7, 2, 64), q=q(), q1=q(), q2=q())
+    t.update(kw)
+    a = native.VqPagedAppendArgs()
+    native.desc(t.pop("v_pool"), a.kv.v)
+    for name, x in t.items():
+        native.desc(x, getattr(a.kv if name != "v" and hasattr(a.kv, name) else a, name))
+    return native.lib.vqattn_paged_append(ctypes.byref(a), None)
+
+
+def test_append_refuses_two_outputs_in_one_place():
+    assert _append() == -4
+    s, q = z(4, 2, 16), z(7, 4, 64)
+    for pair in (("k1", "k3"), ("k1", "v"), ("k3", "v")):
+        assert _append(**{n + "_scale": s for n in pair}) == -7
+    assert _append(q1=q, q2=q) == -7
+    # what is read may be one tensor, and queries may be rotated in place
+    assert _append(q=q, q1=q) == -4 and _append(q2=None) == -4
+    x = z(7, 2, 64)
+    assert _append(k=x, v=x) == -4

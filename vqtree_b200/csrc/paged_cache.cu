@@ -335,7 +335,11 @@ extern "C" int vqattn_paged_append(const VqPagedAppendArgs *a, void *stream)
     PagedArgs kv;
     if ((st = check_paged_kv(a->kv, T, a->status_word, kv)) != VQ_OK) return st;
     if (kv.dtype != VQ_I8 && kv.dtype != dt) return VQ_EINVAL_DTYPE;
-    if (a->kv.k3.ptr == a->kv.k1.ptr || a->kv.v.ptr == a->kv.k1.ptr || a->kv.v.ptr == a->kv.k3.ptr) return VQ_EINVAL_ARG;   // three writers of one row
+    // several writers of one row, of one scale, of one query
+    const auto same = [](const VqTensorDesc &x, const VqTensorDesc &y) { return x.ptr != nullptr && x.ptr == y.ptr; };
+    const VqPagedKv &pg = a->kv;
+    if (same(pg.k3, pg.k1) || same(pg.v, pg.k1) || same(pg.v, pg.k3)) return VQ_EINVAL_ARG;
+    if (same(pg.k3_scale, pg.k1_scale) || same(pg.v_scale, pg.k1_scale) || same(pg.v_scale, pg.k3_scale) || same(a->q1, a->q2)) return VQ_EINVAL_ARG;
     if ((st = check_tokens(a->k, T, kv.Hkv, kv.D, dt)) != VQ_OK) return st;
     if ((st = check_tokens(a->v, T, kv.Hkv, kv.D, dt)) != VQ_OK) return st;
     const bool has_q = a->q.ptr != nullptr;
