@@ -219,6 +219,9 @@ VqTensorDesc any_desc(const std::optional<at::Tensor> &t)
 
 using OptTensor = std::optional<at::Tensor>;
 
+// a CUDA tensor of another device than the call's: what goes to the C function as a bare pointer, which it cannot check
+bool elsewhere(const OptTensor &t, const at::Tensor &call) { return t.has_value() && t->defined() && t->is_cuda() && t->get_device() != call.get_device(); }
+
 VqPagedKv paged_kv(const at::Tensor &k1, const at::Tensor &v, const OptTensor &k3, const OptTensor &k1_scale, const OptTensor &v_scale,
                    const OptTensor &k3_scale, const at::Tensor &table, const at::Tensor &cu_q, const at::Tensor &lens)
 {
@@ -235,7 +238,7 @@ int64_t paged_append_status(const at::Tensor &k, const at::Tensor &v, at::Tensor
                             const at::Tensor &cu_q, const at::Tensor &lens, const OptTensor &q, const OptTensor &q1, const OptTensor &q2,
                             const OptTensor &cos_tab, const OptTensor &sin_tab, int64_t const_pos, const OptTensor &status_word)
 {
-    if (!k.is_cuda()) return VQ_EDEVICE;
+    if (!k.is_cuda() || elsewhere(cos_tab, k) || elsewhere(sin_tab, k) || elsewhere(status_word, k)) return VQ_EDEVICE;
     const c10::cuda::CUDAGuard guard(k.device());
     VqPagedAppendArgs a{};
     a.kv = paged_kv(k1, v_pages, k3, k1_scale, v_scale, k3_scale, table, cu_q, lens);
@@ -259,7 +262,7 @@ int64_t paged_read_status(const at::Tensor &pool0, const OptTensor &scale0, at::
                           const OptTensor &out1, const OptTensor &pool2, const OptTensor &scale2, const OptTensor &out2, const at::Tensor &table,
                           const at::Tensor &start, const at::Tensor &lens, const OptTensor &status_word)
 {
-    if (!pool0.is_cuda()) return VQ_EDEVICE;
+    if (!pool0.is_cuda() || elsewhere(status_word, pool0)) return VQ_EDEVICE;
     const c10::cuda::CUDAGuard guard(pool0.device());
     VqPagedReadArgs a{};
     a.pool[0] = any_desc(pool0); a.pool[1] = any_desc(pool1); a.pool[2] = any_desc(pool2);
@@ -277,7 +280,7 @@ int64_t paged_attention_status(const at::Tensor &q1, const at::Tensor &q2, const
                                const OptTensor &vsum, const OptTensor &snap_table, int64_t window, int64_t max_q, double scale, at::Tensor out,
                                const OptTensor &workspace, const OptTensor &status_word)
 {
-    if (!q1.is_cuda()) return VQ_EDEVICE;
+    if (!q1.is_cuda() || elsewhere(workspace, q1) || elsewhere(status_word, q1)) return VQ_EDEVICE;
     const c10::cuda::CUDAGuard guard(q1.device());
     VqPagedAttentionArgs a{};
     a.kv = paged_kv(k1, v_pages, k3, k1_scale, v_scale, k3_scale, table, cu_q, lens);
