@@ -46,6 +46,8 @@ class PagedVectorQuantizedCache:
         assert max_length % page_size == 0 and max_length >= window_length
         self.window_length, self.page_size, self.max_length = window_length, page_size, max_length
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:      # the current one now, not that of a later call
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.codebooks = (codebook if codebook.dim() == 4 else codebook[:, None]).to(self.device, torch.float32).contiguous()   # [H,M,K,D]
         H, M, K, D = self.codebooks.shape
         assert M * K % BLOCK_SIZE == 0
