@@ -41,12 +41,24 @@ def _device_index(dev) -> int:
     return torch.cuda.current_device() if d.index is None else d.index
 
 
+def _capturing(dev) -> bool:
+    """The current stream of ``dev`` is being captured: what is launched now runs at a replay."""
+    if dev.type != "cuda":
+        return False
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def device_status_word(dev="cuda") -> torch.Tensor:
     """Per-device int32 word the kernels raise when they find a problem on the device (an expired bounded
-    wait, a position outside the RoPE tables, a code outside its codebook)."""
+    wait, a position outside the RoPE tables, a code outside its codebook).  A capture should not be the first to ask for it:
+    that graph's replays would clear it."""
     key = _device_index(dev)
     if key not in _STATUS:
-        _STATUS[key] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+        at = torch.device("cuda", key)
+        _STATUS[key] = torch.zeros(1, dtype=torch.int32, device=at)
+        if not torch.compiler.is_compiling() and not _capturing(at):
+            torch.cuda.current_stream(at).synchronize()     # kernels of every stream may raise it
     return _STATUS[key]
 
 
@@ -155,14 +167,6 @@ def build_aggregates(codes: torch.Tensor, v: torch.Tensor, K: int, nb: Optional[
 
 _ROPE_TABLES = {}
 _ROPE_REPLACED = []     # tables that a longer one replaced: a captured graph may still read them (together they are shorter than the longest)
-
-
-def _capturing(dev) -> bool:
-    """The current stream of ``dev`` is being captured: what is launched now runs at a replay."""
-    if dev.type != "cuda":
-        return False
-    with torch.cuda.device(dev):
-        return torch.cuda.is_current_stream_capturing()
 
 
 def rope_tables(n_pos: int, dim: int, device, base: float = 10000.0):
