@@ -35,6 +35,14 @@ def test_a_second_stream_may_read_a_table_that_the_first_has_just_filled(api):
     a, b = torch.cuda.Stream(), torch.cuda.Stream()
     (p1, first), (p2, second) = _append(api), _append(api)
     busy = torch.randn(8192, 8192, device="cuda")
+    for stream, call in ((a, first), (b, second)):            # kernels are loaded, memory is there
+        with torch.cuda.stream(stream):
+            call()
+            busy @ busy
+    torch.cuda.synchronize()
+    api._ROPE_TABLES.clear()
+    for p in (p1, p2):
+        p.k1.zero_()
     torch.cuda.synchronize()
     with torch.cuda.stream(a):
         for _ in range(5):
