@@ -408,7 +408,7 @@ int vqattn_paged_read(const VqPagedReadArgs *args, void *stream);
  * workspace: NULL, or vqattn_paged_attention_workspace_bytes(...) bytes of device memory, 256-byte aligned, contents arbitrary before and after.
  * With i8 pools and chunks that are long for their windows every key is needed by many query tiles; its codes are then turned into 16-bit
  * floats once, in the workspace, instead of once per tile.  Same results.  The size is 0 where none would be used; one that is too small is not
- * used either.
+ * used either.  It has room for three pools, with raw keys or without.
  */
 typedef struct VqPagedAttentionArgs {
     VqPagedKv kv;

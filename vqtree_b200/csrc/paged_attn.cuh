@@ -128,7 +128,7 @@ inline int64_t paged_blocks(int64_t S, int64_t T, int64_t window) { return S * (
 // 8-bit rows: converting a block once per call pays where its keys meet several query tiles.  Measured, us, first / on the way, 32 query heads over 8,
 // D = 128, MK1024, window 2048 (512), new tokens per sequence: 2 tiles each, 8 sequences 131 / 160 (80 / 83); 4 tiles, 8 sequences 176 / 238 (109 /
 // 122), 24 sequences 414 / 561 (255 / 291); 16 tiles, 2 sequences 118 / 166 (77 / 88).  The line is at four: below it the workspace grows
-// faster than what it saves.
+// faster than what it saves.  It goes by the average, known without the lengths: a long chunk among many single tokens is converted on the way.
 inline bool convert_first(int64_t S, int64_t T, int64_t G) { return T * G >= 4 * kBlock * S; }
 
 constexpr int kFewRows = 32;     // query rows (tokens times query heads of a kv head) of the few-token kernel

@@ -1,6 +1,6 @@
 // Writing new tokens into the pages of a cache and reading rows back.
 //
-// Append: every token brings Hkv keys, Hkv values and Hq queries.  A group of lanes owns one of these rows - each lane 16 bytes of the
+// Append: every token brings Hkv keys, Hkv values and Hq queries.  A group of lanes owns one to four of these rows - each lane 16 bytes of the
 // first half and the matching 16 of the second, so a rotation needs no exchange - and finds the token's sequence by bisecting cu_q
 // (every lane of a token reads the same words).  8-bit rows: scale = max|x| * (1/127), code = rint(x * (1/scale)); the maximum is an
 // exchange inside the group, x is the fp32 rotation (quantising a rotation already rounded to 16 bits would round twice), and every
@@ -88,7 +88,7 @@ struct AppendParams {
 };
 
 // A group of lanes takes U heads of one kind - keys, values or queries - of a token: they share the look-ups and the table's row, which is twice a
-// 16-bit row.
+// 16-bit row.  Three CTAs of an SM leave 80 registers a thread: four heads of 16 bits on their way to 8 spill 344 bytes there (stored; 908 loaded).
 template <typename T, typename KV, int D, int U>
 __global__ void __launch_bounds__(256, sizeof(KV) == 1 ? 3 : 2) paged_append_kernel(const AppendParams p)
 {
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(256, 8) paged_read_kernel(const ReadParams p)
 // Rows per thread: several where there are many CTAs anyway, one where there are few.  Measured with several / with one, us: appending 2048 tokens
 // of 32 kv heads, 16 bits 29.8 / 32.5; second turns of 12 sequences, 8 bits, with reading them back 120 / 132; reading 16 windows of 2303 rows,
 // 32 heads, 8 bits to half (915 MB) 162 / 215.
-constexpr int kManyCtas = 148 * 8;
+constexpr int kManyCtas = 148 * 8;      // eight for each SM of the chip
 
 template <typename T, typename KV, int D>
 static int launch_append(AppendParams &p, cudaStream_t stream)

@@ -8,13 +8,15 @@
 // Which rows a tile has is read on the device (one warp counts the tiles of 32 sequences at a time), so a captured call may be
 // replayed with other lengths.
 //   16-bit rows   a thread loads pages by TMA, 128 / P boxes a tile, into a ring of four 32 KB slots.
-//   8-bit rows    where a block of keys meets four query tiles or more and the caller gave a workspace, a kernel before this one turns every
-//                 block's codes into 16-bit floats (exact) there once, with a factor per row beside them, and this one loads tiles of it as above.
+//   8-bit rows    where a call's sequences bring four query tiles each, on the average, and the caller gave a workspace, a kernel before this one turns
+//                 every block's codes into 16-bit floats (exact) there once, with a factor per row beside them, and this one loads tiles of it as above.
 //                 Otherwise codes arrive by TMA in two staging tiles and three warps convert them into a ring of three slots, in the swizzled layout
 //                 the tensor cores read.  The scales of a step's keys multiply scores, those of its values weights, per column.
 // Bound by the hand-offs between the softmax warps and the tensor pipe, as the prefill kernel is.  Measured: 4096 tokens at
 // context 32768, 32 heads, D = 128, MK1024, W1024, bf16: 252 us, 560 TFLOP/s.  Six second turns of 700 tokens and fewer, 32 query heads over 8, 8-bit rows:
 // 203 us, 20 of them converting (converted on the way 283, by plain loads one tile ahead 410; 16-bit rows 162).
+// The softmax over 8-bit rows spills 112 - 188 bytes a thread (128 registers; scores, factors of keys and of values).
+// Weights are rounded to 16 bits before they meet their values, as in the prefill kernels: P is an operand of the tensor pipe.  Their sum is not.
 // Rows behind a sequence's end hold anything: their scores are masked and their value rows are zeroed before the product.
 #include "codes8.cuh"
 #include "paged_attn.cuh"

@@ -5,7 +5,7 @@
 // rows x 4 keys, then owns 2 rows x D / 8 columns of the sums - the same two rows, so maximum, denominator and rescaling stay inside
 // groups of eight lanes.  The next step's rows are on their way to registers meanwhile.  Where the tiles do not fill the chip, the CTAs
 // of a cluster share a tile's steps and merge their sums through distributed shared memory.
-// One warp per query row, each lane a key (the first version): 220 us for 290 tokens of 8 heads of 64 over 512 codes and a window of 128;
+// One warp per query row, each lane a key (the first version): 220 us for 178 tokens of 8 heads of 64 over 512 codes and a window of 128;
 // this: 47 us.
 #include <cooperative_groups.h>
 

@@ -5,7 +5,7 @@
 // matrix product only has to keep out of its way: mma.sync with the KEYS on the M axis (16 per instruction) and 8 query rows on N, for
 // which a tile of 128 rows of tcgen05 would be nearly empty.  A warp takes steps of 16 keys (32 of 8-bit rows) and keeps its own online
 // softmax: no barrier in the loop.
-//   - A warp's keys and values arrive by TMA, 16 rows a box, in a FIFO of its own, filled by one lane of a fifth warp (no CTA barrier).  Both products may
+//   - A warp's keys and values arrive by TMA, 16 rows a box, in a FIFO of its own, filled by one more warp of the CTA (no CTA barrier).  Both products may
 //     permute their reduction index: a thread reads 16 contiguous bytes of a swizzled key row, which hold its operands of several k-steps, and q
 //     is read in the same order.  Values enter as V^T (D on M): pairs of keys are interleaved by byte permutes.
 //   - S^T (keys x rows) becomes the B operand of the second product by movmatrix, 8 x 8 at a time.
@@ -13,7 +13,9 @@
 //     the range of a half by a power of two (its largest element to 2^10 .. 2^11; elements above 2^-24 of it stay exact).  Weights carry the
 //     scale of their value.
 //   - Counts multiply the weights of codes in the denominator; codes without members are excluded.
-// One unit = (sequence, block of positions, kv head); its steps are dealt out to the warps of a cluster of 1 - 8 CTAs, which merge their
+//   - Weights are rounded to 16 bits before they meet their values, as the matrix instruction wants both in one type (and as the prefill kernels do);
+//     their sum is not.  It costs as much as rounding the output: 2.3e-3 of the result (bf16, against 64 bits) where that alone is 1.7e-3.
+// One unit = (sequence, block of positions, kv head); its steps are dealt out to the warps of a cluster of 1 - 16 CTAs, which merge their
 // partial sums through distributed shared memory: no workspace, no second launch, the same order of additions every time.
 #include <cooperative_groups.h>
 #include <type_traits>
@@ -57,7 +59,8 @@ struct FewCfg {
     // Up to 8 rows: 64 sequences of 8 kv heads, 16 bits, 3 warps x 2 stages x 4 CTAs / 4 x 3 x 2: 136 / 152 (all 512 units run at once); 16
     // sequences of 32 heads, 8 bits, 5 x 2 x 2 / 4 x 3 x 2 / 3 x 2 x 3: 77 / 87 / 104.  16 rows, 32 sequences of 8 heads, D = 128, 3 x 3 x 2 /
     // 4 x 3 x 2 (8 bits: 5 x 3 x 2): 46 / 50, 8 bits 64 / 90 (which spills); D = 64: 42 / 38, 45 / 34.  32 rows, 7 x 2 x 1 / 4 x 3 x 1: 94 / 123,
-    // 8 bits 125 / 144, D = 64 68 / 74.
+    // 8 bits 125 / 144, D = 64 68 / 74.  With D = 128 that form spills 0.4 KB a thread (8 bits: 1 KB): four column tiles of sums, their operands
+    // and a step's rows are more than 255 registers.
     static constexpr int kWarps = NT == 1 ? (Q8 ? 5 : 3) : NT == 2 ? (D == 128 ? 3 : Q8 ? 5 : 4) : 7, kThreads = (kWarps + 1) * 32;
     static constexpr int kStages = NT == 2 ? 3 : 2;
     static constexpr int kCtas = NT == 1 ? (Q8 ? 2 : 4) : NT == 2 ? 2 : 1;
@@ -87,7 +90,7 @@ struct FewSteps {
 template <typename T, bool Q8, int D, int NT>
 __global__ void __launch_bounds__(FewCfg<T, Q8, D, NT>::kThreads, FewCfg<T, Q8, D, NT>::kCtas)
 paged_few_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constant__ CUtensorMap tm_k3, const __grid_constant__ CUtensorMap tm_v,
-                 const __grid_constant__ CUtensorMap tm_cb, const __grid_constant__ CUtensorMap tm_vs, const PagedAttnParams p, int groups, int nsplit)
+                 const __grid_constant__ CUtensorMap tm_cb, const __grid_constant__ CUtensorMap tm_vs, const PagedAttnParams p, int nsplit)
 {
     using C = FewCfg<T, Q8, D, NT>;
     using M = Mma16816<T>;
@@ -761,7 +764,7 @@ static int launch_few(const PagedAttnParams &p, cudaStream_t stream)
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kern, k1, k3, v, cb, vs, p, groups, nsplit) == cudaSuccess ? launch_status() : (cudaGetLastError(), VQ_ELAUNCH);
+    return cudaLaunchKernelEx(&cfg, kern, k1, k3, v, cb, vs, p, nsplit) == cudaSuccess ? launch_status() : (cudaGetLastError(), VQ_ELAUNCH);
 }
 
 template <typename T, bool Q8, int D>

@@ -40,7 +40,7 @@ __device__ __forceinline__ float t4_max(const uint32_t (&r)[64])
     return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 
-// P = exp2(S * scale - m) of the 64 scores, packed 16-bit floats written to the 32 columns at p_addr; returns
+// P = exp2(S * scale - m) of the 64 scores, packed 16-bit floats (the tensor pipe's operands) written to the 32 columns at p_addr; returns
 // sum plus the (FAR: count-weighted) sums of the two halves, one after the other.
 template <bool FAR, bool F16>
 __device__ __forceinline__ float t4_exp(const uint32_t (&r)[64], uint32_t p_addr, const float *cw, float scale_log2, float neg_m, float sum)
