@@ -6,7 +6,7 @@ from tests import fake_paged
 from tests.paged_scenarios import whole_sequences
 from vqtree_b200 import api
 from vqtree_b200.attn_vq import VectorQuantizedReRoPECache
-from vqtree_b200.paged_cache import OutOfPages, PagedVectorQuantizedCache
+from vqtree_b200.paged_cache import OutOfPages, PagedVectorQuantizedCache, _runs
 
 W, D, M, K = 128, 64, 1, 128
 
@@ -131,3 +131,23 @@ def test_adopt_refuses_another_codebook_and_another_rotary_base():
         cache.adopt(_dense(150, cb, batch=1))
         half = _cache(cb.half().float())
         half.adopt(_dense(150, cb.half(), batch=1))
+
+
+def test_a_failed_call_of_many_sequences_restores_each(monkeypatch):
+    """Blocks leave in three of four slots, two of them neighbours; sums, counts and boundaries are those of before, bit for bit."""
+    assert [(s.start, s.stop) for s in _runs({7, 1, 3, 2})] == [(1, 4), (7, 8)] and _runs(set()) == []
+    cb = torch.randn(1, M, K, D)
+    n = (250, 250, 10, 250)
+    with fake_paged.installed():
+        cache = _cache(cb, max_sequences=4, num_pages=128)
+        sids = [cache.add_sequence() for _ in n]
+        cache.attend(sids, n, *(torch.randn(sum(n), 1, D) for _ in range(3)))
+        held = [t.clone() for t in (cache.cnt, cache.vsum32, cache.vsum)]
+        marks = [(s.n, s.bd, s.first, list(s.pages)) for s in cache._sequences.values()]
+        with monkeypatch.context() as m:
+            _fail_once(m, "paged_attention", 1)
+            with pytest.raises(RuntimeError):
+                cache.attend(sids, [150] * 4, *(torch.randn(600, 1, D) for _ in range(3)))
+        for t, old in zip((cache.cnt, cache.vsum32, cache.vsum), held):
+            assert torch.equal(t[:4], old[:4])
+        assert [(s.n, s.bd, s.first, list(s.pages)) for s in cache._sequences.values()] == marks

@@ -31,6 +31,17 @@ class _Sequence:
         self.pages: List[int] = []     # pages of columns first, first + 1, ...
 
 
+def _runs(numbers) -> List[slice]:
+    """Slices of neighbouring numbers: few large copies instead of many."""
+    out = []
+    for x in sorted(numbers):
+        if out and out[-1].stop == x:
+            out[-1] = slice(out[-1].start, x + 1)
+        else:
+            out.append(slice(x, x + 1))
+    return out
+
+
 class PagedVectorQuantizedCache:
     """window_length, codebook ([H,C,D] or [H,M,K,D]), rope_base: as VectorQuantizedReRoPECache.  num_pages pages of page_size (16, 32, 64
     or 128) tokens are shared by the sequences; a sequence needs those of its window, up to window + 128 tokens and the chunk in flight.
@@ -156,10 +167,9 @@ class PagedVectorQuantizedCache:
             del seq.pages[pages:]
             seq.bd = bd
         for slots, cnt, vsum32 in saved:
-            for i, s in enumerate(slots):
-                self.cnt[s].copy_(cnt[i])
-                self.vsum32[s].copy_(vsum32[i])
-                self.vsum[s].copy_(vsum32[i])
+            self.cnt[slots].copy_(cnt)
+            self.vsum32[slots].copy_(vsum32)
+            self.vsum[slots].copy_(vsum32)
 
     def _upload(self, numbers) -> torch.Tensor:
         t = torch.tensor(numbers, dtype=torch.int32)
@@ -208,12 +218,12 @@ class PagedVectorQuantizedCache:
         if leaving:
             kv = self.pages
             pair = [(kv.k3, kv.k3_scale) if self.rerope else (kv.k1, kv.k1_scale), (kv.v, kv.v_scale)]
-            slots = sorted({seqs[x].slot for x, _ in leaving})
-            idx = self._upload([x for x, _ in leaving] + [b for _, b in leaving] + slots)
-            which, starts, rows = idx[: len(leaving)], idx[len(leaving): 2 * len(leaving)], idx[2 * len(leaving):]
+            idx = self._upload([x for x, _ in leaving] + [b for _, b in leaving])
+            which, starts = idx[: len(leaving)], idx[len(leaving):]
             raw, val = api.paged_read(pair, table.index_select(0, which), starts, seq_lens.index_select(0, which), BLOCK_SIZE, self.dtype)
             codes = api.assign_codes(raw, self.codebooks)
-            saved.append((slots, self.cnt.index_select(0, rows), self.vsum32.index_select(0, rows)))
+            for slots in _runs({seqs[x].slot for x, _ in leaving}):
+                saved.append((slots, self.cnt[slots].clone(), self.vsum32[slots].clone()))
         K, spare, at = self.codebooks.shape[2], self.max_sequences, 0
         for x, (seq, (b0, b1)) in enumerate(zip(seqs, plan)):
             s = seq.slot
