@@ -43,7 +43,7 @@ def _device_index(dev) -> int:
 
 def _capturing(dev) -> bool:
     """The current stream of ``dev`` is being captured: what is launched now runs at a replay."""
-    if dev.type != "cuda":
+    if dev.type != "cuda" or torch.compiler.is_compiling():
         return False
     with torch.cuda.device(dev):
         return torch.cuda.is_current_stream_capturing()
@@ -475,7 +475,8 @@ def store_window(k1, k3, v, k1_win, k3_win, v_win, vsum_f32=None, vsum_act=None)
 class PagedKV(NamedTuple):
     """The pools of a paged cache: rotated keys, values and (ReRoPE) raw keys [NP,Hkv,P,D], pages of P = 16, 32, 64 or 128 tokens, in
     the activations' type or int8 with a scale per row [NP,Hkv,P] f32.  k3 None: plain rotary positions.  Any strides that are
-    multiples of 16 bytes with a contiguous last dim ([NP,P,Hkv,D] storage viewed as [NP,Hkv,P,D], a slice of a pool of all layers)."""
+    multiples of 16 bytes with a contiguous last dim ([NP,P,Hkv,D] storage viewed as [NP,Hkv,P,D], a slice of a pool of all layers); none is
+    0 (an expanded tensor) where rows are written or attended to."""
     k1: torch.Tensor
     v: torch.Tensor
     k3: Optional[torch.Tensor] = None
@@ -575,7 +576,7 @@ def paged_attention(q1: torch.Tensor, q2: torch.Tensor, pages: PagedKV, block_ta
     """Attention of the new tokens of S sequences over their pages (which hold them already): every row is what the same row of
     ``vq_attention_prefill`` over the whole sequence is defined to be.
 
-    q1, q2 [T,Hq,D] (q2 may be q1) packed by cu_q; block_table, cu_q, seq_lens as in ``paged_append``; max_q: an upper bound of the new
+    q1, q2 [T,Hq,D] (q2 may be q1; not expanded) packed by cu_q; block_table, cu_q, seq_lens as in ``paged_append``; max_q: an upper bound of the new
     tokens of one sequence.  codebook [Hkv,MK,D], cnt [NS,Hkv,MK] f32, vsum [NS,Hkv,MK,D], snap_table int32 [S,MS]: keys before the
     boundary b of a query count through snapshot ``snap_table[s, b // 128 % MS]`` (None: the local part only).  Returns [T,Hq,D]; rows
     from cu_q[S] on are left as they are.
