@@ -128,3 +128,27 @@ def test_a_layer_of_real_size_equals_the_dense_prefill(api, hq, hkv, M):
         at += n
     assert at == L
     api.check_status()
+
+
+@pytest.mark.parametrize("dtype,q8", [(BF16, True), (F16, False), (F32, False)])
+def test_a_call_that_fails_half_way_is_undone_to_the_bit(api, monkeypatch, dtype, q8):
+    from vqtree_b200.paged_cache import PagedVectorQuantizedCache
+    g = torch.Generator(device="cuda").manual_seed(9)
+    cb = torch.randn(2, 2, 128, 64, generator=g, device="cuda") * 0.35
+    rows = [torch.randn(1500, h, 64, generator=g, device="cuda").to(dtype) for h in (4, 2, 2)]
+    part = lambda a, b: [x[a:b] for x in rows]
+    made = []
+    for fails in (False, True):
+        cache = PagedVectorQuantizedCache(128, cb, 96, 3, page_size=32, dtype=dtype, quantized=q8, max_length=1024)
+        sids = [cache.add_sequence() for _ in range(3)]
+        cache.attend(sids, [400, 100, 350], *part(0, 850))
+        if fails:
+            held, free = [t[:3].clone() for t in (cache.cnt, cache.vsum32, cache.vsum)], cache.free_pages
+            with monkeypatch.context() as m:
+                m.setattr(api, "paged_attention", lambda *a, **k: (_ for _ in ()).throw(RuntimeError("out of memory")))
+                with pytest.raises(RuntimeError, match="out of memory"):
+                    cache.attend(sids, [300, 50, 300], *part(850, 1500))
+            assert all(torch.equal(t[:3], old) for t, old in zip((cache.cnt, cache.vsum32, cache.vsum), held)) and cache.free_pages == free
+        made.append(cache.attend(sids, [300, 50, 300], *part(850, 1500)))
+    assert torch.equal(*made)
+    api.check_status()
